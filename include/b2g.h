@@ -12,8 +12,8 @@
  *     11 = Q3_K, 12 = Q4_K, 13 = Q5_K, 14 = Q6_K, 16 = IQ2_XXS, 22 = IQ2_S).
  *   - `status` (nullable) is a device int32 the kernels write a non-zero code into when a bounded
  *     device-side wait runs out (1xx-4xx) or an input is out of range (901 receive buffer too small, 902 label
- *     outside the vocabulary, 903 expert id outside [0, E), 904 expert offsets beyond the row count); it is
- *     never written on a healthy run and only the first code is kept.
+ *     outside the vocabulary, 903 expert id outside [0, E), 904 expert offsets beyond the row count, 905 sequence offsets
+ *     that decrease or leave the tokens); it is never written on a healthy run and only the first code is kept.
  *
  * Each entry names the reference interface it stands in for (file:line in
  * woct0rdho/transformers5-qwen3.5-recipe).  The reference reaches these through the third-party
@@ -118,6 +118,53 @@ B2G_API int b2g_cross_entropy_inplace(void* logits, int64_t ld, const int64_t* t
                               int64_t rows, int64_t V, int64_t ignore_index, const int64_t* count, int mean, int* status,
                               void* stream);
 
+/* Log-probabilities of the target tokens of rows of logits [rows, V] (row pitch ld elements; logits_dtype 0 = bf16, 1 = fp32):
+ *   logp[row] = z[target] / temperature - log sum_i exp(z[i] / temperature)
+ * in fp32 or fp64 (logp_dtype 0 | 1: sums over long sequences keep their digits in fp64).  stats[row] (4 floats, 16-byte
+ * aligned) = {max z, 1 / sum_i exp((z[i] - max z) / temperature), 1 - p of the target, log-sum-exp} is what the gradient reads.  A row whose target is
+ * ignore_index gets logp 0 and its logits are not looked at; a target outside [0, V) is reported (status 902) and treated the
+ * same way.  -inf logits have probability zero; a live row that holds NaN or +inf, or nothing but -inf, gives NaN.
+ * This entry has no counterpart in the reference (its losses are supervised only). */
+B2G_API int b2g_token_logprobs(const void* logits, int64_t ld, int logits_dtype, const int64_t* target, void* logp, int logp_dtype, float* stats,
+                       int64_t rows, int64_t V, float temperature, int64_t ignore_index, int* status, void* stream);
+
+/* grad_logits[row, i] = grad_logp[row] * ([i == target] - softmax_i) / temperature in the logits' type (grad_logp in fp32 or fp64), 0 for rows without a
+ * live target and for rows whose grad_logp is 0.  grad_logits may be the logits themselves (same pointer, same pitch).
+ * This entry has no counterpart in the reference. */
+B2G_API int b2g_token_logprobs_bwd(const void* logits, int64_t ld, int logits_dtype, const int64_t* target, const float* stats,
+                           const void* grad_logp, int logp_dtype, void* grad_logits, int64_t ld_grad, int64_t rows, int64_t V, float temperature,
+                           int64_t ignore_index, void* stream);
+
+/* Clipped policy loss with a KL term, loss and cotangent of the logits in one call.  With r = exp(logp - old_logp) (1 when
+ * old_logp is null), d = ref_logp - logp, A = advantage and w = weight (1 when null):
+ *   loss = w * ( -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * kl ),   kl = e^d - d - 1 (0 without ref_logp)
+ *   grad_logits = (d loss / d logp) * (onehot - softmax) / temperature   in the logits' type, possibly in place.
+ * A row takes part when its target is in [0, V) and its weight is not 0; every other row gives zeros in all four outputs and
+ * nothing else of it is read.  A target that is neither ignore_index nor in [0, V) is reported (status 902).
+ * This entry has no counterpart in the reference. */
+B2G_API int b2g_policy_loss(const void* logits, int64_t ld, int logits_dtype, const int64_t* target, const float* advantage,
+                    const float* old_logp, const float* ref_logp, const float* weight, float clip_low, float clip_high, float kl_coef,
+                    float temperature, float* loss, float* logp, float* kl, void* grad_logits, int64_t ld_grad, int64_t rows, int64_t V,
+                    int64_t ignore_index, int* status, void* stream);
+
+/* Preference loss on pairs of sequences.  logp (fp32 or fp64: logp_dtype 0 | 1), ref_logp (fp32, nullable) and target (nullable) hold N tokens; sequence s is the
+ * tokens [offsets[s], offsets[s + 1]) and offsets has 2 * pairs + 1 entries: the `pairs` chosen sequences, then the rejected
+ * ones in the same order.  L_s = sum (average: mean) of logp - ref_logp over the tokens whose target is not ignore_index, an
+ * empty sequence gives 0; with gap = L_chosen - L_rejected
+ *   loss_type 0: loss = -(1 - label_smoothing) log sigmoid(beta gap) - label_smoothing log sigmoid(-beta gap)
+ *   loss_type 1: loss = (gap - 1 / (2 beta))^2
+ * chosen / rejected = beta * L_s (rewards, [pairs]); coef[2 * pairs] = d loss / d logp of a counted token of each sequence.
+ * Offsets that decrease or leave [0, N] are brought into range and reported (status 905).  This entry has no counterpart in the reference. */
+B2G_API int b2g_preference_loss(const void* logp, int logp_dtype, const float* ref_logp, const int64_t* target, const int64_t* offsets, int64_t N,
+                        int64_t pairs, int64_t ignore_index, float beta, float label_smoothing, int loss_type, int average, float* loss, float* chosen,
+                        float* rejected, float* coef, int* status, void* stream);
+
+/* grad_logp[i] = grad_loss[pair] * coef[sequence] for counted tokens, 0 for ignored tokens and tokens of no sequence,
+ * in fp32 or fp64 (logp_dtype).
+ * This entry has no counterpart in the reference. */
+B2G_API int b2g_preference_loss_bwd(const float* grad_loss, const float* coef, const int64_t* target, const int64_t* offsets, void* grad_logp,
+                            int logp_dtype, int64_t N, int64_t pairs, int64_t ignore_index, void* stream);
+
 /* Skinny projection onto the LoRA rank: P[M,r] = X[M,C] . W^T with W given as [r,C] (w_is_cr = 0,
  * lora_A for X.A^T) or as [C,r] (w_is_cr = 1, lora_B for dY.B); r <= 16.
  * Writes out_plain[M,16] = bf16(P) and out_scaled[M,16] = bf16(scale*P), zero in columns >= r
@@ -159,6 +206,27 @@ B2G_API int b2g_lora_wgrad_static(const void* s, const void* t, float scale, voi
  * Replaces router_topk_indices / _router_topk_kernel (fast_moe_ranking.py:166-270). */
 B2G_API int b2g_router_topk(const void* logits, int logits_dtype, const float* bias, int score_fn, int64_t* indices,
                     int64_t T, int E, int top_k, void* stream);
+
+/* Routing to experts: weights[T, top_k] (fp32) and indices[T, top_k] (best first) from logits [T, E] (row pitch ld elements;
+ * logits_dtype 0 = bf16, 1 = fp32).  With l the logits, b = bias[E] (nullable, fp32, enters the choice only):
+ *   s = softmax(l) (score_fn 0) | sigmoid(l) (1) | sqrt(log(1 + e^l)) (2);   c = s + b (order of l without a bias)
+ *   the `top_groups` of `groups` equal groups of experts with the largest sum of their group_experts (1 | 2) best c stay;
+ *   the top_k experts of largest c in them are chosen; ties go to the lower group and the lower expert id;
+ *   weights = scaling * s_j / (sum of the chosen s + 1e-20) when renormalize, else scaling * s_j.
+ * Renormalised softmax weights are the softmax of the chosen logits.  c is compared in 64 bits.  -inf logits have score 0
+ * (0 weight, also where a whole row is -inf); NaN is chosen last and gives NaN weights; indices are distinct and in range
+ * whatever the logits hold.  1 <= E <= 512, top_k <= 32, groups <= 32, top_k <= top_groups * E / groups.
+ * Covers what _deepseek_topk_router_forward and _qwen_router_forward do around the selection (fast_moe_ranking.py:273-316). */
+B2G_API int b2g_route_experts(const void* logits, int64_t ld, int logits_dtype, const float* bias, int score_fn, int groups, int top_groups,
+                      int group_experts, int renormalize, float scaling, float* weights, int64_t* indices, int64_t T, int E,
+                      int top_k, void* stream);
+
+/* Gradient of the weights with respect to the logits: grad_logits [T, E] contiguous, in the logits' type, from grad_weights,
+ * weights and indices [T, top_k] of b2g_route_experts.  Every entry is written; ids outside [0, E) are skipped.
+ * Covers the autograd of the gather / softmax / normalisation of fast_moe_ranking.py:273-316. */
+B2G_API int b2g_route_experts_bwd(const void* logits, int64_t ld, int logits_dtype, const float* grad_weights, const float* weights,
+                          const int64_t* indices, int score_fn, int renormalize, float scaling, void* grad_logits, int64_t T, int E,
+                          int top_k, void* stream);
 
 /* Stable counting sort of the flat [T*top_k] expert ids.  idx_dtype: 0 = int32, 1 = int64.
  * Outputs: sorted_expert[R], perm[R], inv_perm[R] (int64), group_sizes[E], offsets[E] (int32,

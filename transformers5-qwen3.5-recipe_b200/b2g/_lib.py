@@ -24,12 +24,20 @@ SIGNATURES = {
     "b2g_fixed_grouped_fwd": (_i32, [_i32, _vp, _vp, _vp, _i64, _i32, _i64, _i64, _vp, _vp]),
     "b2g_fixed_grouped_dgrad": (_i32, [_i32, _vp, _vp, _vp, _i64, _i32, _i64, _i64, _vp, _vp]),
     "b2g_cross_entropy_inplace": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _vp]),
+    "b2g_token_logprobs": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _vp, _i64, _i64, _f32, _i64, _vp, _vp]),
+    "b2g_token_logprobs_bwd": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _f32, _i64, _vp]),
+    "b2g_policy_loss": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp,
+                               _vp]),
+    "b2g_preference_loss": (_i32, [_vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b2g_preference_loss_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp]),
     "b2g_lora_down": (_i32, [_vp, _vp, _i32, _f32, _vp, _vp, _i64, _i64, _i32, _vp]),
     "b2g_lora_wgrad_workspace_bytes": (_i64, [_i64, _i64]),
     "b2g_lora_wgrad": (_i32, [_vp, _vp, _f32, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _vp]),
     "b2g_lora_wgrad_static_max_bytes": (_i64, []),
     "b2g_lora_wgrad_static": (_i32, [_vp, _vp, _f32, _vp, _i32, _i64, _i64, _i32, _vp]),
     "b2g_router_topk": (_i32, [_vp, _i32, _vp, _i32, _vp, _i64, _i32, _i32, _vp]),
+    "b2g_route_experts": (_i32, [_vp, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _vp, _i64, _i32, _i32, _vp]),
+    "b2g_route_experts_bwd": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _f32, _vp, _i64, _i32, _i32, _vp]),
     "b2g_route_plan_workspace_bytes": (_i64, [_i64, _i32]),
     "b2g_route_plan": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp]),
     "b2g_route_gather": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _vp]),
@@ -85,6 +93,8 @@ KERNELS_PER_CALL = {
     "b2g_router_topk": 1, "b2g_route_plan": 4, "b2g_route_gather": 1, "b2g_route_gather_bwd": 1, "b2g_route_combine": 1,
     "b2g_route_combine_bwd": 1, "b2g_grouped_schedule": 1, "b2g_grouped_fwd": 1, "b2g_grouped_dgrad": 1,
     "b2g_grouped_lora_down": 1, "b2g_grouped_lora_wgrad": 1, "b2g_grouped_lora_up": 1, "b2g_ep_scatter_rows": 1, "b2g_ep_return_rows": 1, "b2g_ep_peer_plan": 1, "b2g_swiglu_fwd": 1, "b2g_swiglu_bwd": 1,
+    "b2g_route_experts": 1, "b2g_route_experts_bwd": 1, "b2g_token_logprobs": 1, "b2g_token_logprobs_bwd": 1, "b2g_policy_loss": 1,
+    "b2g_preference_loss": 1, "b2g_preference_loss_bwd": 1,
     "b2g_cross_entropy_inplace": 1, "b2g_fixed_grouped_fwd": 8, "b2g_fixed_grouped_dgrad": 8,      # one launch per group (eight in the DeepSeek layout)
 }
 COUNT_LAUNCHES = False

@@ -10,6 +10,10 @@ Grouped path
     ``grouped_mmq`` / ``grouped_mmq_pair`` and their ``*_grad_input`` (``fast_moe_lora.py:221-262,339-375``)
     ``grouped_lora_experts``        the expert block of ``fast_moe_lora.py:720-763`` (pair product, LoRA,
                                     SwiGLU, down product, LoRA) with a hand-written backward
+Routing and losses
+    ``route_experts``               expert weights and ids from router logits (groups, balance bias)
+    ``token_logprobs``              log-probabilities of target tokens from rows of logits
+    ``preference_loss``             paired sequence log-ratios
 
 Packed payloads are frozen: none of these ever produces a gradient for them.
 """
@@ -386,3 +390,82 @@ def grouped_lora_experts(sel, gate_payload, up_payload, down_payload, quant_gate
     return _GroupedLoraExperts.apply(sel, gate_payload, up_payload, down_payload, quant_gate_up, quant_down, inter_dim,
                                      expert_indices, expert_offsets, offsets_full, gate_up_a, gate_up_b, down_a, down_b,
                                      scaling, swiglu_limit)
+
+
+# ---- routing and post-training losses -----------------------------------------------------------
+def _first_order_only(what: str) -> None:
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} does not support higher-order gradients")
+
+
+class _RouteExperts(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, score_function, groups, top_groups, group_experts, renormalize, scaling_factor):
+        weights, indices = ops.route_experts(logits, top_k, bias, score_function, groups, top_groups, group_experts, renormalize, scaling_factor)
+        ctx.save_for_backward(logits, weights, indices)
+        ctx.settings = (score_function, renormalize, scaling_factor)
+        ctx.mark_non_differentiable(indices)
+        return weights, indices
+
+    @staticmethod
+    def backward(ctx, grad_weights, _grad_indices):
+        _first_order_only("route_experts")
+        logits, weights, indices = ctx.saved_tensors
+        return (ops.route_experts_bwd(grad_weights.contiguous(), logits, weights, indices, *ctx.settings),) + (None,) * 8
+
+
+def route_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor] = None, score_function: str = "softmax", groups: int = 1,
+                  top_groups: int = 1, group_experts: int = 1, renormalize: bool = True, scaling_factor: float = 1.0):
+    """``ops.route_experts`` whose weights carry the gradient to the logits (the bias enters the choice only and gets none)."""
+    if not (logits.requires_grad and torch.is_grad_enabled()):
+        return ops.route_experts(logits, top_k, bias, score_function, groups, top_groups, group_experts, renormalize, scaling_factor)
+    return _RouteExperts.apply(logits, bias, top_k, score_function, groups, top_groups, group_experts, renormalize, scaling_factor)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, target, temperature, ignore_index, dtype):
+        logp, stats = ops.token_logprobs(logits, target, temperature, ignore_index, dtype)
+        ctx.save_for_backward(logits, target, stats)
+        ctx.settings = (temperature, ignore_index)
+        return logp
+
+    @staticmethod
+    def backward(ctx, grad_logp):
+        _first_order_only("token_logprobs")
+        logits, target, stats = ctx.saved_tensors
+        return ops.token_logprobs_bwd(grad_logp.contiguous(), logits, target, stats, *ctx.settings), None, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, target: torch.Tensor, temperature: float = 1.0, ignore_index: int = -100,
+                   dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Log-probabilities ``[rows]`` (fp32 or fp64) of the targets under ``softmax(logits / temperature)``, 0 where the target is
+    ``ignore_index``; the logits stay as they are and get their gradient in their own type.  Take fp64 where the values are
+    summed over a sequence, as ``preference_loss`` does."""
+    if not (logits.requires_grad and torch.is_grad_enabled()):
+        return ops.token_logprobs(logits, target, temperature, ignore_index, dtype)[0]
+    return _TokenLogprobs.apply(logits, target, temperature, ignore_index, dtype)
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logp, offsets, ref_logp, beta, label_smoothing, loss_type, average, target, ignore_index):
+        loss, chosen, rejected, coef = ops.preference_loss(logp, offsets, ref_logp, beta, label_smoothing, loss_type, average, target, ignore_index)
+        ctx.save_for_backward(coef, offsets, target)
+        ctx.num_tokens, ctx.ignore_index, ctx.dtype = logp.shape[0], ignore_index, logp.dtype
+        ctx.mark_non_differentiable(chosen, rejected)
+        return loss, chosen, rejected
+
+    @staticmethod
+    def backward(ctx, grad_loss, _grad_chosen, _grad_rejected):
+        _first_order_only("preference_loss")
+        coef, offsets, target = ctx.saved_tensors
+        return (ops.preference_loss_bwd(grad_loss.contiguous(), coef, offsets, ctx.num_tokens, target, ctx.ignore_index, ctx.dtype),) + (None,) * 8
+
+
+def preference_loss(logp: torch.Tensor, offsets: torch.Tensor, ref_logp: Optional[torch.Tensor] = None, beta: float = 0.1,
+                    label_smoothing: float = 0.0, loss_type: str = "sigmoid", average: bool = False, target: Optional[torch.Tensor] = None,
+                    ignore_index: int = -100) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(loss [pairs], chosen rewards [pairs], rejected rewards [pairs])`` of ``ops.preference_loss``; the loss carries the
+    gradient to ``logp``, the rewards are for logging."""
+    return _PreferenceLoss.apply(logp, offsets, ref_logp, float(beta), float(label_smoothing), loss_type, average, target, ignore_index)

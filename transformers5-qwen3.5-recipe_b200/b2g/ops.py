@@ -58,6 +58,22 @@ class _DeviceCtx:
         return self.guard.__exit__(*exc)
 
 
+def _a(t: Optional[torch.Tensor]) -> Optional[int]:
+    """A tensor's address as the binding's pointer arguments take it."""
+    return None if t is None else t.data_ptr()
+
+
+def _launch(name: str, t: torch.Tensor, *args) -> None:
+    """Call an entry point on the current stream of ``t``'s device (its last argument), switching devices only when that is
+    not the current one: the calls of a router or of a short loss are as long as what the host does for them."""
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
 # --------------------------------------------------------------------------------------
 # per-device state: status word (set by a kernel whose bounded wait ran out), IQ2_XXS table
 # --------------------------------------------------------------------------------------
@@ -75,8 +91,8 @@ def status_word(device: torch.device) -> torch.Tensor:
 def check_status(device: Optional[torch.device] = None) -> None:
     """Synchronise and raise if any kernel on the device reported a problem through the status word: a bounded wait that
     ran out (sites 1xx-4xx), a receive buffer too small for an expert-parallel exchange (901), a label outside the
-    vocabulary in the cross-entropy kernel (902), an expert id outside the expert count in the routing plan (903), expert
-    offsets beyond the rows of a grouped product (904)."""
+    vocabulary in a loss kernel (902), an expert id outside the expert count in the routing plan (903), expert
+    offsets beyond the rows of a grouped product (904), sequence offsets that decrease or leave the tokens (905)."""
     devs = [device.index if device is not None and device.index is not None else torch.cuda.current_device()] \
         if device is not None else list(_status)
     for idx in devs:
@@ -87,7 +103,8 @@ def check_status(device: Optional[torch.device] = None) -> None:
                 what = {901: "an expert-parallel receive buffer was too small (rows beyond it were dropped)",
                         902: "a cross-entropy target was outside the vocabulary",
                         903: "an expert id was outside the expert count (its route was dropped)",
-                        904: "expert offsets reached beyond the rows of a grouped product (they were clamped)"}.get(
+                        904: "expert offsets reached beyond the rows of a grouped product (they were clamped)",
+                        905: "sequence offsets of a preference loss decreased or left the tokens (they were clamped)"}.get(
                     code, "a libb2g kernel gave up a bounded wait")
                 raise _lib.B2GError(f"{what} on cuda:{idx} (status {code})")
 
@@ -296,6 +313,195 @@ def cross_entropy_inplace(logits: torch.Tensor, target: torch.Tensor, loss: torc
                   int(ignore_index), _p(count) if mean else None, int(bool(mean)), _p(status_word(logits.device)), _stream(logits))
 
 
+# --------------------------------------------------------------------------------------
+# post-training losses on rows of logits
+# --------------------------------------------------------------------------------------
+def _logit_rows(logits: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """(rows, vocabulary, row pitch) of bf16 or fp32 logits whose rows may lie apart but not on one another."""
+    if not logits.is_cuda:
+        raise RuntimeError(f"{what} must be a CUDA tensor (this package has no CPU path)")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{what} must be bf16 or fp32, got {logits.dtype}")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"{what} must be [rows, columns], got {tuple(logits.shape)}")
+    rows, v = logits.shape
+    ld = logits.stride(0) if rows > 1 else v
+    if (v > 1 and logits.stride(1) != 1) or ld < v:
+        raise RuntimeError(f"{what} need unit column stride and rows that do not overlap, got strides {logits.stride()}")
+    return rows, v, ld
+
+
+def _row_vector(t: Optional[torch.Tensor], like: torch.Tensor, rows: int, dtype: torch.dtype, what: str) -> None:
+    """An optional contiguous [rows] vector on the device of ``like``."""
+    if t is None:
+        return
+    _need(t, dtype, what)
+    if tuple(t.shape) != (rows,):
+        raise ValueError(f"{what} must be [{rows}], got {tuple(t.shape)}")
+    if t.device != like.device:
+        raise RuntimeError(f"{what} is on {t.device}, expected {like.device}")
+
+
+def _temperature(temperature: float) -> float:
+    temperature = float(temperature)
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    return temperature
+
+
+def _cotangent_out(logits: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
+    """Where a cotangent of ``logits`` goes: a new contiguous tensor, the logits themselves, or a caller's buffer apart from them."""
+    if out is None:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError(f"{what}: out must match the logits' shape, type and device")
+    _logit_rows(out, f"{what}: out")
+    if out.data_ptr() == logits.data_ptr() and (out.shape[0] <= 1 or out.stride(0) == logits.stride(0)):
+        return out
+    if out.numel() and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr():
+        def span(t):
+            return t.storage_offset(), t.storage_offset() + (t.shape[0] - 1) * t.stride(0) + t.shape[1]
+        (a0, a1), (b0, b1) = span(out), span(logits)
+        if a0 < b1 and b0 < a1:
+            raise ValueError(f"{what}: out overlaps the logits without being the logits")
+    return out
+
+
+_LOGP_DTYPES = (torch.float32, torch.float64)
+
+
+def token_logprobs(logits: torch.Tensor, target: torch.Tensor, temperature: float = 1.0, ignore_index: int = -100,
+                   dtype: torch.dtype = torch.float32):
+    """``(logp [rows], stats [rows, 4])`` of bf16 or fp32 ``logits [rows, V]``: ``logp = z_y / temperature - log sum exp(z / temperature)``
+    in fp32 or fp64 (a sum of many log-probabilities or of their differences keeps its digits in fp64), 0 where ``target`` is
+    ``ignore_index``.  ``stats`` (row maximum, reciprocal sum of exponentials, 1 - p of the target, log-sum-exp) is what
+    ``token_logprobs_bwd`` reads.  A target outside the vocabulary is reported through the status word (902) and ignored."""
+    rows, v, ld = _logit_rows(logits, "logits")
+    if target is None:
+        raise TypeError("token_logprobs needs targets")
+    _row_vector(target, logits, rows, torch.int64, "target")
+    temperature = _temperature(temperature)
+    if dtype not in _LOGP_DTYPES:
+        raise TypeError(f"log-probabilities are fp32 or fp64, not {dtype}")
+    logp = torch.empty(rows, dtype=dtype, device=logits.device)
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=logits.device)
+    _launch("b2g_token_logprobs", logits, _a(logits), ld, int(logits.dtype == torch.float32), _a(target), _a(logp), int(dtype == torch.float64),
+            _a(stats), rows, v, temperature, int(ignore_index), _a(status_word(logits.device)))
+    return logp, stats
+
+
+def token_logprobs_bwd(grad_logp: torch.Tensor, logits: torch.Tensor, target: torch.Tensor, stats: torch.Tensor, temperature: float = 1.0,
+                       ignore_index: int = -100, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``grad_logp * (onehot - softmax) / temperature`` in the logits' type; ``out=logits`` overwrites the logits."""
+    rows, v, ld = _logit_rows(logits, "logits")
+    if grad_logp is None or target is None:
+        raise TypeError("token_logprobs_bwd needs grad_logp and targets")
+    if grad_logp.dtype not in _LOGP_DTYPES:
+        raise TypeError(f"grad_logp must be fp32 or fp64, got {grad_logp.dtype}")
+    _row_vector(grad_logp, logits, rows, grad_logp.dtype, "grad_logp")
+    _row_vector(target, logits, rows, torch.int64, "target")
+    _need(stats, torch.float32, "stats")
+    if tuple(stats.shape) != (rows, 4) or stats.device != logits.device:
+        raise ValueError(f"stats must be the [{rows}, 4] tensor of token_logprobs on the logits' device")
+    temperature = _temperature(temperature)
+    out = _cotangent_out(logits, out, "token_logprobs_bwd")
+    _launch("b2g_token_logprobs_bwd", logits, _a(logits), ld, int(logits.dtype == torch.float32), _a(target), _a(stats), _a(grad_logp),
+            int(grad_logp.dtype == torch.float64), _a(out), out.stride(0) if rows > 1 else v, rows, v, temperature, int(ignore_index))
+    return out
+
+
+def policy_loss(logits: torch.Tensor, target: torch.Tensor, advantage: torch.Tensor, *, old_logp: Optional[torch.Tensor] = None,
+                ref_logp: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None, clip_low: float = 0.2, clip_high: float = 0.2,
+                kl_coef: float = 0.0, temperature: float = 1.0, ignore_index: int = -100, out: Optional[torch.Tensor] = None):
+    """Clipped policy loss of rows of logits with its cotangent: ``(loss [rows], logp [rows], kl [rows], grad_logits [rows, V])``.
+
+    ``loss = weight * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * kl)`` with ``r = exp(logp - old_logp)``
+    (1 without ``old_logp``: the data come from the present policy) and ``kl = e^d - d - 1``, ``d = ref_logp - logp``.
+    ``grad_logits`` is the gradient of ``loss.sum()``; ``out=logits`` overwrites the logits with it.  Rows whose target is
+    ``ignore_index`` or whose weight is 0 give zeros whatever else they hold; a target outside the vocabulary is reported
+    through the status word (902) and ignored."""
+    rows, v, ld = _logit_rows(logits, "logits")
+    if target is None or advantage is None:
+        raise TypeError("policy_loss needs targets and advantages")
+    _row_vector(target, logits, rows, torch.int64, "target")
+    for name, t in (("advantage", advantage), ("old_logp", old_logp), ("ref_logp", ref_logp), ("weight", weight)):
+        _row_vector(t, logits, rows, torch.float32, name)
+    temperature = _temperature(temperature)
+    if not 0.0 <= clip_low <= 1.0 or not 0.0 <= clip_high < float("inf"):
+        raise ValueError(f"clip_low must lie in 0..1 and clip_high must not be negative, got {clip_low}, {clip_high}")
+    if not 0.0 <= kl_coef < float("inf"):
+        raise ValueError(f"kl_coef must be finite and not negative, got {kl_coef}")
+    if kl_coef != 0.0 and ref_logp is None:
+        raise ValueError("policy_loss: a KL term needs ref_logp")
+    out = _cotangent_out(logits, out, "policy_loss")
+    loss, logp, kl = torch.empty(3, rows, dtype=torch.float32, device=logits.device).unbind(0)
+    _launch("b2g_policy_loss", logits, _a(logits), ld, int(logits.dtype == torch.float32), _a(target), _a(advantage), _a(old_logp), _a(ref_logp),
+            _a(weight), float(clip_low), float(clip_high), float(kl_coef), temperature, _a(loss), _a(logp), _a(kl), _a(out),
+            out.stride(0) if rows > 1 else v, rows, v, int(ignore_index), _a(status_word(logits.device)))
+    return loss, logp, kl, out
+
+
+_PAIR_LOSSES = {"sigmoid": 0, "squared": 1}
+
+
+def _pair_shapes(logp_rows: int, like: torch.Tensor, offsets: torch.Tensor, target: Optional[torch.Tensor]) -> int:
+    _need(offsets, torch.int64, "offsets")
+    if offsets.dim() != 1 or offsets.numel() % 2 != 1 or offsets.device != like.device:
+        raise ValueError("offsets must be a [2 * pairs + 1] vector on the log-probabilities' device (chosen sequences, then rejected)")
+    _row_vector(target, like, logp_rows, torch.int64, "target")
+    return offsets.numel() // 2
+
+
+def preference_loss(logp: torch.Tensor, offsets: torch.Tensor, ref_logp: Optional[torch.Tensor] = None, beta: float = 0.1,
+                    label_smoothing: float = 0.0, loss_type: str = "sigmoid", average: bool = False, target: Optional[torch.Tensor] = None,
+                    ignore_index: int = -100):
+    """Preference loss of pairs of sequences: ``(loss [pairs], chosen [pairs], rejected [pairs], coef [2 * pairs])``.
+
+    Sequence ``s`` is the tokens ``offsets[s]:offsets[s + 1]`` of ``logp``; the chosen sequences come first, the rejected ones
+    follow in the same order.  ``L_s`` is the sum (``average``: the mean) of ``logp - ref_logp`` over the tokens whose
+    ``target`` is not ``ignore_index`` (all of them without ``target``), 0 for a sequence without tokens.  ``"sigmoid"``:
+    ``-(1 - label_smoothing) log sigmoid(beta gap) - label_smoothing log sigmoid(-beta gap)``, ``gap = L_chosen - L_rejected``;
+    ``"squared"``: ``(gap - 1 / (2 beta))^2``.  ``chosen`` and ``rejected`` are the rewards ``beta L_s``; ``coef`` is the gradient
+    of a counted token.  Offsets that decrease or leave the tokens are clamped and reported through the status word (905)."""
+    if logp.dtype not in _LOGP_DTYPES:
+        raise TypeError(f"logp must be fp32 or fp64, got {logp.dtype}")
+    _need(logp, logp.dtype, "logp")
+    if logp.dim() != 1:
+        raise ValueError(f"logp must be a vector, got {tuple(logp.shape)}")
+    n = logp.shape[0]
+    pairs = _pair_shapes(n, logp, offsets, target)
+    _row_vector(ref_logp, logp, n, torch.float32, "ref_logp")
+    if loss_type not in _PAIR_LOSSES:
+        raise ValueError(f"loss_type must be one of {sorted(_PAIR_LOSSES)}, got {loss_type!r}")
+    if not 0.0 < beta < float("inf"):
+        raise ValueError(f"beta must be positive and finite, got {beta}")
+    if not 0.0 <= label_smoothing < 0.5 or (label_smoothing and loss_type != "sigmoid"):
+        raise ValueError(f"label_smoothing must lie in [0, 0.5) and belongs to the sigmoid loss, got {label_smoothing}")
+    loss, chosen, rejected = torch.empty(3, pairs, dtype=torch.float32, device=logp.device).unbind(0)
+    coef = torch.empty(2 * pairs, dtype=torch.float32, device=logp.device)
+    _launch("b2g_preference_loss", logp, _a(logp), int(logp.dtype == torch.float64), _a(ref_logp), _a(target), _a(offsets), n, pairs,
+            int(ignore_index), float(beta), float(label_smoothing), _PAIR_LOSSES[loss_type], int(bool(average)), _a(loss), _a(chosen),
+            _a(rejected), _a(coef), _a(status_word(logp.device)))
+    return loss, chosen, rejected, coef
+
+
+def preference_loss_bwd(grad_loss: torch.Tensor, coef: torch.Tensor, offsets: torch.Tensor, num_tokens: int,
+                        target: Optional[torch.Tensor] = None, ignore_index: int = -100, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Gradient (fp32 or fp64) of the token log-probabilities: ``grad_loss[pair] * coef[sequence]`` for counted tokens, 0 for all others."""
+    _need(coef, torch.float32, "coef")
+    pairs = _pair_shapes(num_tokens, coef, offsets, target)
+    _need(grad_loss, torch.float32, "grad_loss")
+    _row_vector(grad_loss, coef, pairs, torch.float32, "grad_loss")
+    if tuple(coef.shape) != (2 * pairs,):
+        raise ValueError(f"coef must be the [{2 * pairs}] tensor of preference_loss, got {tuple(coef.shape)}")
+    if dtype not in _LOGP_DTYPES:
+        raise TypeError(f"log-probabilities are fp32 or fp64, not {dtype}")
+    out = torch.empty(num_tokens, dtype=dtype, device=coef.device)
+    _launch("b2g_preference_loss_bwd", coef, _a(grad_loss), _a(coef), _a(target), _a(offsets), _a(out), int(dtype == torch.float64),
+            int(num_tokens), pairs, int(ignore_index))
+    return out
+
+
 def _fixed_group_geometry(a: torch.Tensor, payload: torch.Tensor, qtype: int, forward: bool):
     """Shapes of the fixed-group product: activations [..., G, width] (contiguous), payload [G, N, row bytes]."""
     _need(a, torch.bfloat16, "activation")
@@ -385,6 +591,54 @@ def router_topk(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor], 
         _lib.call("b2g_router_topk", _p(logits), int(logits.dtype == torch.float32), _p(bias), int(sqrt_softplus), _p(out),
                   t, e, int(top_k), _stream(logits))
     return out
+
+
+_ROUTE_SCORES = {"softmax": 0, "sigmoid": 1, "sqrtsoftplus": 2}
+
+
+def _route_settings(logits: torch.Tensor, score_function: str, scaling_factor: float) -> tuple[int, int, int, int]:
+    t, e, ld = _logit_rows(logits, "router logits")
+    if score_function not in _ROUTE_SCORES:
+        raise ValueError(f"score_function must be one of {sorted(_ROUTE_SCORES)}, got {score_function!r}")
+    if not 0.0 < scaling_factor < float("inf"):
+        raise ValueError(f"scaling_factor must be positive and finite, got {scaling_factor}")
+    return t, e, ld, _ROUTE_SCORES[score_function]
+
+
+def route_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor] = None, score_function: str = "softmax", groups: int = 1,
+                  top_groups: int = 1, group_experts: int = 1, renormalize: bool = True,
+                  scaling_factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(weights [T, top_k] fp32, indices [T, top_k] int64)`` of bf16 or fp32 ``logits [T, E]``, best expert first.
+
+    Scores ``s`` (softmax, sigmoid or sqrt-softplus), choices ``c = s + bias`` compared in 64 bits (ties: the lower id), of the
+    ``groups`` equal groups only the ``top_groups`` with the largest sum of their ``group_experts`` best choices, weights from
+    the unbiased scores, optionally renormalised, times ``scaling_factor``."""
+    t, e, ld, fn = _route_settings(logits, score_function, scaling_factor)
+    _row_vector(bias, logits, e, torch.float32, "bias")
+    weights = torch.empty(t, int(top_k), dtype=torch.float32, device=logits.device)
+    indices = torch.empty(t, int(top_k), dtype=torch.int64, device=logits.device)
+    _launch("b2g_route_experts", logits, _a(logits), ld, int(logits.dtype == torch.float32), _a(bias), fn, int(groups), int(top_groups),
+            int(group_experts), int(bool(renormalize)), float(scaling_factor), _a(weights), _a(indices), t, e, int(top_k))
+    return weights, indices
+
+
+def route_experts_bwd(grad_weights: torch.Tensor, logits: torch.Tensor, weights: torch.Tensor, indices: torch.Tensor,
+                      score_function: str = "softmax", renormalize: bool = True, scaling_factor: float = 1.0) -> torch.Tensor:
+    """Gradient ``[T, E]`` of the logits, in their type, from that of the weights; ``weights`` and ``indices`` are ``route_experts``' own."""
+    t, e, ld, fn = _route_settings(logits, score_function, scaling_factor)
+    _need(indices, torch.int64, "indices")
+    if indices.dim() != 2 or indices.shape[0] != t:
+        raise ValueError(f"indices must be [{t}, top_k], got {tuple(indices.shape)}")
+    for name, x in (("weights", weights), ("grad_weights", grad_weights)):
+        _need(x, torch.float32, name)
+        if x.shape != indices.shape:
+            raise ValueError(f"{name} must be {tuple(indices.shape)}, got {tuple(x.shape)}")
+    if not logits.device == indices.device == weights.device == grad_weights.device:
+        raise RuntimeError("route_experts_bwd: all tensors must be on the logits' device")
+    grad = torch.empty(t, e, dtype=logits.dtype, device=logits.device)
+    _launch("b2g_route_experts_bwd", logits, _a(logits), ld, int(logits.dtype == torch.float32), _a(grad_weights), _a(weights), _a(indices), fn,
+            int(bool(renormalize)), float(scaling_factor), _a(grad), t, e, indices.shape[1])
+    return grad
 
 
 def route_plan(top_k_index: torch.Tensor, num_experts: int = 256):

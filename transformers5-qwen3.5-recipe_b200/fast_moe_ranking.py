@@ -4,6 +4,8 @@ Public surface of the reference module of this name: ``router_topk_indices``,
 ``configure_fast_moe_ranking``, the geometry check and the launch helper.  Selection is one warp
 per token over the 256 expert scores with packed (score, 256 - id) keys, so equal scores resolve to
 the smaller expert id; normalisation of the selected scores stays ordinary autograd.
+``route_experts`` is the general form next to it: any expert count up to 512, softmax, sigmoid or sqrt-softplus scores, a
+balance bias, expert groups and renormalised weights, with the gradient of the logits, in one kernel per direction.
 """
 from __future__ import annotations
 
@@ -13,6 +15,7 @@ from typing import Any, cast
 import torch
 import torch.nn.functional as F
 
+from b2g import autograd as _autograd
 from b2g import ops
 
 try:
@@ -69,6 +72,37 @@ def router_topk_indices(logits: torch.Tensor, top_k: int, *, correction_bias: to
         if correction_bias.device != logits.device:
             raise ValueError("Router correction bias must be on the logits device.")
     return ops.router_topk(logits.contiguous(), top_k, correction_bias, sqrt_softplus)
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, correction_bias: torch.Tensor | None = None, score_function: str = "softmax",
+                  num_groups: int = 1, top_groups: int = 1, group_experts: int = 2, renormalize: bool = True,
+                  scaling_factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Route tokens to experts: ``(weights [tokens, top_k] fp32, indices [tokens, top_k] int64)``, best expert first.
+
+    ``logits`` are BF16 or FP32 ``[tokens, experts]`` (rows may be strided).  Experts are chosen by ``score + correction_bias``;
+    with ``num_groups > 1`` only experts of the ``top_groups`` groups whose ``group_experts`` (1 or 2) best choices sum highest are
+    eligible.  Ties go to the lower id.  The weights are the unbiased scores of the chosen experts, divided by their sum when
+    ``renormalize``, times ``scaling_factor``, and carry the gradient to the logits.  The result feeds ``prepare_expert_routing``
+    or an expert module directly."""
+    if logits.ndim != 2:
+        raise ValueError(f"Router logits must be [tokens,experts], got {logits.shape}.")
+    num_experts = logits.shape[1]
+    if score_function not in {"softmax", "sigmoid", "sqrtsoftplus"}:
+        raise ValueError(f"Unsupported router score function: {score_function!r}.")
+    if correction_bias is not None and correction_bias.shape != (num_experts,):
+        raise ValueError(f"Router correction bias must have shape {(num_experts,)}, got {correction_bias.shape}.")
+    if not 1 <= num_experts <= 512:
+        raise ValueError(f"Expert routing supports 1 to 512 experts, got {num_experts}.")
+    if not 1 <= num_groups <= 32 or num_experts % num_groups or not 1 <= top_groups <= num_groups:
+        raise ValueError(f"{num_groups} groups ({top_groups} kept) do not split {num_experts} experts.")
+    if group_experts not in (1, 2):
+        raise ValueError(f"group_experts must be 1 or 2, got {group_experts}.")
+    if not 1 <= top_k <= min(32, top_groups * (num_experts // num_groups)):
+        raise ValueError(f"top_k={top_k} must lie between 1 and the {top_groups * (num_experts // num_groups)} eligible experts (32 at most).")
+    if logits.device.type != "cuda" or logits.dtype not in {torch.bfloat16, torch.float32}:
+        raise RuntimeError("Expert routing requires CUDA BF16 or FP32 logits.")
+    return _autograd.route_experts(logits, top_k, correction_bias, score_function, num_groups, top_groups, group_experts, renormalize,
+                                   scaling_factor)
 
 
 def _qwen_router_forward(self: Any, hidden_states: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
