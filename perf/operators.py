@@ -353,9 +353,10 @@ def _own(s):
     if not c["vocab"]:
         loss, chosen, rejected = autograd.preference_loss(s["logp"], s["offsets"], ref_logp=s["ref"], **settings)
         return loss.detach(), chosen, rejected, torch.autograd.grad(loss, s["logp"], s["grad"])[0]
-    logp = autograd.token_logprobs(s["logits"], s["target"], ignore_index=_IGNORE)
+    # the sequences' sums of differences need more digits of the log-probabilities than 32 bits hold
+    logp = autograd.token_logprobs(s["logits"], s["target"], ignore_index=_IGNORE, dtype=torch.float64)
     loss, chosen, rejected = autograd.preference_loss(logp, s["offsets"], ref_logp=s["ref"], **settings)
-    return loss.detach(), chosen, rejected, logp.detach(), torch.autograd.grad(loss, s["logits"], s["grad"])[0]
+    return loss.detach(), chosen, rejected, logp.detach().float(), torch.autograd.grad(loss, s["logits"], s["grad"])[0]
 
 
 def run(state):
