@@ -344,8 +344,8 @@ def _row_vector(t: Optional[torch.Tensor], like: torch.Tensor, rows: int, dtype:
 
 def _temperature(temperature: float) -> float:
     temperature = float(temperature)
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-20 < temperature < 1e20:
+        raise ValueError(f"temperature must lie in 1e-20..1e20, got {temperature}")
     return temperature
 
 

@@ -7,6 +7,8 @@
 // sequence all lose what a 32-bit log-probability has already rounded away.
 #include "b2g_common.cuh"
 
+#include <cmath>
+
 namespace b2g {
 namespace policy {
 
@@ -170,7 +172,7 @@ __device__ __forceinline__ void put_logp(const RowArgs& a, int64_t row, double l
 
 // Loss, log-probability and KL estimate of a live row; returns d loss / d logp.
 __device__ __forceinline__ float policy_scalars(const RowArgs& a, const Given& in, double logp, int64_t row, bool write) {
-  const double adv = in.advantage, ratio = a.old_logp ? exp(logp - (double)in.old_logp) : 1.0;
+  const double adv = in.advantage, ratio = a.old_logp ? exp(logp - (double)in.old_logp) : (logp != logp ? logp : 1.0);
   const double clipped = fmin(fmax(ratio, 1.0 - (double)a.clip_low), 1.0 + (double)a.clip_high);
   const bool inside = ratio * adv <= clipped * adv || ratio != ratio;
   double loss = inside ? -ratio * adv : -clipped * adv, slope = inside ? -ratio * adv : 0.0, kl = 0.0;
@@ -601,7 +603,7 @@ static int check_rows(const char* what, int dtype, int64_t rows, int64_t V, int6
   B2G_REQUIRE(dtype == 0 || dtype == 1, "%s: logits_dtype must be 0 (bf16) or 1 (fp32)", what);
   B2G_REQUIRE(rows >= 0 && rows < (1ll << 28) && V >= 1 && V < (1ll << 31) && (rows <= 1 || ld >= V), "%s: bad shape rows=%lld V=%lld ld=%lld", what,
               (long long)rows, (long long)V, (long long)ld);
-  B2G_REQUIRE(tau > 0.f && tau <= 3.4e38f, "%s: the temperature must be positive and finite", what);
+  B2G_REQUIRE(tau >= 1e-20f && tau <= 1e20f, "%s: the temperature must lie in 1e-20..1e20", what);
   return 0;
 }
 
@@ -610,6 +612,7 @@ static policy::RowArgs row_args(const int64_t* target, int64_t V, int64_t ignore
   a.target = target; a.V = V; a.ignore_index = ignore_index; a.tau = tau; a.status = status;
   const double c = 1.4426950408889634 / tau;    // log2(e) / tau
   a.c.hi = (float)c;
+  if ((double)a.c.hi >= c) a.c.hi = nextafterf(a.c.hi, 0.f);   // the low part is positive: -inf logits times both parts stay -inf
   a.c.lo = (float)(c - (double)a.c.hi);
   a.c.inv = 1.f / tau;
   return a;
