@@ -2,9 +2,11 @@
 //   s = softmax(l) | sigmoid(l) | sqrt(log(1 + e^l)),  c = s + b,  best M of G groups by the sum of their n best c,
 //   best k of c in them,  w_j = alpha s_j / (sum_i s_i + 1e-20)  or  alpha s_j.
 // Softmax weights that are renormalised are the softmax of the chosen logits (the common denominator cancels).
+//
 // One warp per token; lane i holds experts [i * kPer, (i + 1) * kPer), so the lowest lane of a tie holds the lowest expert.
 // The order of c is its order in 64 bits (without a bias: the order of the logits), so the choice does not depend on how an
-// exponential is rounded.
+// exponential is rounded.  The work is done in 32 bits; where two neighbours of the order lie closer than the 32-bit scores can
+// be wrong and are not equal by construction (same logit, same bias), the warp goes over its token once more in 64 bits.
 #include "b2g_common.cuh"
 
 namespace b2g {
@@ -22,9 +24,23 @@ __device__ __forceinline__ unsigned long long key_of(double v) {
   return b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
 }
 
+__device__ __forceinline__ uint32_t key_of(float v) {
+  if (v != v) return 1u;
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b ^ ((b >> 31) ? ~0u : 0x80000000u);
+}
+
 __device__ __forceinline__ double score_of(double x, int fn) {
   if (fn == kSigmoid) return 1.0 / (1.0 + exp(-x));
   return sqrt(fmax(x, 0.0) + log1p(exp(-fabs(x))));
+}
+
+// Relative error 2^-21.5 at most: exponential and logarithm 2^-22, sum, quotient and root half a step each.
+__device__ __forceinline__ float score_of(float x, int fn) {
+  const float n = expf(-fabsf(x));
+  if (fn == kSigmoid) return __fdividef(x >= 0.f ? 1.f : n, 1.f + n);
+  // far below 0 the logarithm is n to within n^2 / 2, and its root is exp(x / 2), which does not underflow where n does
+  return x < -16.f ? expf(0.5f * x) : sqrtf(fmaxf(x, 0.f) + log1pf(n));
 }
 
 __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
@@ -42,113 +58,333 @@ __device__ __forceinline__ float load_logit(const T* p, int64_t i) {
   else return p[i];
 }
 
+// The whole route of one token in 64 bits, by one warp.  The choices live in `value` (32 * kPer doubles of shared memory) and
+// everything else is computed again where it is needed: few registers, because the 32-bit pass would have to keep as many free.
+template <typename T, int kPer>
+__device__ __noinline__ void route_in_64_bits(const T* row, const float* bias, int fn, int G, int M, int best, int renorm, float alpha,
+                                              float* weights, int64_t* indices, int E, int K, double* value) {
+  const int lane = threadIdx.x & 31, first = lane * kPer, mine = max(0, min(kPer, E - first));
+  double top = -INFINITY, sum = 0.0;
+  if (fn == kSoftmax) {
+#pragma unroll 1
+    for (int j = 0; j < mine; ++j) top = fmax(top, (double)load_logit(row, first + j));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll 1
+    for (int j = 0; j < mine; ++j) {
+      const double x = load_logit(row, first + j);
+      sum += top == -INFINITY && x == x ? 0.0 : exp(x - top);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  auto score = [&](double x) {
+    if (fn != kSoftmax) return score_of(x, fn);
+    const double e = top == -INFINITY && x == x ? 0.0 : exp(x - top);
+    return e == 0.0 ? 0.0 : e / sum;
+  };
+  uint32_t gone = 0u;       // bit j: expert first + j has been chosen, or its group dropped
+  if (M < G) {
+    const int per = E / G;
+#pragma unroll 1
+    for (int j = 0; j < mine; ++j) {
+      const double v = score((double)load_logit(row, first + j));
+      value[first + j] = bias ? v + (double)bias[first + j] : v;
+    }
+    __syncwarp();
+    unsigned long long worth = 0ull;
+    if (lane < G) {
+      double a = -INFINITY, b = -INFINITY;
+#pragma unroll 1
+      for (int i = 0; i < per; ++i) {
+        const double v = value[lane * per + i];
+        if (v > a || v != v) { b = a; a = v; }
+        else if (v > b) b = v;
+      }
+      worth = key_of(best == 2 && per > 1 ? a + b : a);
+    }
+    unsigned kept = 0u;
+#pragma unroll 1
+    for (int r = 0; r < M; ++r) {
+      const unsigned long long all = warp_max(worth);
+      const int g = __ffs(__ballot_sync(0xffffffffu, worth == all)) - 1;
+      kept |= 1u << g;
+      if (lane == g) worth = 0ull;
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int j = 0; j < mine; ++j)
+      if (!((kept >> ((first + j) / per)) & 1u)) gone |= 1u << j;
+  }
+#pragma unroll 1
+  for (int j = 0; j < mine; ++j) {
+    const double x = load_logit(row, first + j);
+    value[first + j] = bias ? score(x) + (double)bias[first + j] : x;
+  }
+  __syncwarp();
+  int id = 0;         // lane r keeps the r-th choice
+#pragma unroll 1
+  for (int r = 0; r < K; ++r) {
+    unsigned long long own = 0ull;
+    int at = 0;
+#pragma unroll 1
+    for (int j = 0; j < mine; ++j) {
+      const unsigned long long k = (gone >> j) & 1u ? 0ull : key_of(value[first + j]);
+      if (k > own) { own = k; at = j; }
+    }
+    const unsigned long long all = warp_max(own);
+    const int src = __ffs(__ballot_sync(0xffffffffu, own == all)) - 1;
+    const int e = __shfl_sync(0xffffffffu, first + at, src);
+    if (lane == src) gone |= 1u << at;
+    if (lane == r) id = e;
+  }
+  const bool out = lane < K;
+  const double raw = out ? (double)load_logit(row, id) : -INFINITY;
+  double w = 0.0;
+  if (renorm && fn == kSoftmax) {     // softmax of the chosen logits
+    double m = raw;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (out) w = m == -INFINITY && raw == raw ? 0.0 : exp(raw - m);
+  } else if (out) {
+    w = score(raw);
+  }
+  if (renorm) {
+    double total = w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    w = w / (total + 1e-20);
+  }
+  if (out) {
+    weights[lane] = (float)(w * alpha);
+    indices[lane] = id;
+  }
+}
+
+// kPer consecutive values of a row; `wide`: 16-byte loads are aligned.
+template <typename T, int kPer>
+__device__ __forceinline__ void load_lane(const T* row, int first, int E, bool wide, float fill, float (&x)[kPer]) {
+  constexpr int N = 16 / sizeof(T);
+  if constexpr (kPer % N == 0) {
+    if (wide && first + kPer <= E) {
+#pragma unroll
+      for (int i = 0; i < kPer; i += N) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(row + first + i));
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (sizeof(T) == 2) { x[i + 2 * j] = dev::bf16_lo(w[j]); x[i + 2 * j + 1] = dev::bf16_hi(w[j]); }
+          else x[i + j] = __uint_as_float(w[j]);
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) x[j] = first + j < E ? load_logit(row, first + j) : fill;
+}
+
+__device__ __forceinline__ float warp_maxf(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+constexpr int kCandidates = 64;     // two per lane
+
+// One chosen (or candidate) expert: order key of its choice, id, logit and score.
+struct Pick { uint32_t key; int id; float x, s; };
+static_assert(sizeof(Pick) == 16, "a pick is one 16-byte access");
+
+template <int kPer>
+struct WarpSpace {
+  union {
+    double value[32 * kPer];          // the 64-bit pass
+    struct {
+      Pick candidate[kCandidates];
+      Pick sorted[kMaxTopK + 1];
+    };
+    float choice[32 * kPer];          // groups that do not fall on lane borders
+  };
+};
+
+// The best two of a group's choices, n of them summed.
+struct Two { float a, b; };
+__device__ __forceinline__ Two add_to(Two t, float v) { return Two{fmaxf(t.a, v), fmaxf(t.b, fminf(t.a, v))}; }
+__device__ __forceinline__ Two merge(Two t, Two u) { return Two{fmaxf(t.a, u.a), fmaxf(fminf(t.a, u.a), fmaxf(t.b, u.b))}; }
+
 template <typename T, int kPer>
 __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ bias, int fn,
                                                             int G, int M, int best, int renorm, float alpha, float* __restrict__ weights,
                                                             int64_t* __restrict__ indices, int64_t tokens, int E, int K) {
-  __shared__ double value[kWarps][32 * kPer];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ WarpSpace<kPer> space[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = lane * kPer;
   const int64_t t = (int64_t)blockIdx.x * kWarps + warp;
   if (t >= tokens) return;
   const T* row = logits + t * ld;
-  double x[kPer], s[kPer];
-  double top = -INFINITY;
+  WarpSpace<kPer>& ws = space[warp];
+  const bool wide = (reinterpret_cast<uintptr_t>(row) & 15) == 0, grouped = M < G;
+  // 32-bit scores are off by 2^-21.5 (softmax: 2^-18, the exponent being rounded at sizes up to 100); twice that for a difference
+  const float eps = fn == kSoftmax ? 7.62939453125e-6f : 9.5367431640625e-7f;
+  constexpr float kStep = 2.384185791015625e-7f;      // and 2^-22 of the sums
+
+  float x[kPer], s[kPer];
+  uint32_t key[kPer];
+  load_lane<T, kPer>(row, first, E, wide, -INFINITY, x);
+  const bool scored = bias || grouped || (fn == kSoftmax && !renorm);
+  float top = x[0], denominator = 1.f, smax = 1.f;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int e = lane * kPer + j;
-    x[j] = e < E ? (double)load_logit(row, e) : -INFINITY;
-    top = fmax(top, x[j]);
+  for (int j = 1; j < kPer; ++j) top = fmaxf(top, x[j]);
+  if (scored) {
+    top = warp_maxf(top);
+    if (fn == kSoftmax) {
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        s[j] = top == -INFINITY && x[j] == x[j] ? 0.f : expf(x[j] - top);
+        sum += s[j];
+      }
+      denominator = warp_sum(sum);
+      smax = 1.f / denominator;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) s[j] = s[j] == 0.f ? 0.f : s[j] * smax;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) s[j] = score_of(x[j], fn);
+      smax = score_of(top, fn);
+    }
   }
-  if (fn == kSoftmax) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    double sum = 0.0;
+  bool unsure = false;
+  if (bias) {
+    float b[kPer];
+    load_lane<float, kPer>(bias, first, E, (reinterpret_cast<uintptr_t>(bias) & 15) == 0, 0.f, b);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      s[j] = top == -INFINITY && x[j] == x[j] ? 0.0 : exp(x[j] - top);
-      sum += s[j];
+      const float c = s[j] + b[j];
+      key[j] = first + j < E ? key_of(c) : 0u;
+      if (grouped) ws.choice[first + j] = c;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) s[j] = s[j] == 0.0 ? 0.0 : s[j] / sum;
   } else {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) s[j] = score_of(x[j], fn);
-  }
-  unsigned long long key[kPer];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int e = lane * kPer + j;
-    key[j] = e < E ? key_of(bias ? s[j] + (double)bias[e] : x[j]) : 0ull;
-  }
-  if (M < G) {
-    const int per = E / G;
-#pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const int e = lane * kPer + j;
-      value[warp][e] = e < E ? (bias ? s[j] + (double)bias[e] : s[j]) : 0.0;
+      key[j] = first + j < E ? key_of(x[j]) : 0u;
+      if (grouped) ws.choice[first + j] = s[j];
+    }
+  }
+  if (grouped) {
+    const int per = E / G;
+    __syncwarp();
+    Two two{-INFINITY, -INFINITY};
+    uint32_t mine = 0u;
+    float worth = 0.f;
+    if (lane < G) {
+      bool number = true;
+      for (int i = 0; i < per; ++i) {
+        const float v = ws.choice[lane * per + i];
+        number = number && v == v;
+        two = add_to(two, v);
+      }
+      worth = best == 2 && per > 1 ? two.a + two.b : two.a;
+      if (!number) worth = NAN;
+      mine = key_of(worth);
     }
     __syncwarp();
-    unsigned long long mine = 0ull;
-    if (lane < G) {
-      double a = -INFINITY, b = -INFINITY;
-      for (int i = 0; i < per; ++i) {
-        const double v = value[warp][lane * per + i];
-        if (v > a || v != v) { b = a; a = v; }
-        else if (v > b) b = v;
-      }
-      mine = key_of(best == 2 && per > 1 ? a + b : a);
-    }
     unsigned kept = 0u;
-    for (int r = 0; r < M; ++r) {
-      const unsigned long long all = warp_max(mine);
+    float last = 0.f;
+    for (int r = 0; r <= M; ++r) {
+      const uint32_t all = __reduce_max_sync(0xffffffffu, mine);
       const int g = __ffs(__ballot_sync(0xffffffffu, mine == all)) - 1;
-      kept |= 1u << g;
-      if (lane == g) mine = 0ull;
+      const float v = __shfl_sync(0xffffffffu, worth, g);
+      if (r < M) {
+        kept |= 1u << g;
+        last = v;
+        if (lane == g) mine = 0u;
+      } else {
+        unsure = !(last - v > 2.f * eps * smax + kStep * fabsf(last));
+      }
     }
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int e = lane * kPer + j;
-      if (e < E && !((kept >> (e / per)) & 1u)) key[j] = 0ull;
-    }
-  }
-  int id = 0;         // lane r keeps the r-th choice
-  double picked = 0.0, raw = -INFINITY;
-  for (int r = 0; r < K; ++r) {
-    unsigned long long own = key[0];
-    int at = 0;
-#pragma unroll
-    for (int j = 1; j < kPer; ++j)
-      if (key[j] > own) { own = key[j]; at = j; }
-    const unsigned long long all = warp_max(own);
-    const int src = __ffs(__ballot_sync(0xffffffffu, own == all)) - 1;
-    double sj = 0.0, xj = 0.0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (j == at) { sj = s[j]; xj = x[j]; if (lane == src) key[j] = 0ull; }
-    const int ej = __shfl_sync(0xffffffffu, lane * kPer + at, src);
-    sj = __shfl_sync(0xffffffffu, sj, src);
-    xj = __shfl_sync(0xffffffffu, xj, src);
-    if (lane == r) { id = ej; picked = sj; raw = xj; }
+      if (first + j < E && !((kept >> ((first + j) / per)) & 1u)) key[j] = 0u;
   }
-  const bool out = lane < K;
-  double w = out ? picked : 0.0;
-  if (renorm) {
-    if (fn == kSoftmax) {     // softmax of the chosen logits
-      double m = out ? raw : -INFINITY;
+
+  // Candidates: everything not below the L-th largest lane maximum, L = the ranks that are looked at (with a bias, whether the
+  // last choice is clear of the first one left out).  At least L of them, hardly ever more than 2 L, whatever the order is.
+  const int ranks = K + (bias ? 1 : 0);
+  uint32_t head = key[0], floor_key = 1u;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-      w = !out ? 0.0 : (m == -INFINITY && raw == raw ? 0.0 : exp(raw - m));
+  for (int j = 1; j < kPer; ++j) head = max(head, key[j]);
+  if (ranks <= 32) {
+    for (int r = 0; r < ranks; ++r) {
+      floor_key = __reduce_max_sync(0xffffffffu, head);
+      if (head == floor_key) head = 0u;
     }
-    double sum = w;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    w = w / (sum + 1e-20);
+    floor_key = max(floor_key, 1u);
   }
-  if (out) {
-    weights[t * K + lane] = (float)(w * alpha);
-    indices[t * K + lane] = id;
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const bool in = key[j] >= floor_key;
+    const unsigned mask = __ballot_sync(0xffffffffu, in);
+    const int at = n + __popc(mask & ((1u << lane) - 1u));
+    if (in && at < kCandidates) ws.candidate[at] = Pick{key[j], first + j, x[j], scored ? s[j] : 0.f};
+    n += __popc(mask);
+  }
+  if (n > kCandidates) unsure = true;
+  if (!unsure) {
+    __syncwarp();
+    Pick mine[2];
+    int rank[2] = {0, 0};
+    const Pick none{0u, 0, 0.f, 0.f};
+    mine[0] = lane < n ? ws.candidate[lane] : none;
+    mine[1] = lane + 32 < n ? ws.candidate[lane + 32] : none;
+    for (int q = 0; q < n; ++q) {
+      const uint2 other = *reinterpret_cast<const uint2*>(&ws.candidate[q]);
+      rank[0] += other.x > mine[0].key || (other.x == mine[0].key && (int)other.y < mine[0].id);
+    }
+    if (n > 32) {
+      for (int q = 0; q < n; ++q) {
+        const uint2 other = *reinterpret_cast<const uint2*>(&ws.candidate[q]);
+        rank[1] += other.x > mine[1].key || (other.x == mine[1].key && (int)other.y < mine[1].id);
+      }
+    }
+    if (lane < n && rank[0] < ranks) ws.sorted[rank[0]] = mine[0];
+    if (lane + 32 < n && rank[1] < ranks) ws.sorted[rank[1]] = mine[1];
+    __syncwarp();
+    const Pick p = lane < K ? ws.sorted[lane] : none;
+    if (bias) {
+      bool close = false;
+      if (lane < K && lane + 1 < min(n, ranks)) {
+        const Pick q = ws.sorted[lane + 1];
+        const float bp = bias[p.id], bq = bias[q.id], c = p.s + bp;
+        close = !(c - (q.s + bq) > eps * fmaxf(p.s, q.s) + kStep * fabsf(c)) && !(p.x == q.x && bp == bq);
+      }
+      unsure = __any_sync(0xffffffffu, close);
+    }
+    if (!unsure) {
+      float w = 0.f;
+      if (lane < K) w = scored ? p.s : (fn == kSoftmax ? 0.f : score_of(p.x, fn));
+      if (renorm) {
+        if (fn == kSoftmax) {
+          const float m = warp_maxf(lane < K ? p.x : -INFINITY);
+          w = lane >= K || (m == -INFINITY && p.x == p.x) ? 0.f : expf(p.x - m);
+        }
+        w = w / (warp_sum(w) + 1e-20f);
+      }
+      if (lane < K) {
+        weights[t * K + lane] = w * alpha;
+        indices[t * K + lane] = p.id;
+      }
+    }
+  }
+  if (unsure) {
+    __syncwarp();
+    route_in_64_bits<T, kPer>(row, bias, fn, G, M, best, renorm, alpha, weights + t * K, indices + t * K, E, K, ws.value);
   }
 }
 
@@ -159,8 +395,9 @@ template <typename T, int kPer>
 __global__ void __launch_bounds__(kWarps * 32) route_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ grad_w,
                                                                 const float* __restrict__ weights, const int64_t* __restrict__ indices, int fn,
                                                                 int renorm, float alpha, T* __restrict__ grad, int64_t tokens, int E, int K) {
-  __shared__ float value[kWarps][32 * kPer];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int N = 16 / sizeof(T);
+  __shared__ __align__(16) float value[kWarps][32 * kPer];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = lane * kPer;
   const int64_t t = (int64_t)blockIdx.x * kWarps + warp;
   if (t >= tokens) return;
   const T* row = logits + t * ld;
@@ -169,49 +406,59 @@ __global__ void __launch_bounds__(kWarps * 32) route_bwd_kernel(const T* __restr
   const int64_t e64 = in ? indices[t * K + lane] : -1;
   const bool ok = e64 >= 0 && e64 < E;
   const int e = ok ? (int)e64 : 0;
-  float dot = g * w;
+  const float raw = ok && fn != kSoftmax ? load_logit(row, e) : 0.f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+  for (int j = 0; j < kPer; ++j) value[warp][first + j] = 0.f;
+  const float dot = warp_sum(g * w);
   float d = renorm ? (w / alpha) * (alpha * g - dot) : g * w;
-  if (ok && fn != kSoftmax) {
-    const float x = load_logit(row, e);
-    const float n = expf(-fabsf(x));
-    const float sig = x >= 0.f ? 1.f / (1.f + n) : n / (1.f + n);
-    if (fn == kSigmoid) d *= x >= 0.f ? n / (1.f + n) : 1.f / (1.f + n);
-    else d *= x < -16.f ? 0.5f : sig / (2.f * (fmaxf(x, 0.f) + log1pf(n)));
+  if (fn != kSoftmax) {
+    const float n = expf(-fabsf(raw));
+    if (fn == kSigmoid) d *= (raw >= 0.f ? n : 1.f) / (1.f + n);
+    else d *= raw < -16.f ? 0.5f : (raw >= 0.f ? 1.f : n) / ((1.f + n) * 2.f * (fmaxf(raw, 0.f) + log1pf(n)));
   }
-  for (int j = lane; j < E; j += 32) value[warp][j] = 0.f;
   __syncwarp();
   if (ok) value[warp][e] = d;
   __syncwarp();
-  T* out = grad + t * (int64_t)E;
-  float x[kPer], top = -INFINITY, sum = 0.f;
-  const bool full = fn == kSoftmax && !renorm;
-  if (full) {
+  float v[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int i = j * 32 + lane;
-      x[j] = i < E ? load_logit(row, i) : -INFINITY;
-      top = fmaxf(top, x[j]);
-    }
+  for (int j = 0; j < kPer; ++j) v[j] = value[warp][first + j];
+  if (fn == kSoftmax && !renorm) {
+    float x[kPer], sum = 0.f;
+    load_lane<T, kPer>(row, first, E, (reinterpret_cast<uintptr_t>(row) & 15) == 0, -INFINITY, x);
+    float top = x[0];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int j = 1; j < kPer; ++j) top = fmaxf(top, x[j]);
+    top = warp_maxf(top);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       x[j] = top == -INFINITY && x[j] == x[j] ? 0.f : expf(x[j] - top);
       sum += x[j];
     }
+    sum = warp_sum(sum);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int j = 0; j < kPer; ++j) v[j] -= x[j] == 0.f ? 0.f : x[j] / sum * dot;
+  }
+  T* out = grad + t * (int64_t)E;
+  if constexpr (kPer % N == 0) {
+    if (first + kPer <= E && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+#pragma unroll
+      for (int i = 0; i < kPer; i += N) {
+        uint4 q;
+        if constexpr (sizeof(T) == 2)
+          q = make_uint4(dev::pack_bf16(v[i], v[i + 1]), dev::pack_bf16(v[i + 2], v[i + 3]), dev::pack_bf16(v[i + 4], v[i + 5]),
+                         dev::pack_bf16(v[i + 6], v[i + 7]));
+        else
+          q = make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
+        *reinterpret_cast<uint4*>(out + first + i) = q;
+      }
+      return;
+    }
   }
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    const int i = j * 32 + lane;
-    if (i < E) {
-      float v = value[warp][i];
-      if (full) v -= x[j] == 0.f ? 0.f : x[j] / sum * dot;
-      if constexpr (sizeof(T) == 2) out[i] = __float2bfloat16_rn(v);
-      else out[i] = v;
+    if (first + j < E) {
+      if constexpr (sizeof(T) == 2) out[first + j] = __float2bfloat16_rn(v[j]);
+      else out[first + j] = v[j];
     }
   }
 }
