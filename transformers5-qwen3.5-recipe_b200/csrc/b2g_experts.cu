@@ -24,12 +24,6 @@ __device__ __forceinline__ unsigned long long key_of(double v) {
   return b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
 }
 
-__device__ __forceinline__ uint32_t key_of(float v) {
-  if (v != v) return 1u;
-  const uint32_t b = __float_as_uint(v + 0.f);
-  return b ^ ((b >> 31) ? ~0u : 0x80000000u);
-}
-
 __device__ __forceinline__ double score_of(double x, int fn) {
   if (fn == kSigmoid) return 1.0 / (1.0 + exp(-x));
   return sqrt(fmax(x, 0.0) + log1p(exp(-fabs(x))));
@@ -195,30 +189,35 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// The largest of 32 lanes' values; NaN (a lane without a value) loses against every number.
+__device__ __forceinline__ float lanes_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 constexpr int kCandidates = 64;     // two per lane
 
-// One chosen (or candidate) expert: order key of its choice, id, logit and score.
-struct Pick { uint32_t key; int id; float x, s; };
-static_assert(sizeof(Pick) == 16, "a pick is one 16-byte access");
+// A candidate: the value it is chosen by, and its id.
+struct Pick { float c; int id; };
 
 template <int kPer>
 struct WarpSpace {
   union {
-    double value[32 * kPer];          // the 64-bit pass
-    struct {
-      Pick candidate[kCandidates];
-      Pick sorted[kMaxTopK + 1];
-    };
-    float choice[32 * kPer];          // groups that do not fall on lane borders
+    double value[32 * kPer];                 // the 64-bit pass
+    float choice[32 * kPer];                 // groups that do not fall on lane borders
+    Pick candidate[32 * kPer];
   };
+  Pick sorted[kMaxTopK + 1];
 };
 
-// The best two of a group's choices, n of them summed.
+// The best two of a group's choices.
 struct Two { float a, b; };
 __device__ __forceinline__ Two add_to(Two t, float v) { return Two{fmaxf(t.a, v), fmaxf(t.b, fminf(t.a, v))}; }
 __device__ __forceinline__ Two merge(Two t, Two u) { return Two{fmaxf(t.a, u.a), fmaxf(fminf(t.a, u.a), fmaxf(t.b, u.b))}; }
 
-template <typename T, int kPer>
+// kScored: the choice needs the scores (a bias, groups) or the weights need the whole row's (softmax that is not renormalised).
+template <typename T, int kPer, bool kScored>
 __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ bias, int fn,
                                                             int G, int M, int best, int renorm, float alpha, float* __restrict__ weights,
                                                             int64_t* __restrict__ indices, int64_t tokens, int E, int K) {
@@ -228,155 +227,164 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
   if (t >= tokens) return;
   const T* row = logits + t * ld;
   WarpSpace<kPer>& ws = space[warp];
-  const bool wide = (reinterpret_cast<uintptr_t>(row) & 15) == 0, grouped = M < G;
+  const bool wide = (reinterpret_cast<uintptr_t>(row) & 15) == 0, grouped = kScored && M < G, biased = kScored && bias;
   // 32-bit scores are off by 2^-21.5 (softmax: 2^-18, the exponent being rounded at sizes up to 100); twice that for a difference
   const float eps = fn == kSoftmax ? 7.62939453125e-6f : 9.5367431640625e-7f;
   constexpr float kStep = 2.384185791015625e-7f;      // and 2^-22 of the sums
 
-  float x[kPer], s[kPer];
-  uint32_t key[kPer];
-  load_lane<T, kPer>(row, first, E, wide, -INFINITY, x);
-  const bool scored = bias || grouped || (fn == kSoftmax && !renorm);
-  float top = x[0], denominator = 1.f, smax = 1.f;
+  // c[j]: what expert first + j is chosen by; NaN where there is none to choose
+  float c[kPer], top = -INFINITY, denominator = 1.f;
+  load_lane<T, kPer>(row, first, E, wide, NAN, c);
+  bool unsure = false;
+  if constexpr (kScored) {
+    float s[kPer];
+    bool odd = false;                                  // NaN among the logits: left to the 64-bit pass
 #pragma unroll
-  for (int j = 1; j < kPer; ++j) top = fmaxf(top, x[j]);
-  if (scored) {
-    top = warp_maxf(top);
+    for (int j = 0; j < kPer; ++j) {
+      odd = odd || (c[j] != c[j] && first + j < E);
+      top = fmaxf(top, c[j]);
+    }
+    unsure = __any_sync(0xffffffffu, odd);
+    top = lanes_max(top);
+    float smax;
     if (fn == kSoftmax) {
-      float sum = 0.f;
+      denominator = 0.f;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        s[j] = top == -INFINITY && x[j] == x[j] ? 0.f : expf(x[j] - top);
-        sum += s[j];
+        s[j] = top == -INFINITY || !(c[j] == c[j]) ? 0.f : expf(c[j] - top);
+        denominator += s[j];
       }
-      denominator = warp_sum(sum);
+      denominator = warp_sum(denominator);
       smax = 1.f / denominator;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) s[j] = s[j] == 0.f ? 0.f : s[j] * smax;
     } else {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) s[j] = score_of(x[j], fn);
+      for (int j = 0; j < kPer; ++j) s[j] = score_of(c[j], fn);
       smax = score_of(top, fn);
     }
-  }
-  bool unsure = false;
-  if (bias) {
-    float b[kPer];
-    load_lane<float, kPer>(bias, first, E, (reinterpret_cast<uintptr_t>(bias) & 15) == 0, 0.f, b);
+    if (biased) {
+      float b[kPer];
+      load_lane<float, kPer>(bias, first, E, (reinterpret_cast<uintptr_t>(bias) & 15) == 0, NAN, b);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const float c = s[j] + b[j];
-      key[j] = first + j < E ? key_of(c) : 0u;
-      if (grouped) ws.choice[first + j] = c;
+      for (int j = 0; j < kPer; ++j) s[j] = c[j] = s[j] + b[j];
     }
-  } else {
+    if (grouped) {                                     // s: what the groups are compared by
+      const int per = E / G, lanes = per / kPer;
+      const bool on_lanes = lanes * kPer == per && (lanes & (lanes - 1)) == 0;
+      Two two{-INFINITY, -INFINITY};
+      int group = lane;
+      if (on_lanes) {                                  // a power of two of whole lanes per group: its last lane speaks for it
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      key[j] = first + j < E ? key_of(x[j]) : 0u;
-      if (grouped) ws.choice[first + j] = s[j];
-    }
-  }
-  if (grouped) {
-    const int per = E / G;
-    __syncwarp();
-    Two two{-INFINITY, -INFINITY};
-    uint32_t mine = 0u;
-    float worth = 0.f;
-    if (lane < G) {
-      bool number = true;
-      for (int i = 0; i < per; ++i) {
-        const float v = ws.choice[lane * per + i];
-        number = number && v == v;
-        two = add_to(two, v);
-      }
-      worth = best == 2 && per > 1 ? two.a + two.b : two.a;
-      if (!number) worth = NAN;
-      mine = key_of(worth);
-    }
-    __syncwarp();
-    unsigned kept = 0u;
-    float last = 0.f;
-    for (int r = 0; r <= M; ++r) {
-      const uint32_t all = __reduce_max_sync(0xffffffffu, mine);
-      const int g = __ffs(__ballot_sync(0xffffffffu, mine == all)) - 1;
-      const float v = __shfl_sync(0xffffffffu, worth, g);
-      if (r < M) {
-        kept |= 1u << g;
-        last = v;
-        if (lane == g) mine = 0u;
+        for (int j = 0; j < kPer; ++j) two = add_to(two, s[j]);
+        for (int o = 1; o < lanes; o *= 2) two = merge(two, Two{__shfl_xor_sync(0xffffffffu, two.a, o), __shfl_xor_sync(0xffffffffu, two.b, o)});
+        group = lane % lanes == 0 ? lane / lanes : G;
       } else {
-        unsure = !(last - v > 2.f * eps * smax + kStep * fabsf(last));
-      }
-    }
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (first + j < E && !((kept >> ((first + j) / per)) & 1u)) key[j] = 0u;
+        for (int j = 0; j < kPer; ++j) ws.choice[first + j] = s[j];
+        __syncwarp();
+        if (lane < G) {
+          int at = lane % per;                         // lanes start apart, so that they meet few of one another's banks
+          for (int i = 0; i < per; ++i) {
+            two = add_to(two, ws.choice[lane * per + at]);
+            at = at + 1 == per ? 0 : at + 1;
+          }
+        }
+        __syncwarp();
+      }
+      float worth = group < G ? (best == 2 && per > 1 ? two.a + two.b : two.a) : NAN;
+      unsigned kept = 0u;
+      float last = 0.f;
+      for (int r = 0; r <= M; ++r) {
+        const float all = lanes_max(worth);
+        if (r < M) {
+          const int src = __ffs(__ballot_sync(0xffffffffu, worth == all)) - 1;
+          kept |= 1u << __shfl_sync(0xffffffffu, group & 31, max(src, 0));
+          last = all;
+          if (lane == src) worth = NAN;
+        } else {
+          unsure = unsure || !(last - all > 2.f * eps * smax + kStep * fabsf(last));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (first + j < E && !((kept >> ((first + j) / per)) & 1u)) c[j] = NAN;
+    }
   }
 
   // Candidates: everything not below the L-th largest lane maximum, L = the ranks that are looked at (with a bias, whether the
   // last choice is clear of the first one left out).  At least L of them, hardly ever more than 2 L, whatever the order is.
-  const int ranks = K + (bias ? 1 : 0);
-  uint32_t head = key[0], floor_key = 1u;
+  const int ranks = K + (biased ? 1 : 0);
+  float head = c[0], floor_value = -INFINITY;
 #pragma unroll
-  for (int j = 1; j < kPer; ++j) head = max(head, key[j]);
+  for (int j = 1; j < kPer; ++j) head = fmaxf(head, c[j]);
   if (ranks <= 32) {
     for (int r = 0; r < ranks; ++r) {
-      floor_key = __reduce_max_sync(0xffffffffu, head);
-      if (head == floor_key) head = 0u;
+      floor_value = lanes_max(head);
+      if (head == floor_value) head = NAN;
     }
-    floor_key = max(floor_key, 1u);
+    if (floor_value != floor_value) floor_value = -INFINITY;
   }
   int n = 0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    const bool in = key[j] >= floor_key;
+    const bool in = c[j] >= floor_value;
     const unsigned mask = __ballot_sync(0xffffffffu, in);
-    const int at = n + __popc(mask & ((1u << lane) - 1u));
-    if (in && at < kCandidates) ws.candidate[at] = Pick{key[j], first + j, x[j], scored ? s[j] : 0.f};
+    if (in) ws.candidate[n + __popc(mask & ((1u << lane) - 1u))] = Pick{c[j], first + j};
     n += __popc(mask);
   }
-  if (n > kCandidates) unsure = true;
+  unsure = unsure || n > kCandidates || n < K;         // few: there are NaN among the logits
   if (!unsure) {
     __syncwarp();
-    Pick mine[2];
-    int rank[2] = {0, 0};
-    const Pick none{0u, 0, 0.f, 0.f};
-    mine[0] = lane < n ? ws.candidate[lane] : none;
-    mine[1] = lane + 32 < n ? ws.candidate[lane + 32] : none;
-    for (int q = 0; q < n; ++q) {
-      const uint2 other = *reinterpret_cast<const uint2*>(&ws.candidate[q]);
-      rank[0] += other.x > mine[0].key || (other.x == mine[0].key && (int)other.y < mine[0].id);
+    {
+      const Pick mine = lane < n ? ws.candidate[lane] : Pick{0.f, 0};
+      int rank = 0;
+#pragma unroll 4
+      for (int q = 0; q < n; ++q) {
+        const Pick o = ws.candidate[q];
+        rank += o.c > mine.c || (o.c == mine.c && o.id < mine.id);
+      }
+      if (lane < n && rank < ranks) ws.sorted[rank] = mine;
     }
     if (n > 32) {
+      const Pick mine = lane + 32 < n ? ws.candidate[lane + 32] : Pick{0.f, 0};
+      int rank = 0;
+#pragma unroll 4
       for (int q = 0; q < n; ++q) {
-        const uint2 other = *reinterpret_cast<const uint2*>(&ws.candidate[q]);
-        rank[1] += other.x > mine[1].key || (other.x == mine[1].key && (int)other.y < mine[1].id);
+        const Pick o = ws.candidate[q];
+        rank += o.c > mine.c || (o.c == mine.c && o.id < mine.id);
       }
+      if (lane + 32 < n && rank < ranks) ws.sorted[rank] = mine;
     }
-    if (lane < n && rank[0] < ranks) ws.sorted[rank[0]] = mine[0];
-    if (lane + 32 < n && rank[1] < ranks) ws.sorted[rank[1]] = mine[1];
     __syncwarp();
-    const Pick p = lane < K ? ws.sorted[lane] : none;
-    if (bias) {
+    const bool out = lane < K;
+    const Pick p = out ? ws.sorted[lane] : Pick{0.f, 0};
+    const float x = biased || grouped ? load_logit(row, p.id) : p.c;
+    float w = 0.f;
+    if (fn == kSoftmax) {
+      if (kScored) w = top == -INFINITY ? 0.f : expf(x - top) / denominator;
+    } else {
+      w = score_of(x, fn);
+    }
+    if (biased) {
       bool close = false;
-      if (lane < K && lane + 1 < min(n, ranks)) {
-        const Pick q = ws.sorted[lane + 1];
-        const float bp = bias[p.id], bq = bias[q.id], c = p.s + bp;
-        close = !(c - (q.s + bq) > eps * fmaxf(p.s, q.s) + kStep * fabsf(c)) && !(p.x == q.x && bp == bq);
+      if (out && lane + 1 < min(n, ranks)) {
+        const Pick q = ws.sorted[lane + 1];            // its score is at most its choice less its bias, give or take a step
+        const float bp = bias[p.id], bq = bias[q.id], xq = load_logit(row, q.id);
+        close = !(p.c - q.c > eps * fmaxf(w, fabsf(q.c - bq)) + kStep * (fabsf(p.c) + fabsf(bq))) && !(x == xq && bp == bq);
       }
       unsure = __any_sync(0xffffffffu, close);
     }
     if (!unsure) {
-      float w = 0.f;
-      if (lane < K) w = scored ? p.s : (fn == kSoftmax ? 0.f : score_of(p.x, fn));
+      if (!out) w = 0.f;
       if (renorm) {
         if (fn == kSoftmax) {
-          const float m = warp_maxf(lane < K ? p.x : -INFINITY);
-          w = lane >= K || (m == -INFINITY && p.x == p.x) ? 0.f : expf(p.x - m);
+          const float m = kScored ? warp_maxf(out ? x : -INFINITY) : __shfl_sync(0xffffffffu, x, 0);
+          w = !out || (m == -INFINITY) ? 0.f : expf(x - m);
         }
         w = w / (warp_sum(w) + 1e-20f);
       }
-      if (lane < K) {
+      if (out) {
         weights[t * K + lane] = w * alpha;
         indices[t * K + lane] = p.id;
       }
@@ -504,13 +512,20 @@ extern "C" int b2g_route_experts(const void* logits, int64_t ld, int logits_dtyp
   B2G_REQUIRE(weights && indices, "route_experts: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int blocks = (int)((T + experts::kWarps - 1) / experts::kWarps);
-#define B2G_ROUTE(PER)                                                                                                                  \
-  if (logits_dtype)                                                                                                                     \
-    experts::route_kernel<float, PER><<<blocks, experts::kWarps * 32, 0, s>>>(static_cast<const float*>(logits), ld, bias, score_fn, groups, \
-        top_groups, group_experts, renormalize, scaling, weights, indices, T, E, top_k);                                                \
-  else                                                                                                                                  \
-    experts::route_kernel<__nv_bfloat16, PER><<<blocks, experts::kWarps * 32, 0, s>>>(static_cast<const __nv_bfloat16*>(logits), ld, bias, \
-        score_fn, groups, top_groups, group_experts, renormalize, scaling, weights, indices, T, E, top_k)
+  const bool scored = bias || top_groups < groups || (score_fn == experts::kSoftmax && !renormalize);
+#define B2G_ROUTE_AS(TYPE, PER, SCORED)                                                                                                \
+  experts::route_kernel<TYPE, PER, SCORED><<<blocks, experts::kWarps * 32, 0, s>>>(static_cast<const TYPE*>(logits), ld, bias, score_fn, groups, \
+      top_groups, group_experts, renormalize, scaling, weights, indices, T, E, top_k)
+#define B2G_ROUTE(PER)                                                   \
+  do {                                                                   \
+    if (logits_dtype) {                                                  \
+      if (scored) B2G_ROUTE_AS(float, PER, true);                        \
+      else B2G_ROUTE_AS(float, PER, false);                              \
+    } else {                                                             \
+      if (scored) B2G_ROUTE_AS(__nv_bfloat16, PER, true);                \
+      else B2G_ROUTE_AS(__nv_bfloat16, PER, false);                      \
+    }                                                                    \
+  } while (0)
   B2G_BY_EXPERTS(E, B2G_ROUTE);
   B2G_CUDA_OK(cudaGetLastError());
   return 0;
