@@ -37,11 +37,43 @@ __device__ __forceinline__ float ex2(float x) {
 // which times the spread of the logits would reach every log-probability with the same sign).  fp32 logits, whose gradient
 // keeps 24 bits, take the full exponential; they move twice the bytes per value, so it is as well hidden.
 struct Scale { float hi, lo, inv; };
-template <typename T>
-__device__ __forceinline__ float exp_from(float z, float m, const Scale& c) {
-  const float x = z - m;
-  if constexpr (sizeof(T) == 2) return ex2(fmaf(x, c.hi, x * c.lo));
-  else return expf(x * c.inv);
+// Two floats in one 64-bit register pair: one instruction of the two-wide fp32 pipe each.
+struct F2 { uint64_t v; };
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// A pair of exponentials.  kSum: for the sum, where the factor's second part counts; a 16-bit cotangent is good without it.
+template <typename T, bool kSum>
+__device__ __forceinline__ F2 exp_from(F2 z, F2 minus_m, const Scale& c) {
+  const F2 x = z + minus_m;
+  float lo, hi;
+  if constexpr (sizeof(T) == 2) {
+    const F2 h = f2(c.hi, c.hi);
+    split(kSum ? fma2(x, h, x * f2(c.lo, c.lo)) : x * h, lo, hi);
+    return f2(ex2(lo), ex2(hi));
+  } else {
+    split(x * f2(c.inv, c.inv), lo, hi);
+    return f2(expf(lo), expf(hi));
+  }
 }
 // The sum without ex2's shortfall; the largest term is exp(0), which is exact.
 template <typename T>
@@ -56,11 +88,53 @@ struct Vec {
     if constexpr (sizeof(T) == 2) return (i & 1) ? dev::bf16_hi(w[i >> 1]) : dev::bf16_lo(w[i >> 1]);
     else return __uint_as_float(w[i]);
   }
+  // pair i of the N / 2
+  __device__ __forceinline__ F2 pair(int i) const {
+    if constexpr (sizeof(T) == 2) return f2(dev::bf16_lo(w[i]), dev::bf16_hi(w[i]));
+    else return f2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  }
   __device__ __forceinline__ void set_nothing() {   // -inf everywhere: the maximum and the sum do not see it
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;
   }
 };
+
+// Sum of exponentials of a vector, summed as a tree.
+template <typename T>
+__device__ __forceinline__ F2 exp_sum(const Vec<T>& x, F2 minus_m, const Scale& c) {
+  constexpr int P = Vec<T>::N / 2;
+  F2 e[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) e[i] = exp_from<T, true>(x.pair(i), minus_m, c);
+#pragma unroll
+  for (int s = P / 2; s > 0; s >>= 1)
+#pragma unroll
+    for (int i = 0; i < s; ++i) e[i] = e[i] + e[i + s];
+  return e[0];
+}
+__device__ __forceinline__ float sum_of(F2 a) {
+  float lo, hi;
+  split(a, lo, hi);
+  return lo + hi;
+}
+
+// factor * exponentials of a vector, in the logits' type.
+template <typename T>
+__device__ __forceinline__ Vec<T> scaled_exp(const Vec<T>& x, F2 minus_m, F2 factor, const Scale& c) {
+  Vec<T> r;
+#pragma unroll
+  for (int i = 0; i < Vec<T>::N / 2; ++i) {
+    float lo, hi;
+    split(exp_from<T, false>(x.pair(i), minus_m, c) * factor, lo, hi);
+    if constexpr (sizeof(T) == 2) {
+      r.w[i] = dev::pack_bf16(lo, hi);
+    } else {
+      r.w[2 * i] = __float_as_uint(lo);
+      r.w[2 * i + 1] = __float_as_uint(hi);
+    }
+  }
+  return r;
+}
 
 // A row as 16-byte vectors of the memory it lies in: vector v holds the columns [v * N - shift, (v + 1) * N - shift), so the
 // inner vectors are aligned whatever the row's own alignment is, and at most the first and the last one are partial.
@@ -68,13 +142,15 @@ template <typename T>
 struct Row {
   static constexpr int N = Vec<T>::N;
   const T* x;
-  int shift, nvec;
-  int64_t V;
-  __device__ Row(const T* p, int64_t V_) : x(p), shift((int)((reinterpret_cast<uintptr_t>(p) / sizeof(T)) % N)), V(V_) {
-    nvec = (int)((V + shift + N - 1) / N);
+  int shift, nvec, first_full, full_end;
+  int V;
+  __device__ Row(const T* p, int64_t width) : x(p), shift((int)((reinterpret_cast<uintptr_t>(p) / sizeof(T)) % N)), V((int)width) {
+    nvec = (int)((width + shift + N - 1) / N);
+    first_full = shift ? 1 : 0;
+    full_end = (int)((width + shift) / N);
   }
   __device__ __forceinline__ int64_t column(int v) const { return (int64_t)v * N - shift; }
-  __device__ __forceinline__ bool full(int v) const { return column(v) >= 0 && column(v) + N <= V; }
+  __device__ __forceinline__ bool full(int v) const { return v >= first_full && v < full_end; }
   __device__ __forceinline__ Vec<T> load(int v) const {
     Vec<T> r;
     if (full(v)) {
@@ -97,24 +173,28 @@ struct Row {
     }
     return r;
   }
-  // Writes g[0..N) to the same columns of `out`; `wide`: out is aligned as the row is.
-  __device__ __forceinline__ void store(T* out, int v, const float (&g)[N], bool wide) const {
+  // Writes a vector to the same columns of `out`; `wide`: out is aligned as the row is.
+  __device__ __forceinline__ void store(T* out, int v, const Vec<T>& g, bool wide) const {
     if (wide && full(v)) {
-      uint4 q;
-      if constexpr (sizeof(T) == 2)
-        q = make_uint4(dev::pack_bf16(g[0], g[1]), dev::pack_bf16(g[2], g[3]), dev::pack_bf16(g[4], g[5]), dev::pack_bf16(g[6], g[7]));
-      else
-        q = make_uint4(__float_as_uint(g[0]), __float_as_uint(g[1]), __float_as_uint(g[2]), __float_as_uint(g[3]));
-      __stcs(reinterpret_cast<uint4*>(out + column(v)), q);
+      __stcs(reinterpret_cast<uint4*>(out + column(v)), make_uint4(g.w[0], g.w[1], g.w[2], g.w[3]));
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int64_t c = column(v) + i;
-        if (c >= 0 && c < V) out[c] = from_float<T>(g[i]);
+        if (c >= 0 && c < V) {
+          if constexpr (sizeof(T) == 2) out[c] = __ushort_as_bfloat16((unsigned short)((i & 1) ? g.w[i >> 1] >> 16 : g.w[i >> 1] & 0xFFFFu));
+          else out[c] = __uint_as_float(g.w[i]);
+        }
       }
     }
   }
 };
+template <typename T>
+__device__ __forceinline__ Vec<T> zeros() {
+  Vec<T> z;
+  z.w[0] = z.w[1] = z.w[2] = z.w[3] = 0u;
+  return z;
+}
 template <typename T>
 __device__ __forceinline__ bool same_alignment(const T* a, const T* b) {
   return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
@@ -125,6 +205,7 @@ struct RowArgs {
   const int64_t* target;
   int64_t V, ignore_index;
   float tau;
+  double inv_tau;
   Scale c;
   int* status;
   // log-probabilities
@@ -150,17 +231,26 @@ __device__ __forceinline__ Given given(const RowArgs& a, int64_t row) {
   return Given{a.weight ? a.weight[row] : 1.f, a.advantage[row], a.old_logp ? a.old_logp[row] : 0.f, a.ref_logp ? a.ref_logp[row] : 0.f};
 }
 
-// What a row's maximum, sum and target logit say.  `rest` is 1 - p of the target, the entry of the cotangent that cancels when
-// the target is nearly certain.  16-bit logits take it from the 64-bit log-probability; fp32 logits from z/tau, m/tau and lse
-// rounded to 32 bits, as the elementary form of the gradient in that type does (off by half a step of lse).  A vocabulary
-// masked throughout by the type's lowest value has an lse that holds no log d any more and stays with 64 bits.
+// 1 - p of the target, the entry of the cotangent that cancels when the target is nearly certain.  16-bit logits take the exact
+// value; fp32 logits take it from z/tau and lse rounded to 32 bits, as the elementary form of the gradient in that type does (off
+// by half a step of lse), unless lse is so large (a vocabulary masked throughout by the type's lowest value) that it holds no
+// log d any more.
+template <typename T>
+__device__ __forceinline__ float rest_of(double exact, float zy, double logp, float tau) {
+  if (sizeof(T) == 2) return (float)exact;
+  const float z = zy / tau, lse = (float)((double)z - logp);
+  return fabsf(lse) < 16384.f ? 1.f - expf(z - lse) : (float)exact;
+}
+
+// What a row's maximum, sum and target logit say.
 struct Scalars { double lse, logp; float rest; };
 template <typename T>
-__device__ __forceinline__ Scalars row_scalars(float m, double d, float zy, float tau) {
+__device__ __forceinline__ Scalars row_scalars(float m, double d, float zy, const RowArgs& a) {
   Scalars s;
-  s.lse = (double)m / (double)tau + log(d);
-  s.logp = ((double)zy - (double)m) / (double)tau - log(d);
-  s.rest = sizeof(T) == 4 && fabs(s.lse) < 16384.0 ? 1.f - expf(zy / tau - (float)((double)(m / tau) + log(d))) : (float)-expm1(s.logp);
+  const double log_d = log(d);
+  s.lse = (double)m * a.inv_tau + log_d;
+  s.logp = ((double)zy - (double)m) * a.inv_tau - log_d;
+  s.rest = rest_of<T>(-expm1(s.logp), zy, s.logp, a.tau);
   return s;
 }
 
@@ -193,10 +283,15 @@ __device__ __forceinline__ float policy_scalars(const RowArgs& a, const Given& i
 // A maximum and the sum of exponentials against it.  The maximum starts at the type's lowest value, not at -inf, so that -inf
 // logits (a masked vocabulary) meet a finite maximum: exp(-inf - lowest) = 0.
 struct Stat { float m; double d; };
-__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float tau) {
-  const float m = fmaxf(a.m, b.m);
-  const double da = a.m == m ? a.d : a.d * exp(((double)a.m - m) / tau), db = b.m == m ? b.d : b.d * exp(((double)b.m - m) / tau);
-  return Stat{m, da + db};
+
+// The joint statistic of `count` lanes (a power of two), in every one of them.
+__device__ __forceinline__ Stat join_lanes(Stat s, int count, double inv_tau) {
+  float m = s.m;
+  for (int o = count / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (s.m != m) s.d *= exp(((double)s.m - (double)m) * inv_tau);
+  s.m = m;
+  for (int o = count / 2; o > 0; o >>= 1) s.d += __shfl_xor_sync(0xffffffffu, s.d, o);
+  return s;
 }
 
 // ---- rows held on chip ----------------------------------------------------------------------------
@@ -237,12 +332,11 @@ __device__ __forceinline__ float vec_max(const Vec<T>& x, float m) {
 }
 
 template <typename T, int kThreads, bool kPolicy>
-__global__ void __launch_bounds__(kThreads, 1536 / kThreads) held_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out,
+__global__ void __launch_bounds__(kThreads, 8) held_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out,
                                                                          int cluster) {
   constexpr int N = Vec<T>::N, kWarps = kThreads / 32;
   extern __shared__ __align__(16) uint8_t slice[];
-  __shared__ float warp_m[kWarps];
-  __shared__ double warp_d[kWarps];
+  __shared__ Stat warp_stat[kWarps];
   __shared__ Stat slot[8];
   __shared__ float4 bcast;
   const int rank = blockIdx.x % cluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -264,10 +358,8 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads) held_kernel(const T
       if (kPolicy) { a.loss[r] = 0.f; a.kl[r] = 0.f; static_cast<float*>(a.logp)[r] = 0.f; }
       else put_logp(a, r, 0.0, make_float4(0.f, 0.f, 0.f, 0.f));
     }
-    if (kPolicy) {
-      const float zero[N] = {};
-      for (int v = begin + threadIdx.x; v < end; v += kThreads) row.store(o, v, zero, wide);
-    }
+    if (kPolicy)
+      for (int v = begin + threadIdx.x; v < end; v += kThreads) row.store(o, v, zeros<T>(), wide);
     return;
   }
 
@@ -275,13 +367,16 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads) held_kernel(const T
   const int v0 = begin + threadIdx.x, n = v0 < end ? (end - v0 + kThreads - 1) / kThreads : 0;
   const uint32_t mine = dev::smem_u32(slice) + threadIdx.x * 16;
   const int group = (per + kThreads * kGroups - 1) / (kThreads * kGroups);
+  const T* const base = row.x - row.shift;          // vector v lies at base + v * N
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    for (int i = g * group; i < min(n, (g + 1) * group); ++i) {
+    const int stop = min(n, (g + 1) * group);
+#pragma unroll 4
+    for (int i = g * group; i < stop; ++i) {
       const int v = v0 + i * kThreads;
       const uint32_t at = mine + i * (kThreads * 16);
       if (row.full(v)) {
-        copy16(at, row.x + row.column(v));
+        copy16(at, base + (int64_t)v * N);
       } else {
         const Vec<T> x = row.load(v);
         dev::sts128(at, x.w[0], x.w[1], x.w[2], x.w[3]);
@@ -293,8 +388,9 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads) held_kernel(const T
 
   float m = kLowest;
   auto max_of = [&](int g) {
+    const int stop = min(n, (g + 1) * group);
 #pragma unroll 4
-    for (int i = g * group; i < min(n, (g + 1) * group); ++i) m = vec_max(from_shared<T>(mine + i * (kThreads * 16)), m);
+    for (int i = g * group; i < stop; ++i) m = vec_max(from_shared<T>(mine + i * (kThreads * 16)), m);
   };
   copy_wait<3>(); max_of(0);
   copy_wait<2>(); max_of(1);
@@ -302,68 +398,464 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads) held_kernel(const T
   copy_wait<0>(); max_of(3);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-  if (lane == 0) warp_m[warp] = m;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) m = fmaxf(m, warp_m[i]);
 
-  // eight (four) terms are summed in 32 bits, everything above them in 64
+  // Every warp sums against its own maximum, so no barrier comes first.  The terms of two vectors are summed in 32 bits,
+  // everything above them in 64.
   const Scale c = a.c;
   double d = 0.0;
+  {
+    const F2 minus_m = f2(-m, -m);
+    int i = 0;
 #pragma unroll 2
-  for (int i = 0; i < n; ++i) {
-    const Vec<T> x = from_shared<T>(mine + i * (kThreads * 16));
-    float e[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) e[j] = exp_from<T>(x.get(j), m, c);
-#pragma unroll
-    for (int s = N / 2; s > 0; s >>= 1)
-#pragma unroll
-      for (int j = 0; j < s; ++j) e[j] += e[j + s];
-    d += (double)e[0];
+    for (; i + 1 < n; i += 2)
+      d += (double)sum_of(exp_sum(from_shared<T>(mine + i * (kThreads * 16)), minus_m, c) +
+                          exp_sum(from_shared<T>(mine + (i + 1) * (kThreads * 16)), minus_m, c));
+    if (i < n) d += (double)sum_of(exp_sum(from_shared<T>(mine + i * (kThreads * 16)), minus_m, c));
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-  if (lane == 0) warp_d[warp] = d;
+  if (lane == 0) warp_stat[warp] = Stat{m, d};
   __syncthreads();
-  if (threadIdx.x < cluster) {              // thread k gives this CTA's share to CTA k
-    d = 0.0;
-    for (int i = 0; i < kWarps; ++i) d += warp_d[i];
-    const uint32_t to = dev::map_to_cta(dev::smem_u32(&slot[rank]), threadIdx.x);
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(m) : "memory");
-    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to + 8), "d"(d) : "memory");
+  if (warp == 0) {
+    Stat t = join_lanes(lane < kWarps ? warp_stat[lane] : Stat{kLowest, 0.0}, kWarps, a.inv_tau);
+    t.m = __shfl_sync(0xffffffffu, t.m, 0);   // a CTA of few warps has the sum in fewer lanes than the cluster has CTAs
+    t.d = __shfl_sync(0xffffffffu, t.d, 0);
+    if (lane < cluster) {                     // lane k gives this CTA's share to CTA k
+      const uint32_t to = dev::map_to_cta(dev::smem_u32(&slot[rank]), lane);
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(t.m) : "memory");
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to + 8), "d"(t.d) : "memory");
+    }
   }
   dev::cluster_sync_all();
-  if (threadIdx.x == 0) {
-    Stat t = slot[0];
-    for (int i = 1; i < cluster; ++i) t = join(t, slot[i], a.tau);
-    t.d = whole_sum<T>(t.d);
-    const Scalars v = row_scalars<T>(t.m, t.d, zy, a.tau);
-    if (kPolicy) {
-      const float coef = policy_scalars(a, in, v.logp, r, rank == 0) / a.tau;
-      bcast = make_float4(coef, (float)(coef / t.d), t.m, coef * v.rest);
-    } else if (rank == 0) {
-      put_logp(a, r, v.logp, make_float4(t.m, (float)(1.0 / t.d), v.rest, (float)v.lse));
+  if (warp == 0) {
+    Stat t = join_lanes(lane < cluster ? slot[lane] : Stat{kLowest, 0.0}, cluster, a.inv_tau);
+    if (lane == 0) {
+      t.d = whole_sum<T>(t.d);
+      const Scalars v = row_scalars<T>(t.m, t.d, zy, a);
+      if (kPolicy) {
+        const float coef = (float)(policy_scalars(a, in, v.logp, r, rank == 0) * a.inv_tau);
+        bcast = make_float4(coef, (float)(-coef / t.d), t.m, coef * v.rest);
+      } else if (rank == 0) {
+        put_logp(a, r, v.logp, make_float4(t.m, (float)(1.0 / t.d), v.rest, (float)v.lse));
+      }
     }
   }
   if (!kPolicy) return;
   __syncthreads();
-  const float coef = bcast.x, k = bcast.y, top = bcast.z, at_target = bcast.w;
-  const int vy = (int)((y + row.shift) / N), jy = (int)((y + row.shift) % N);
+  const float coef = bcast.x;
+  if (coef == 0.f) {                          // clipped: nothing of the row is wanted
+    for (int i = 0; i < n; ++i) row.store(o, v0 + i * kThreads, zeros<T>(), wide);
+    return;
+  }
+  const F2 factor = f2(bcast.y, bcast.y), minus_m = f2(-bcast.z, -bcast.z);
+  T* const to = o - row.shift;
 #pragma unroll 2
   for (int i = 0; i < n; ++i) {
     const int v = v0 + i * kThreads;
-    const Vec<T> x = from_shared<T>(mine + i * (kThreads * 16));
-    float g[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) g[j] = coef == 0.f ? 0.f : -k * exp_from<T>(x.get(j), top, c);
-    if (v == vy && coef != 0.f) {
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (j == jy) g[j] = at_target;
-    }
-    row.store(o, v, g, wide);
+    const Vec<T> g = scaled_exp(from_shared<T>(mine + i * (kThreads * 16)), minus_m, factor, c);
+    if (wide && row.full(v)) __stcs(reinterpret_cast<uint4*>(to + (int64_t)v * N), make_uint4(g.w[0], g.w[1], g.w[2], g.w[3]));
+    else row.store(o, v, g, wide);
   }
+  const int vy = (int)((y + row.shift) / N);  // its writer puts the target's entry right
+  if (vy >= v0 && vy < end && (vy - v0) % kThreads == 0) o[y] = from_float<T>(bcast.w);
+}
+
+// ---- rows in a pipeline ------------------------------------------------------------------------------
+// One CTA per SM, clusters that stay and go from row to row, `slots` slices of rows in shared memory.  15 warps work, one more
+// does everything that is latency.  For every row k:
+//   the scalar warp reads 128 samples and the target's logit, and publishes their maximum as the row's reference: a sum of
+//     exponentials in 32 bits needs no more than a reference within 80 tau of the maximum (rows where that fails are summed
+//     once more, below), so the workers need no pass for the maximum and all their sums simply add up;
+//   S(k): the workers' sums of exp((z - reference)/tau) over everything but the target, one pair of numbers per thread;
+//   the scalar warp adds them up, sends the CTA's share to the others of the cluster (asynchronous remote stores that count on
+//     their barrier), adds theirs, finishes the row's scalars and lets the workers know;
+//   G(k), the cotangent, only `lead` rows after S(k): the workers never wait for the exchange.
+// The target's own term is added in 64 bits: where it dominates, nothing of the small rest is lost to its rounding, and 1 - p
+// is the rest's share without a cancellation.
+// Every vector is private to one thread: it copies it in (cp.async), reads it in S and in G, and copies the vector of the row
+// `slots` further on into the same place.
+// A sum that is no number, or 0 (a reference too low by 88 tau, NaN, +inf, a vocabulary masked by the type's lowest value) is
+// made again against the true maximum, by the scalar warps alone, and G then takes the exact form of the exponent.
+// All waits are bounded; a CTA whose wait ran out stops working, and all CTAs of a cluster leave together.
+#ifndef WW
+#define WW 19
+#endif
+constexpr int kWorkerWarps = WW, kWorkers = kWorkerWarps * 32, kRing = 8, kMaxCluster = 10, kMaxSlots = 4, kMaxLead = 3, kAhead = 7, kInfo = 16, kSamples = 4;
+
+struct Share { float m, unused; double d; };       // what a CTA sends: its sum and what it is against
+
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int where) {
+  for (uint32_t spin = 0; spin < B2G_SPIN_LIMIT; ++spin) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((spin & 255u) == 255u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  if (status) atomicCAS(status, 0, where);
+  return false;
+}
+__device__ __forceinline__ void send_share(uint32_t to, uint32_t bar, const Share& s) {
+  const uint64_t lo = __float_as_uint(s.m), hi = (uint64_t)__double_as_longlong(s.d);
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(to), "l"(lo), "l"(hi), "r"(bar)
+               : "memory");
+}
+// The first and the last vector of a row, where they are partial: out of line, they are few.
+template <typename T>
+__device__ __noinline__ void fetch_edge(const T* x, int64_t V, int v, uint32_t at) {
+  const Vec<T> w = Row<T>(x, V).load(v);
+  dev::sts128(at, w.w[0], w.w[1], w.w[2], w.w[3]);
+}
+template <typename T>
+__device__ __noinline__ void store_edge(const T* x, int64_t V, int v, T* out, Vec<T> w) { Row<T>(x, V).store(out, v, w, false); }
+
+// A row's part of one warp: vectors [begin, end), of which those in [full_begin, full_end) are whole; lane l reads begin + l + 32 i,
+// i < n.  Rows whose pitch is a multiple of 16 bytes all have the same one.
+template <typename T>
+struct Part {
+  static constexpr int N = Vec<T>::N;
+  int shift, full_begin, full_end, end, n;
+  __device__ __forceinline__ Part(const T* x, uint32_t V, int begin, int limit, int lane) {
+    shift = (int)((uint32_t)reinterpret_cast<uintptr_t>(x) & 15u) / (int)sizeof(T);
+    const uint32_t width = V + shift;
+    full_begin = max(begin, shift != 0 ? 1 : 0);
+    end = min(limit, (int)((width + N - 1) / N));
+    full_end = min(end, (int)(width / N));
+    n = end > begin + lane ? (end - 1 - begin - lane) / 32 + 1 : 0;
+  }
+  __device__ __forceinline__ bool full(int v) const { return v >= full_begin && v < full_end; }
+  // One lane: the whole vectors as one bulk copy that counts on `bar`, the partial ones by hand.  `at`: place of vector `begin`.
+  __device__ __forceinline__ void fetch(const T* x, int begin, uint32_t at, uint32_t bar, int64_t V) const {
+    const int whole = max(0, full_end - full_begin);
+    dev::mbar_arrive_expect_tx(bar, (uint32_t)whole * 16);
+    if (whole)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at + (full_begin - begin) * 16),
+                   "l"(x - shift + (int64_t)full_begin * N), "r"(whole * 16), "r"(bar)
+                   : "memory");
+    for (int v = begin; v < min(full_begin, end); ++v) fetch_edge(x, V, v, at + (v - begin) * 16);
+    for (int v = max(full_end, full_begin); v < end; ++v) fetch_edge(x, V, v, at + (v - begin) * 16);
+  }
+  // index i of this lane's vector that holds column y, or -1
+  __device__ __forceinline__ int owns(int y, int begin, int lane) const {
+    const int v = (int)((uint32_t)(y + shift) / N), k = v - begin - lane;
+    return k >= 0 && v < end && k % 32 == 0 ? k / 32 : -1;
+  }
+};
+
+// What the workers need to know of a row: what to sum against, and its target, or -1 where it takes no part.
+struct Info { float reference; int y; };
+
+// 2^(z c - reference) as pairs: two fused steps, the exponent rounded where it is small.
+__device__ __forceinline__ F2 ex2_pair(F2 t) {
+  float lo, hi;
+  split(t, lo, hi);
+  return f2(ex2(lo), ex2(hi));
+}
+// What the workers sum against: bf16 in units of log2 (any number serves, so its rounding costs nothing), fp32 as a logit.
+template <typename T>
+__device__ __forceinline__ float reference_of(float m, const Scale& c) {
+  return sizeof(T) == 2 ? fminf(fmaxf(m * c.hi, -3e38f), 3e38f) : fmaxf(m, kLowest);
+}
+template <typename T>
+__device__ __forceinline__ F2 sum_vec(const Vec<T>& x, F2 minus_ref, const Scale& c) {
+  constexpr int P = Vec<T>::N / 2;
+  F2 e[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if constexpr (sizeof(T) == 2) e[i] = ex2_pair(fma2(x.pair(i), f2(c.lo, c.lo), fma2(x.pair(i), f2(c.hi, c.hi), minus_ref)));
+    else e[i] = exp_from<T, true>(x.pair(i), minus_ref, c);
+  }
+#pragma unroll
+  for (int s = P / 2; s > 0; s >>= 1)
+#pragma unroll
+    for (int i = 0; i < s; ++i) e[i] = e[i] + e[i + s];
+  return e[0];
+}
+template <typename T>
+__device__ __forceinline__ Vec<T> cotangent_vec(const Vec<T>& x, F2 minus_ref, F2 factor, const Scale& c) {
+  if constexpr (sizeof(T) == 4) {
+    return scaled_exp(x, minus_ref, factor, c);
+  } else {
+    Vec<T> r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float lo, hi;
+      split(ex2_pair(fma2(x.pair(i), f2(c.hi, c.hi), minus_ref)) * factor, lo, hi);
+      r.w[i] = dev::pack_bf16(lo, hi);
+    }
+    return r;
+  }
+}
+
+// One warp's sum over columns [begin, end) of a row but for column y, against their maximum.
+template <typename T>
+__device__ __noinline__ Stat sum_again(const T* x, int begin, int end, int y, const RowArgs& a) {
+  const int lane = threadIdx.x & 31;
+  float m = kLowest;
+  for (int i = begin + lane; i < end; i += 32) m = fmaxf(m, to_float(x[i]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  double d = 0.0;
+  for (int i = begin + lane; i < end; i += 32)
+    if (i != y) d += exp(((double)to_float(x[i]) - (double)m) * a.inv_tau);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  return Stat{m, d};
+}
+
+template <typename T, bool kPolicy>
+__global__ void __launch_bounds__(kWorkers + 64, 1) pipe_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out, int64_t rows,
+                                                                int cluster, int slots, int lead, int per, int per_warp) {
+  constexpr int N = Vec<T>::N, kStep = 32 * 16;
+  extern __shared__ __align__(16) uint8_t space[];
+  __shared__ uint64_t arrived[kMaxSlots][kWorkerWarps];      // one per slot and warp: a warp's copies are its own
+  __shared__ __align__(16) Share share[2][kRing][kMaxCluster];
+  __shared__ double sums[kRing][kWorkerWarps];
+  __shared__ __align__(8) Info info[kInfo];
+  __shared__ float2 known[kInfo];                // the samples' maximum and the target's logit
+  __shared__ float4 bcast[kRing];
+  __shared__ int exact_form[kRing];
+  __shared__ uint64_t referred[kInfo], summed[kRing], joined[2][kRing], ready[kRing];
+  __shared__ int gave_up;
+  const int rank = blockIdx.x % cluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t first = blockIdx.x / cluster, stride = gridDim.x / cluster;
+  const int count = (int)((rows - first + stride - 1) / stride);       // rows of this cluster: first + k * stride
+  if (threadIdx.x == 0) {
+    gave_up = 0;
+    for (int i = 0; i < kInfo; ++i) dev::mbar_init(dev::smem_u32(&referred[i]), 1);
+    for (int i = 0; i < kMaxSlots * kWorkerWarps; ++i) dev::mbar_init(dev::smem_u32(&arrived[0][i]), 1);
+    for (int i = 0; i < kRing; ++i) {
+      dev::mbar_init(dev::smem_u32(&summed[i]), kWorkerWarps);
+      dev::mbar_init(dev::smem_u32(&joined[0][i]), 1);
+      dev::mbar_init(dev::smem_u32(&joined[1][i]), 1);
+      dev::mbar_init(dev::smem_u32(&ready[i]), 1);
+    }
+    dev::fence_barrier_init();
+  }
+  dev::cluster_sync_all();          // nobody sends to a barrier that is not there yet
+
+  if (warp == kWorkerWarps) {       // references, and the CTA's share
+    const Scale c = a.c;
+    const int64_t apart = a.V / (32 * kSamples);
+    float sample[kSamples], target_logit = 0.f;
+    int y_ahead = -1;
+    auto look_at = [&](int k) {     // issue the loads of row k's reference
+      if (k >= count) return;
+      const int64_t r = first + k * stride;
+      const T* x = logits + r * ld;
+#pragma unroll
+      for (int i = 0; i < kSamples; ++i) sample[i] = to_float(x[(lane * kSamples + i) * apart]);
+      const int64_t y = a.target[r];
+      const bool in_range = y >= 0 && y < a.V;
+      target_logit = in_range ? to_float(x[y]) : -INFINITY;
+      y_ahead = in_range && y != a.ignore_index && !(kPolicy && a.weight && a.weight[r] == 0.f) ? (int)y : -1;
+    };
+    auto refer = [&](int k) {
+      if (k >= count) return;
+      float m = fmaxf(kLowest, target_logit);
+#pragma unroll
+      for (int i = 0; i < kSamples; ++i) m = fmaxf(m, sample[i]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (lane == 0) {
+        info[k % kInfo] = Info{reference_of<T>(m, c), y_ahead};
+        known[k % kInfo] = make_float2(m, target_logit);
+        dev::mbar_arrive(dev::smem_u32(&referred[k % kInfo]));
+      }
+    };
+    for (int k = 0; k < kAhead; ++k) {
+      look_at(k);
+      refer(k);
+    }
+    for (int k = 0; k < count; ++k) {
+      const int p = k % kRing, parity = (k / kRing) & 1;
+      look_at(k + kAhead);
+      if (!dev::mbar_wait(dev::smem_u32(&summed[p]), parity, &gave_up, a.status, 501)) break;
+      double d = lane < kWorkerWarps ? sums[p][lane] : 0.0;      // of a row that takes no part nobody looks at it
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      if (lane < cluster)
+        send_share(dev::map_to_cta(dev::smem_u32(&share[0][p][rank]), lane), dev::map_to_cta(dev::smem_u32(&joined[0][p]), lane), Share{0.f, 0.f, d});
+      refer(k + kAhead);
+    }
+  } else if (warp == kWorkerWarps + 1) {       // the row's scalars
+    int again = 0;                  // rows that needed the second exchange
+    for (int k = 0; k < count; ++k) {
+      const int64_t r = first + k * stride, y = a.target[r];
+      const int p = k % kRing, parity = (k / kRing) & 1;
+      const uint32_t bar = dev::smem_u32(&joined[0][p]);
+      if (lane == 0) dev::mbar_arrive_expect_tx(bar, cluster * (uint32_t)sizeof(Share));
+      Given in{1.f, 0.f, 0.f, 0.f};
+      bool live = target_ok(y, a, rank == 0 && lane == 0);
+      if (kPolicy) {
+        in = given(a, r);
+        live = live && in.weight != 0.f;
+      }
+      if (!wait_cluster(bar, parity, &gave_up, a.status, 502)) break;
+      if (live) {
+        double d = lane < cluster ? share[0][p][lane].d : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        if (sizeof(T) == 2) d += d * kEx2Shortfall;
+        const float zy = known[k % kInfo].y;
+        float ref = info[k % kInfo].reference, m = known[k % kInfo].x;
+        // the target's own term
+        double own = sizeof(T) == 2 ? exp2((double)zy * (a.inv_tau * 1.4426950408889634) - (double)ref) : exp(((double)zy - (double)ref) * a.inv_tau);
+        bool exact = false;
+        if (!(own + d > 0.0 && own + d < 1e300)) {             // the same for every CTA: they added the same numbers
+          exact = true;
+          const int shift = (int)((uint32_t)reinterpret_cast<uintptr_t>(logits + r * ld) & 15u) / (int)sizeof(T);
+          const int64_t begin = (int64_t)rank * per * N - shift, end = min(a.V, (int64_t)(rank + 1) * per * N - shift);
+          const Stat s = sum_again(logits + r * ld, (int)(begin < 0 ? 0 : begin), (int)end, (int)y, a);
+          const int p2 = again % kRing, parity2 = (again / kRing) & 1;
+          const uint32_t bar2 = dev::smem_u32(&joined[1][p2]);
+          ++again;
+          if (lane == 0) dev::mbar_arrive_expect_tx(bar2, cluster * (uint32_t)sizeof(Share));
+          __syncwarp();
+          if (lane < cluster) send_share(dev::map_to_cta(dev::smem_u32(&share[1][p2][rank]), lane), dev::map_to_cta(bar2, lane), Share{s.m, 0.f, s.d});
+          if (!wait_cluster(bar2, parity2, &gave_up, a.status, 505)) break;
+          const Share got = lane < cluster ? share[1][p2][lane] : Share{kLowest, 0.f, 0.0};
+          const Stat t = join_lanes(Stat{got.m, got.d}, 32, a.inv_tau);
+          ref = m = t.m;
+          d = t.d;
+          own = exp(((double)zy - (double)m) * a.inv_tau);
+        }
+        const double logp = -log1p(d / own), all = own + d;
+        if (lane == 0) {
+          const float rest = rest_of<T>(d / all, zy, logp, a.tau);
+          if (kPolicy) {
+            const float coef = (float)(policy_scalars(a, in, logp, r, rank == 0) * a.inv_tau);
+            bcast[p] = make_float4(coef, (float)(-coef / all), ref, coef * rest);
+            exact_form[p] = exact;
+          } else if (rank == 0) {
+            // the backward pass takes exp((z - m)/tau) over a sum against the same m
+            const double lse = (exact || sizeof(T) == 4 ? (double)ref * a.inv_tau : (double)ref * 0.6931471805599453) + log(all);
+            put_logp(a, r, logp, make_float4(m, (float)exp((double)m * a.inv_tau - lse), rest, (float)lse));
+          }
+        }
+      } else if (rank == 0 && lane == 0) {
+        if (kPolicy) { a.loss[r] = 0.f; a.kl[r] = 0.f; static_cast<float*>(a.logp)[r] = 0.f; }
+        else put_logp(a, r, 0.0, make_float4(0.f, 0.f, 0.f, 0.f));
+      }
+      __syncwarp();
+      if (lane == 0) dev::mbar_arrive(dev::smem_u32(&ready[p]));
+    }
+  } else {
+    const int begin = rank * per + warp * per_warp, limit = min((rank + 1) * per, begin + per_warp), slot_bytes = per * 16;
+    const uint32_t base = dev::smem_u32(space) + warp * per_warp * 16, V = (uint32_t)a.V;
+    const Scale c = a.c;
+    const bool steady = (ld * (int64_t)sizeof(T)) % 16 == 0;
+    const T* const x0 = logits + first * ld;
+    const int64_t pitch = stride * ld;
+    Part<T> part(x0, V, begin, limit, lane);            // of the row at hand
+    auto look_up = [&](int k) { return info[k % kInfo]; };
+    auto wait_for = [&](int k) { return dev::mbar_wait(dev::smem_u32(&referred[k % kInfo]), (k / kInfo) & 1, &gave_up, a.status, 504); };
+    bool fine = true;
+    uint32_t phase = 0u;            // bit i: parity of the next arrival in slot i
+    for (int k = 0; k < min(slots, count) && fine; ++k) {
+      fine = wait_for(k);
+      const T* const x = x0 + k * pitch;
+      if (!steady) part = Part<T>(x, V, begin, limit, lane);
+      if (look_up(k).y >= 0 && lane == 0) part.fetch(x, begin, base + k * slot_bytes, dev::smem_u32(&arrived[k][warp]), a.V);
+      __syncwarp();
+    }
+    int s_slot = 0, g_slot = 0;
+    for (int k = 0; k < count + lead && fine; ++k) {
+      const int j = k - lead, q = (kPolicy ? j : k) + slots;      // G's row, and the row that takes the place freed in this turn
+      int slot = s_slot;                                          // the place at hand
+      if (k < count) {
+        const int p = k % kRing;
+        const Info row = look_up(k);
+        if (row.y >= 0) {
+          if (!steady) part = Part<T>(x0 + k * pitch, V, begin, limit, lane);
+          const uint32_t place = base + s_slot * slot_bytes + lane * 16;
+          if (!dev::mbar_wait(dev::smem_u32(&arrived[s_slot][warp]), phase >> s_slot & 1u, &gave_up, a.status, 506)) break;
+          phase ^= 1u << s_slot;
+          __syncwarp();                                 // partial vectors are lane 0's ordinary stores
+          const int mine = part.owns(row.y, begin, lane);
+          if (mine >= 0) {                              // the target's term is the scalar warp's
+            const uint32_t e = place + mine * kStep + ((row.y + part.shift) % N) * (uint32_t)sizeof(T);
+            if (sizeof(T) == 2) asm volatile("st.shared.u16 [%0], %1;" ::"r"(e), "h"((unsigned short)0xFF80) : "memory");
+            else asm volatile("st.shared.u32 [%0], %1;" ::"r"(e), "r"(0xFF800000u) : "memory");
+          }
+          const F2 minus_ref = f2(-row.reference, -row.reference);
+          F2 d = f2(0.f, 0.f);
+          int i = 0;
+#pragma unroll 2
+          for (; i + 1 < part.n; i += 2)
+            d = d + (sum_vec(from_shared<T>(place + i * kStep), minus_ref, c) + sum_vec(from_shared<T>(place + (i + 1) * kStep), minus_ref, c));
+          if (i < part.n) d = d + sum_vec(from_shared<T>(place + i * kStep), minus_ref, c);
+          float lo, hi;
+          split(d, lo, hi);
+          double all = (double)lo + (double)hi;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+          if (lane == 0) sums[p][warp] = all;
+        }
+        __syncwarp();
+        if (lane == 0) dev::mbar_arrive(dev::smem_u32(&summed[p]));
+        if (++s_slot == slots) s_slot = 0;
+      }
+
+      bool fill = false;
+      if (q >= slots && q < count) {
+        if (!wait_for(q)) break;
+        fill = look_up(q).y >= 0;
+      }
+      if (j >= 0) {
+        const int p = j % kRing;
+        if (!dev::mbar_wait(dev::smem_u32(&ready[p]), (j / kRing) & 1, &gave_up, a.status, 503)) break;
+        if (kPolicy) {
+          slot = g_slot;
+          const int y = look_up(j).y;
+          const float4 b = y >= 0 ? bcast[p] : make_float4(0.f, 0.f, 0.f, 0.f);
+          const T* const x = x0 + j * pitch;
+          T* const o = out + (first + j * stride) * ld_out;
+          if (!steady) part = Part<T>(x, V, begin, limit, lane);
+          const uint32_t place = base + g_slot * slot_bytes + lane * 16;
+          T* const to = o - part.shift;
+          const bool wide = same_alignment(x, (const T*)o);
+          auto put = [&](int v, const Vec<T>& w) {
+            if (wide && part.full(v)) __stcs(reinterpret_cast<uint4*>(to + (int64_t)v * N), make_uint4(w.w[0], w.w[1], w.w[2], w.w[3]));
+            else store_edge(x, a.V, v, o, w);
+          };
+          if (b.x == 0.f) {                     // a clipped token, a row that takes no part: nothing of the logits is wanted
+            for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, zeros<T>());
+          } else {
+            const F2 factor = f2(b.y, b.y), minus_ref = f2(-b.z, -b.z);
+            if (exact_form[p]) {
+              for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled_exp(from_shared<T>(place + i * kStep), minus_ref, factor, c));
+            } else {
+#pragma unroll 2
+              for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, cotangent_vec(from_shared<T>(place + i * kStep), minus_ref, factor, c));
+            }
+            if (part.owns(y, begin, lane) >= 0) o[y] = from_float<T>(b.w);              // its writer puts the target's entry right
+          }
+        }
+        if (++g_slot == slots) g_slot = 0;
+      }
+      if (fill) {                               // into the place that this warp is done with
+        const T* const x = x0 + q * pitch;
+        if (!steady) part = Part<T>(x, V, begin, limit, lane);
+        dev::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) part.fetch(x, begin, base + slot * slot_bytes, dev::smem_u32(&arrived[slot][warp]), a.V);
+        __syncwarp();
+      }
+    }
+    // the copies that are still on their way when a wait ran out have nowhere to go once the CTA has left
+    if (gave_up) {
+      for (int i = 0; i < slots; ++i)
+        for (uint32_t spin = 0; spin < (1u << 16) && !dev::mbar_try_wait(dev::smem_u32(&arrived[i][warp]), phase >> i & 1u); ++spin) {}
+    }
+  }
+  dev::cluster_sync_all();          // no CTA's memory goes before what was sent to it has come
 }
 
 // ---- rows of any width ----------------------------------------------------------------------------
@@ -372,8 +864,7 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads) held_kernel(const T
 template <typename T, bool kPolicy>
 __global__ void __launch_bounds__(512) wide_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out) {
   constexpr int N = Vec<T>::N, kThreads = 512, kWarps = kThreads / 32;
-  __shared__ float warp_m[kWarps];
-  __shared__ double warp_d[kWarps];
+  __shared__ Stat warp_stat[kWarps];
   __shared__ float4 bcast;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t r = blockIdx.x, y = a.target[r];
@@ -391,63 +882,43 @@ __global__ void __launch_bounds__(512) wide_kernel(const T* logits, int64_t ld, 
       if (kPolicy) { a.loss[r] = 0.f; a.kl[r] = 0.f; static_cast<float*>(a.logp)[r] = 0.f; }
       else put_logp(a, r, 0.0, make_float4(0.f, 0.f, 0.f, 0.f));
     }
-    if (kPolicy) {
-      const float zero[N] = {};
-      for (int v = threadIdx.x; v < row.nvec; v += kThreads) row.store(o, v, zero, wide);
-    }
+    if (kPolicy)
+      for (int v = threadIdx.x; v < row.nvec; v += kThreads) row.store(o, v, zeros<T>(), wide);
     return;
   }
   float m = kLowest;
-  for (int v = threadIdx.x; v < row.nvec; v += kThreads) {
-    const Vec<T> x = row.load(v);
-#pragma unroll
-    for (int j = 0; j < N; ++j) m = fmaxf(m, x.get(j));
-  }
+  for (int v = threadIdx.x; v < row.nvec; v += kThreads) m = vec_max(row.load(v), m);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-  if (lane == 0) warp_m[warp] = m;
-  __syncthreads();
-  for (int i = 0; i < kWarps; ++i) m = fmaxf(m, warp_m[i]);
   const Scale c = a.c;
   double d = 0.0;
-  for (int v = threadIdx.x; v < row.nvec; v += kThreads) {
-    const Vec<T> x = row.load(v);
-    float e = 0.f;
-#pragma unroll
-    for (int j = 0; j < N; ++j) e += exp_from<T>(x.get(j), m, c);
-    d += (double)e;
-  }
+  for (int v = threadIdx.x; v < row.nvec; v += kThreads) d += (double)sum_of(exp_sum(row.load(v), f2(-m, -m), c));
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-  if (lane == 0) warp_d[warp] = d;
+  if (lane == 0) warp_stat[warp] = Stat{m, d};
   const float zy = to_float(row.x[y]);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    d = 0.0;
-    for (int i = 0; i < kWarps; ++i) d += warp_d[i];
-    d = whole_sum<T>(d);
-    const Scalars v = row_scalars<T>(m, d, zy, a.tau);
-    if (kPolicy) {
-      const float coef = policy_scalars(a, in, v.logp, r, true) / a.tau;
-      bcast = make_float4(coef, (float)(coef / d), m, coef * v.rest);
-    } else {
-      put_logp(a, r, v.logp, make_float4(m, (float)(1.0 / d), v.rest, (float)v.lse));
+  if (warp == 0) {
+    Stat t = join_lanes(lane < kWarps ? warp_stat[lane] : Stat{kLowest, 0.0}, kWarps, a.inv_tau);
+    if (lane == 0) {
+      t.d = whole_sum<T>(t.d);
+      const Scalars v = row_scalars<T>(t.m, t.d, zy, a);
+      if (kPolicy) {
+        const float coef = (float)(policy_scalars(a, in, v.logp, r, true) * a.inv_tau);
+        bcast = make_float4(coef, (float)(-coef / t.d), t.m, coef * v.rest);
+      } else {
+        put_logp(a, r, v.logp, make_float4(t.m, (float)(1.0 / t.d), v.rest, (float)v.lse));
+      }
     }
   }
   if (!kPolicy) return;
   __syncthreads();
-  const float coef = bcast.x, k = bcast.y, at_target = bcast.w;
-  const int vy = (int)((y + row.shift) / N), jy = (int)((y + row.shift) % N);
-  for (int v = threadIdx.x; v < row.nvec; v += kThreads) {
-    const Vec<T> x = row.load(v);
-    float g[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      g[j] = coef == 0.f ? 0.f : -k * exp_from<T>(x.get(j), m, c);
-      if (v == vy && j == jy && coef != 0.f) g[j] = at_target;
-    }
-    row.store(o, v, g, wide);
-  }
+  const float coef = bcast.x;
+  const F2 factor = f2(bcast.y, bcast.y), minus_m = f2(-bcast.z, -bcast.z);
+  for (int v = threadIdx.x; v < row.nvec; v += kThreads)
+    row.store(o, v, coef == 0.f ? zeros<T>() : scaled_exp(row.load(v), minus_m, factor, c), wide);
+  const int vy = (int)((y + row.shift) / N);
+  if (coef != 0.f && vy % kThreads == threadIdx.x) o[y] = from_float<T>(bcast.w);
 }
 
 // ---- gradient of the log-probabilities --------------------------------------------------------------
@@ -466,17 +937,14 @@ __global__ void __launch_bounds__(kBwdThreads) logp_bwd_kernel(const T* logits, 
   float g = 0.f;
   if (live) g = (a.logp64 ? (float)static_cast<const double*>(grad_logp)[r] : static_cast<const float*>(grad_logp)[r]) / a.tau;
   if (g == 0.f) {
-    const float zero[N] = {};
     for (int i = 0; i < kBwdVecs; ++i) {
       const int v = begin + i * kBwdThreads + threadIdx.x;
-      if (v < row.nvec) row.store(o, v, zero, wide);
+      if (v < row.nvec) row.store(o, v, zeros<T>(), wide);
     }
     return;
   }
   const float4 st = a.stats[r];
-  const float m = st.x, k = g * st.y, at_target = g * st.z;
-  const Scale c = a.c;
-  const int vy = (int)((y + row.shift) / N), jy = (int)((y + row.shift) % N);
+  const F2 factor = f2(-g * st.y, -g * st.y), minus_m = f2(-st.x, -st.x);
   Vec<T> x[kBwdVecs];
 #pragma unroll
   for (int i = 0; i < kBwdVecs; ++i) {
@@ -487,16 +955,10 @@ __global__ void __launch_bounds__(kBwdThreads) logp_bwd_kernel(const T* logits, 
 #pragma unroll
   for (int i = 0; i < kBwdVecs; ++i) {
     const int v = begin + i * kBwdThreads + threadIdx.x;
-    if (v < row.nvec) {
-      float e[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        e[j] = -k * exp_from<T>(x[i].get(j), m, c);
-        if (v == vy && j == jy) e[j] = at_target;
-      }
-      row.store(o, v, e, wide);
-    }
+    if (v < row.nvec) row.store(o, v, scaled_exp(x[i], minus_m, factor, a.c), wide);
   }
+  const int at = (int)((y + row.shift) / N) - begin - (int)threadIdx.x;      // its writer puts the target's entry right
+  if (at >= 0 && at < kBwdThreads * kBwdVecs && at % kBwdThreads == 0) o[y] = from_float<T>(g * st.z);
 }
 
 // ---- preference loss ------------------------------------------------------------------------------
@@ -610,6 +1072,7 @@ static int check_rows(const char* what, int dtype, int64_t rows, int64_t V, int6
 static policy::RowArgs row_args(const int64_t* target, int64_t V, int64_t ignore_index, float tau, int* status) {
   policy::RowArgs a = {};
   a.target = target; a.V = V; a.ignore_index = ignore_index; a.tau = tau; a.status = status;
+  a.inv_tau = 1.0 / tau;
   const double c = 1.4426950408889634 / tau;    // log2(e) / tau
   a.c.hi = (float)c;
   if ((double)a.c.hi >= c) a.c.hi = nextafterf(a.c.hi, 0.f);   // the low part is positive: -inf logits times both parts stay -inf
@@ -618,15 +1081,87 @@ static policy::RowArgs row_args(const int64_t* target, int64_t V, int64_t ignore
   return a;
 }
 
-// Cluster size and threads of the held kernel.  The cluster is the smallest that leaves three CTAs' slices room on an SM, and
-// larger while there are so few rows that SMs would be idle.  Slices of at most 16 KB use CTAs of 128 threads, whose
-// reductions are shorter.  Rows beyond 8 CTAs' shared memory go to wide_kernel.
-constexpr int64_t kSliceBytes = 72 * 1024, kSliceLimit = 224 * 1024;
+// Which kernel, cluster and slices.
+//   Rows of at most kSmallRow bytes: held_kernel with one CTA of 128 threads per row, many CTAs per SM.
+//   Else pipe_kernel with the cluster size whose clusters have the fewest bytes to go through one after the other,
+//     rounds * (slice + kRoundBytes),  rounds = rows / clusters that the device holds at once (8-CTA clusters leave 28 of 148 SMs
+//     empty, 9-CTA clusters 13: the GPCs have 16 to 20 SMs), among those whose slices leave room for three slots (more are taken where they fit).
+//   Rows too wide for that: two slots, or one; beyond it wide_kernel.
+constexpr int64_t kSmallRow = 16 * 1024, kSliceLimit = 221 * 1024, kRoundBytes = 8 * 1024;
+
+template <typename T, bool kPolicy>
+static cudaLaunchConfig_t pipe_config(int cluster, int64_t bytes, cudaLaunchAttribute* at) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cluster);
+  cfg.blockDim = dim3(policy::kWorkers + 64);
+  cfg.dynamicSmemBytes = (size_t)bytes;
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// Clusters of pipe_kernel that the device holds at once: one CTA per SM whatever the slices are, so asked once per size.
+template <typename T, bool kPolicy>
+static int resident_clusters(int cluster, int* out) {
+  static std::atomic<int> known[64][policy::kMaxCluster + 1];
+  int dev = 0;
+  B2G_CUDA_OK(cudaGetDevice(&dev));
+  B2G_REQUIRE(dev >= 0 && dev < 64, "device index %d out of range", dev);
+  int n = known[dev][cluster].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchAttribute at[1];
+    const cudaLaunchConfig_t cfg = pipe_config<T, kPolicy>(cluster, kSliceLimit, at);
+    B2G_CUDA_OK(cudaOccupancyMaxActiveClusters(&n, policy::pipe_kernel<T, kPolicy>, &cfg));
+    n = n < 1 ? -1 : n;
+    known[dev][cluster].store(n, std::memory_order_relaxed);
+  }
+  *out = n < 0 ? 0 : n;
+  return 0;
+}
+
+template <typename T, bool kPolicy>
+static int launch_pipe(const T* logits, int64_t ld, const policy::RowArgs& a, T* out, int64_t ld_out, int64_t rows, cudaStream_t s, bool* taken) {
+  constexpr int N = 16 / sizeof(T);
+  static std::atomic<uint64_t> seen{0};
+  if (first_use_on_device(seen)) {
+    B2G_CUDA_OK(cudaFuncSetAttribute(policy::pipe_kernel<T, kPolicy>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSliceLimit));
+    B2G_CUDA_OK(cudaFuncSetAttribute(policy::pipe_kernel<T, kPolicy>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  }
+  const int64_t need = (a.V + 2 * (N - 1)) / N;      // vectors of a row at its worst alignment
+  int best = 0, best_resident = 0;
+  for (int slots = 3; slots >= 1 && best == 0; --slots) {
+    int64_t best_cost = 0;
+    for (int c = 1; c <= policy::kMaxCluster; ++c) {
+      const int64_t slice = (need + c - 1) / c * 16;
+      if (slice * slots > kSliceLimit) continue;
+      int resident = 0;
+      if (int rc = resident_clusters<T, kPolicy>(c, &resident)) return rc;
+      if (resident == 0) continue;
+      const int64_t cost = (rows + resident - 1) / resident * (slice + kRoundBytes);
+      if (best == 0 || cost < best_cost) { best = c; best_cost = cost; best_resident = resident; }
+    }
+  }
+  *taken = best != 0;
+  if (best == 0) return 0;
+  const int64_t slice = (need + best - 1) / best * 16;
+  const int slots = (int)(kSliceLimit / slice < policy::kMaxSlots ? kSliceLimit / slice : policy::kMaxSlots);
+  // G may trail S by as many rows as there are slots beside the one being filled; without G only the rings bound it
+  const int lead = kPolicy ? (slots >= 3 ? slots - 2 : slots - 1) : policy::kMaxLead;
+  // whole turns of 32 vectors per warp; the last warps may have none
+  const int per_warp = (int)((slice / 16 + policy::kWorkers - 1) / policy::kWorkers) * 32;
+  cudaLaunchAttribute at[1];
+  cudaLaunchConfig_t cfg = pipe_config<T, kPolicy>(best, slice * slots, at);
+  cfg.gridDim = dim3((unsigned)((rows < best_resident ? rows : best_resident) * best));
+  cfg.stream = s;
+  B2G_CUDA_OK(cudaLaunchKernelEx(&cfg, policy::pipe_kernel<T, kPolicy>, logits, ld, a, out, ld_out, rows, best, slots, lead, (int)(slice / 16), per_warp));
+  return 0;
+}
 
 template <typename T, int kThreads, bool kPolicy>
 static int launch_held(const T* logits, int64_t ld, const policy::RowArgs& a, T* out, int64_t ld_out, int64_t rows, int cluster, int64_t bytes,
                        cudaStream_t s) {
-  B2G_KERNEL_SMEM((policy::held_kernel<T, kThreads, kPolicy>), kSliceLimit);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * cluster));
   cfg.blockDim = dim3(kThreads);
@@ -644,19 +1179,15 @@ static int launch_held(const T* logits, int64_t ld, const policy::RowArgs& a, T*
 template <typename T, bool kPolicy>
 static int launch_rows(const T* logits, int64_t ld, const policy::RowArgs& a, T* out, int64_t ld_out, int64_t rows, cudaStream_t s) {
   constexpr int N = 16 / sizeof(T);
-  const int64_t need = (a.V + 2 * (N - 1)) / N;      // vectors of a row at its worst alignment
-  auto slice = [&](int c) { return (need + c - 1) / c * 16; };
-  int cluster = 1;
-  while (cluster < 8 && slice(cluster) > kSliceBytes) cluster *= 2;
-  while (cluster < 8 && rows * cluster < 2 * sm_count() && slice(cluster) > 8 * 1024) cluster *= 2;
-  const int64_t bytes = slice(cluster);
-  if (bytes > kSliceLimit) {
+  const int64_t bytes = (a.V + 2 * (N - 1)) / N * 16;
+  if (bytes <= kSmallRow) return launch_held<T, 128, kPolicy>(logits, ld, a, out, ld_out, rows, 1, bytes, s);
+  bool taken = false;
+  if (int rc = launch_pipe<T, kPolicy>(logits, ld, a, out, ld_out, rows, s, &taken)) return rc;
+  if (!taken) {
     policy::wide_kernel<T, kPolicy><<<(unsigned)rows, 512, 0, s>>>(logits, ld, a, out, ld_out);
     B2G_CUDA_OK(cudaGetLastError());
-    return 0;
   }
-  if (bytes <= 16 * 1024) return launch_held<T, 128, kPolicy>(logits, ld, a, out, ld_out, rows, cluster, bytes, s);
-  return launch_held<T, 512, kPolicy>(logits, ld, a, out, ld_out, rows, cluster, bytes, s);
+  return 0;
 }
 
 extern "C" int b2g_token_logprobs(const void* logits, int64_t ld, int logits_dtype, const int64_t* target, void* logp, int logp_dtype, float* stats,
