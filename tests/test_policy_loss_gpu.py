@@ -34,7 +34,7 @@ def _check_cotangent(got, logits, target, coef, coef_tol, tau, dtype, live):
     z = logits.double() / tau
     z = torch.where(live[:, None], z, torch.zeros_like(z))
     lse = torch.logsumexp(z, 1, keepdim=True)
-    p = torch.exp(z - lse)
+    p = torch.softmax(z, 1)
     want = -p.clone()
     hot = torch.arange(n), target.clamp(min=0)
     want[hot] += 1.0
@@ -492,3 +492,68 @@ def test_refusals(cuda):
     tau = C.c_float(1.0)
     from b2g import _lib
     assert _lib.load().b2g_token_logprobs(None, 16, 0, None, None, 0, None, 4, 16, tau, -100, None, None) == -1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [3000, 20001, 130003])
+def test_maxima_that_no_sample_sees(cuda, dtype, vocab):
+    """One logit far above everything else, at a column of its own in every row: sums taken against too low a reference must
+    overflow unnoticed or be made again.  Among the rows are a NaN, a +inf, a row of -inf but for the target, one masked
+    throughout by the type's lowest value, and ignored ones between them."""
+    from b2g import ops
+
+    logits, target = _rows(24, vocab, dtype, vocab)
+    for r in range(24):
+        logits[r, (r * 7919 + 5) % vocab] = 20.0 + 12.0 * r                # 20 ... 296
+    logits[3] = torch.finfo(dtype).min
+    logits[7] = float("-inf")
+    logits[7, target[7]] = 1.5
+    logits[11, 17] = float("nan")
+    logits[13, 19] = float("inf")
+    target[[5, 12, 20]] = -100
+    takes = target != -100
+    whole = takes.clone()
+    whole[[11, 13]] = False
+    clean = torch.where(whole[:, None], logits, torch.zeros_like(logits))
+    logp = ref.logprobs(clean.double(), target)
+    adv = torch.linspace(-1, 1, 24) + 0.01
+    x, t = logits.to(cuda), target.to(cuda)
+    for tau in (1.0, 3.0):
+        logp = ref.logprobs(clean.double(), target, tau)
+        got, stats = ops.token_logprobs(x, t, tau, dtype=torch.float64)
+        assert bool(torch.isnan(got[[11, 13]]).all()) and bool((got[[5, 12, 20]] == 0).all())
+        off = (got.cpu() - logp).abs()[whole]
+        assert bool((off <= ref.lse_error(vocab) + logp.abs()[whole] * 2.0 ** -50).all()), float(off.max())
+        loss, lp, _, grad = ops.policy_loss(x, t, adv.to(cuda), temperature=tau)
+        assert bool(torch.isnan(loss[[11, 13]]).all())
+        assert bool(((lp.cpu().double() - logp).abs() <= _logp_tol(logp, vocab))[whole].all())
+        back = ops.token_logprobs_bwd(-adv.to(cuda), x, t, stats, tau)
+        for g in (grad, back):
+            g = g.clone()
+            g[[11, 13]] = 0
+            _check_cotangent(g[whole.to(cuda)], clean[whole], target[whole], -adv.double()[whole], adv.double().abs()[whole] * 2.0 ** -22, tau, dtype,
+                             target[whole] != -100)
+
+
+def test_many_rows_of_every_path_repeat_bit_for_bit(cuda):
+    """More rows than clusters, ignored ones among them, several times over: the pipeline's order does not show."""
+    from b2g import ops
+
+    for vocab, rows in ((1001, 900), (9000, 700), (40003, 400), (129280, 200)):
+        g = torch.Generator(device=cuda).manual_seed(vocab)
+        x = (torch.randn(rows, vocab, generator=g, device=cuda) * 2).bfloat16()
+        t = torch.randint(0, vocab, (rows,), generator=g, device=cuda)
+        t[torch.rand(rows, generator=g, device=cuda) < 0.3] = -100
+        t[rows // 2:rows // 2 + 40] = -100
+        adv = torch.randn(rows, generator=g, device=cuda)
+        want = ops.policy_loss(x, t, adv)
+        logp = ops.token_logprobs(x, t)[0]
+        assert torch.equal(logp, want[1])
+        for _ in range(3):
+            got = ops.policy_loss(x, t, adv)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(ops.token_logprobs(x, t)[0], logp)
+        some = torch.randint(0, rows, (12,)).tolist()
+        for r in some:                                                   # a row's result does not depend on its neighbours
+            one = ops.policy_loss(x[r:r + 1], t[r:r + 1], adv[r:r + 1])
+            assert torch.equal(one[1], want[1][r:r + 1]) or abs(float(one[1] - want[1][r])) <= 2 * ref.lse_error(vocab)
+            torch.testing.assert_close(one[3].float(), want[3][r:r + 1].float(), rtol=2.0 ** -7, atol=1e-6)

@@ -93,6 +93,11 @@ struct Vec {
     if constexpr (sizeof(T) == 2) return f2(dev::bf16_lo(w[i]), dev::bf16_hi(w[i]));
     else return f2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
   }
+  // Between two passes over registers: the compiler may not keep the unpacked floats of the first, at a register each.
+  __device__ __forceinline__ void packed_again() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+r"(w[i]));
+  }
   __device__ __forceinline__ void set_nothing() {   // -inf everywhere: the maximum and the sum do not see it
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;
@@ -134,6 +139,29 @@ __device__ __forceinline__ Vec<T> scaled_exp(const Vec<T>& x, F2 minus_m, F2 fac
     }
   }
   return r;
+}
+
+// 2^(z c - reference) as pairs: two fused steps, the exponent rounded where it is small.
+__device__ __forceinline__ F2 ex2_pair(F2 t) {
+  float lo, hi;
+  split(t, lo, hi);
+  return f2(ex2(lo), ex2(hi));
+}
+template <typename T>
+__device__ __forceinline__ Vec<T> cotangent_vec(const Vec<T>& x, F2 minus_ref, F2 factor, const Scale& c) {
+  if constexpr (sizeof(T) == 4) {
+    return scaled_exp(x, minus_ref, factor, c);
+  } else {
+    Vec<T> r;
+    const F2 h = f2(c.hi, c.hi);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float lo, hi;
+      split(ex2_pair(fma2(x.pair(i), h, minus_ref)) * factor, lo, hi);
+      r.w[i] = dev::pack_bf16(lo, hi);
+    }
+    return r;
+  }
 }
 
 // A row as 16-byte vectors of the memory it lies in: vector v holds the columns [v * N - shift, (v + 1) * N - shift), so the
@@ -211,7 +239,10 @@ struct RowArgs {
   // log-probabilities
   void* logp;          // fp32, or fp64 when logp64
   int logp64;
-  float4* stats;       // what the backward pass of the log-probabilities reads: m, 1/d, 1 - p of the target, lse
+  // What the backward pass of the log-probabilities reads: what the exponentials are against, 1/sum, 1 - p of the target, lse.
+  // A positive 1/sum stands for the pipeline's form (16-bit logits: 2^(z log2(e)/tau - reference)), a negative one for
+  // exp((z - m)/tau).
+  float4* stats;
   // policy loss
   const float *advantage, *old_logp, *ref_logp, *weight;
   float clip_low, clip_high, kl_coef;
@@ -332,7 +363,7 @@ __device__ __forceinline__ float vec_max(const Vec<T>& x, float m) {
 }
 
 template <typename T, int kThreads, bool kPolicy>
-__global__ void __launch_bounds__(kThreads, 8) held_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out,
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) held_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out,
                                                                          int cluster) {
   constexpr int N = Vec<T>::N, kWarps = kThreads / 32;
   extern __shared__ __align__(16) uint8_t slice[];
@@ -436,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 8) held_kernel(const T* logits, int6
         const float coef = (float)(policy_scalars(a, in, v.logp, r, rank == 0) * a.inv_tau);
         bcast = make_float4(coef, (float)(-coef / t.d), t.m, coef * v.rest);
       } else if (rank == 0) {
-        put_logp(a, r, v.logp, make_float4(t.m, (float)(1.0 / t.d), v.rest, (float)v.lse));
+        put_logp(a, r, v.logp, make_float4(t.m, (float)(-1.0 / t.d), v.rest, (float)v.lse));
       }
     }
   }
@@ -460,27 +491,96 @@ __global__ void __launch_bounds__(kThreads, 8) held_kernel(const T* logits, int6
   if (vy >= v0 && vy < end && (vy - v0) % kThreads == 0) o[y] = from_float<T>(bcast.w);
 }
 
+// ---- short rows --------------------------------------------------------------------------------------
+// One warp per row, kVecs vectors of it in every lane's registers: no barrier, and the scalars of the rows that share an SM
+// overlap.
+constexpr int kShortWarps = 4;
+template <typename T, int kVecs, bool kPolicy>
+__global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out, int64_t rows) {
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * kShortWarps + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const int64_t y = a.target[r];
+  const Row<T> row(logits + r * ld, a.V);
+  T* const o = kPolicy ? out + r * ld_out : nullptr;
+  const bool wide = kPolicy && same_alignment(row.x, (const T*)o);
+  bool live = target_ok(y, a, lane == 0);
+  Given in{1.f, 0.f, 0.f, 0.f};
+  if (kPolicy) {
+    in = given(a, r);
+    live = live && in.weight != 0.f;
+  }
+  if (!live) {
+    if (lane == 0) {
+      if (kPolicy) { a.loss[r] = 0.f; a.kl[r] = 0.f; static_cast<float*>(a.logp)[r] = 0.f; }
+      else put_logp(a, r, 0.0, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
+    if (kPolicy)
+      for (int v = lane; v < row.nvec; v += 32) row.store(o, v, zeros<T>(), wide);
+    return;
+  }
+  Vec<T> x[kVecs];
+  float m = kLowest;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = lane + i * 32;
+    if (v < row.nvec) x[i] = row.load(v);
+    else x[i].set_nothing();
+  }
+  const float zy = to_float(row.x[y]);
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) m = vec_max(x[i], m);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+  double d = 0.0;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    x[i].packed_again();
+    d += (double)sum_of(exp_sum(x[i], f2(-m, -m), a.c));
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
+  d = whole_sum<T>(d);
+  const Scalars v = row_scalars<T>(m, d, zy, a);
+  if (!kPolicy) {
+    if (lane == 0) put_logp(a, r, v.logp, make_float4(m, (float)(-1.0 / d), v.rest, (float)v.lse));
+    return;
+  }
+  const float coef = (float)(policy_scalars(a, in, v.logp, r, lane == 0) * a.inv_tau), k = (float)(-coef / d);
+  const int vy = (int)((y + row.shift) / Vec<T>::N);
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int u = lane + i * 32;
+    x[i].packed_again();
+    if (u < row.nvec) row.store(o, u, coef == 0.f ? zeros<T>() : scaled_exp(x[i], f2(-m, -m), f2(k, k), a.c), wide);
+  }
+  if (coef != 0.f && vy % 32 == lane) o[y] = from_float<T>(coef * v.rest);      // its writer puts the target's entry right
+}
+
 // ---- rows in a pipeline ------------------------------------------------------------------------------
-// One CTA per SM, clusters that stay and go from row to row, `slots` slices of rows in shared memory.  15 warps work, one more
-// does everything that is latency.  For every row k:
-//   the scalar warp reads 128 samples and the target's logit, and publishes their maximum as the row's reference: a sum of
-//     exponentials in 32 bits needs no more than a reference within 80 tau of the maximum (rows where that fails are summed
-//     once more, below), so the workers need no pass for the maximum and all their sums simply add up;
-//   S(k): the workers' sums of exp((z - reference)/tau) over everything but the target, one pair of numbers per thread;
-//   the scalar warp adds them up, sends the CTA's share to the others of the cluster (asynchronous remote stores that count on
-//     their barrier), adds theirs, finishes the row's scalars and lets the workers know;
-//   G(k), the cotangent, only `lead` rows after S(k): the workers never wait for the exchange.
+// Clusters that stay and go from row to row, two CTAs on every SM (two whose phases differ keep memory and the special-function
+// unit busier than one of twice the size: 1024 x 248320 bf16 in 215 against 233 us), each with `slots` slices of rows in shared
+// memory.  13 warps work, two more do everything that is latency.  For every row k:
+//   the first of them reads 128 samples and the target's logit, and publishes their maximum as the row's reference: a sum of
+//     exponentials needs no maximum, only a number near it, so the workers need no pass for one and their sums simply add up;
+//   S(k): the workers' sums of exp((z - reference)/tau) over everything but the target, one number per warp.  A warp whose sum
+//     says that a logit of its own lies far above the reference (more than 14 log2 units: the exponent would be rounded too
+//     coarsely there, and overflow at 128) sums once more, against its own maximum;
+//   the first warp adds them up and sends the CTA's share to the others of the cluster (asynchronous remote stores that count on
+//     their barrier); the second adds the shares, finishes the row's scalars and lets the workers know;
+//   G(k), the cotangent, `lead` rows after S(k): the workers never wait for the exchange.
 // The target's own term is added in 64 bits: where it dominates, nothing of the small rest is lost to its rounding, and 1 - p
 // is the rest's share without a cancellation.
-// Every vector is private to one thread: it copies it in (cp.async), reads it in S and in G, and copies the vector of the row
-// `slots` further on into the same place.
-// A sum that is no number, or 0 (a reference too low by 88 tau, NaN, +inf, a vocabulary masked by the type's lowest value) is
-// made again against the true maximum, by the scalar warps alone, and G then takes the exact form of the exponent.
+// A warp's vectors are its own: it fetches them (one bulk copy per row, issued by one lane: as 16-byte copies of every lane they
+// took the load-store unit as long as the arithmetic), reads them in S and in G, and fetches those of the row `slots` further
+// on into the same place.
+// A row whose sum is no number, or 0 (NaN, +inf, a vocabulary masked throughout by the type's lowest value) is summed again by
+// the scalar warps alone, and G then takes the exact form of the exponent.
+// What bounds it: two exponentials per logit at 16 per cycle and SM (126 us of the 215), then HBM (155 us); the two overlap
+// only between CTAs.  Replacing one exponential in four by a polynomial on the fp32 pipe was slower (231 us): the loops issue
+// 12 instructions per logit, and the polynomial adds six to every one that it replaces.
 // All waits are bounded; a CTA whose wait ran out stops working, and all CTAs of a cluster leave together.
-#ifndef WW
-#define WW 19
-#endif
-constexpr int kWorkerWarps = WW, kWorkers = kWorkerWarps * 32, kRing = 8, kMaxCluster = 10, kMaxSlots = 4, kMaxLead = 3, kAhead = 7, kInfo = 16, kSamples = 4;
+constexpr int kWorkerWarps = 13, kWorkers = kWorkerWarps * 32, kRing = 8, kMaxCluster = 10, kMaxSlots = 2, kMaxLead = 3, kAhead = 7, kInfo = 16, kSamples = 4;
 
 struct Share { float m, unused; double d; };       // what a CTA sends: its sum and what it is against
 
@@ -551,12 +651,6 @@ struct Part {
 // What the workers need to know of a row: what to sum against, and its target, or -1 where it takes no part.
 struct Info { float reference; int y; };
 
-// 2^(z c - reference) as pairs: two fused steps, the exponent rounded where it is small.
-__device__ __forceinline__ F2 ex2_pair(F2 t) {
-  float lo, hi;
-  split(t, lo, hi);
-  return f2(ex2(lo), ex2(hi));
-}
 // What the workers sum against: bf16 in units of log2 (any number serves, so its rounding costs nothing), fp32 as a logit.
 template <typename T>
 __device__ __forceinline__ float reference_of(float m, const Scale& c) {
@@ -577,20 +671,46 @@ __device__ __forceinline__ F2 sum_vec(const Vec<T>& x, F2 minus_ref, const Scale
     for (int i = 0; i < s; ++i) e[i] = e[i] + e[i + s];
   return e[0];
 }
+constexpr double kFarAbove = 16384.0;      // 2^14
+// The joint sum of a warp's lanes, whose references differ only where one of them met a logit far above the others'.
 template <typename T>
-__device__ __forceinline__ Vec<T> cotangent_vec(const Vec<T>& x, F2 minus_ref, F2 factor, const Scale& c) {
-  if constexpr (sizeof(T) == 4) {
-    return scaled_exp(x, minus_ref, factor, c);
-  } else {
-    Vec<T> r;
+__device__ __forceinline__ Stat join_references(Stat s, double inv_tau) {
+  float m = s.m;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float lo, hi;
-      split(ex2_pair(fma2(x.pair(i), f2(c.hi, c.hi), minus_ref)) * factor, lo, hi);
-      r.w[i] = dev::pack_bf16(lo, hi);
-    }
-    return r;
-  }
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (s.d != 0.0 && s.m != m) s.d *= sizeof(T) == 2 ? exp2((double)s.m - (double)m) : exp(((double)s.m - (double)m) * inv_tau);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s.d += __shfl_xor_sync(0xffffffffu, s.d, o);
+  return Stat{m, s.d};
+}
+
+// A warp's sum over its vectors in shared memory, n of this lane's 512 bytes apart.
+template <typename T>
+__device__ __forceinline__ double warp_sum_against(uint32_t place, int n, float ref, const Scale& c) {
+  constexpr int kStep = 32 * 16;
+  const F2 minus_ref = f2(-ref, -ref);
+  F2 d = f2(0.f, 0.f);
+  int i = 0;
+#pragma unroll 2
+  for (; i + 1 < n; i += 2)
+    d = d + (sum_vec(from_shared<T>(place + i * kStep), minus_ref, c) + sum_vec(from_shared<T>(place + (i + 1) * kStep), minus_ref, c));
+  if (i < n) d = d + sum_vec(from_shared<T>(place + i * kStep), minus_ref, c);
+  float lo, hi;
+  split(d, lo, hi);
+  double all = (double)lo + (double)hi;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  return all;
+}
+// The same against its own maximum; out of line, it is rare.
+template <typename T>
+__device__ __noinline__ Stat warp_sum_far(uint32_t place, int n, Scale c) {
+  float m = kLowest;
+  for (int i = 0; i < n; ++i) m = vec_max(from_shared<T>(place + i * 512), m);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float ref = reference_of<T>(m, c);
+  return Stat{ref, warp_sum_against<T>(place, n, ref, c)};
 }
 
 // One warp's sum over columns [begin, end) of a row but for column y, against their maximum.
@@ -610,18 +730,19 @@ __device__ __noinline__ Stat sum_again(const T* x, int begin, int end, int y, co
 }
 
 template <typename T, bool kPolicy>
-__global__ void __launch_bounds__(kWorkers + 64, 1) pipe_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out, int64_t rows,
+__global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out, int64_t rows,
                                                                 int cluster, int slots, int lead, int per, int per_warp) {
   constexpr int N = Vec<T>::N, kStep = 32 * 16;
   extern __shared__ __align__(16) uint8_t space[];
   __shared__ uint64_t arrived[kMaxSlots][kWorkerWarps];      // one per slot and warp: a warp's copies are its own
-  __shared__ __align__(16) Share share[2][kRing][kMaxCluster];
-  __shared__ double sums[kRing][kWorkerWarps];
+  __shared__ __align__(16) Share share[kRing][kMaxCluster];
+  __shared__ __align__(16) Share share_again[2][kMaxCluster];   // a CTA sends its next one only after all have sent the one before
+  __shared__ Stat sums[kRing][kWorkerWarps];
   __shared__ __align__(8) Info info[kInfo];
-  __shared__ float2 known[kInfo];                // the samples' maximum and the target's logit
+  __shared__ float known[kInfo];                 // the target's logit
   __shared__ float4 bcast[kRing];
   __shared__ int exact_form[kRing];
-  __shared__ uint64_t referred[kInfo], summed[kRing], joined[2][kRing], ready[kRing];
+  __shared__ uint64_t referred[kInfo], summed[kRing], joined[kRing], joined_again[2], ready[kRing];
   __shared__ int gave_up;
   const int rank = blockIdx.x % cluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t first = blockIdx.x / cluster, stride = gridDim.x / cluster;
@@ -632,10 +753,10 @@ __global__ void __launch_bounds__(kWorkers + 64, 1) pipe_kernel(const T* logits,
     for (int i = 0; i < kMaxSlots * kWorkerWarps; ++i) dev::mbar_init(dev::smem_u32(&arrived[0][i]), 1);
     for (int i = 0; i < kRing; ++i) {
       dev::mbar_init(dev::smem_u32(&summed[i]), kWorkerWarps);
-      dev::mbar_init(dev::smem_u32(&joined[0][i]), 1);
-      dev::mbar_init(dev::smem_u32(&joined[1][i]), 1);
+      dev::mbar_init(dev::smem_u32(&joined[i]), 1);
       dev::mbar_init(dev::smem_u32(&ready[i]), 1);
     }
+    for (int i = 0; i < 2; ++i) dev::mbar_init(dev::smem_u32(&joined_again[i]), 1);
     dev::fence_barrier_init();
   }
   dev::cluster_sync_all();          // nobody sends to a barrier that is not there yet
@@ -645,16 +766,22 @@ __global__ void __launch_bounds__(kWorkers + 64, 1) pipe_kernel(const T* logits,
     const int64_t apart = a.V / (32 * kSamples);
     float sample[kSamples], target_logit = 0.f;
     int y_ahead = -1;
+    // the target and weight of the row after the one that is looked at, so that its logit's address is at hand in time
+    int64_t target_next = a.target[first];
+    float weight_next = kPolicy && a.weight ? a.weight[first] : 1.f;
     auto look_at = [&](int k) {     // issue the loads of row k's reference
       if (k >= count) return;
-      const int64_t r = first + k * stride;
+      const int64_t r = first + k * stride, y = target_next;
       const T* x = logits + r * ld;
 #pragma unroll
       for (int i = 0; i < kSamples; ++i) sample[i] = to_float(x[(lane * kSamples + i) * apart]);
-      const int64_t y = a.target[r];
       const bool in_range = y >= 0 && y < a.V;
       target_logit = in_range ? to_float(x[y]) : -INFINITY;
-      y_ahead = in_range && y != a.ignore_index && !(kPolicy && a.weight && a.weight[r] == 0.f) ? (int)y : -1;
+      y_ahead = in_range && y != a.ignore_index && weight_next != 0.f ? (int)y : -1;
+      if (k + 1 < count) {
+        target_next = a.target[r + stride];
+        if (kPolicy && a.weight) weight_next = a.weight[r + stride];
+      }
     };
     auto refer = [&](int k) {
       if (k >= count) return;
@@ -665,7 +792,7 @@ __global__ void __launch_bounds__(kWorkers + 64, 1) pipe_kernel(const T* logits,
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (lane == 0) {
         info[k % kInfo] = Info{reference_of<T>(m, c), y_ahead};
-        known[k % kInfo] = make_float2(m, target_logit);
+        known[k % kInfo] = target_logit;
         dev::mbar_arrive(dev::smem_u32(&referred[k % kInfo]));
       }
     };
@@ -677,34 +804,35 @@ __global__ void __launch_bounds__(kWorkers + 64, 1) pipe_kernel(const T* logits,
       const int p = k % kRing, parity = (k / kRing) & 1;
       look_at(k + kAhead);
       if (!dev::mbar_wait(dev::smem_u32(&summed[p]), parity, &gave_up, a.status, 501)) break;
-      double d = lane < kWorkerWarps ? sums[p][lane] : 0.0;      // of a row that takes no part nobody looks at it
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      // of a row that takes no part nobody looks at it
+      const Stat t = join_references<T>(lane < kWorkerWarps ? sums[p][lane] : Stat{kLowest, 0.0}, a.inv_tau);
       if (lane < cluster)
-        send_share(dev::map_to_cta(dev::smem_u32(&share[0][p][rank]), lane), dev::map_to_cta(dev::smem_u32(&joined[0][p]), lane), Share{0.f, 0.f, d});
+        send_share(dev::map_to_cta(dev::smem_u32(&share[p][rank]), lane), dev::map_to_cta(dev::smem_u32(&joined[p]), lane), Share{t.m, 0.f, t.d});
       refer(k + kAhead);
     }
   } else if (warp == kWorkerWarps + 1) {       // the row's scalars
     int again = 0;                  // rows that needed the second exchange
+    int64_t target_next = a.target[first];
+    Given given_next{1.f, 0.f, 0.f, 0.f};
+    if (kPolicy) given_next = given(a, first);
     for (int k = 0; k < count; ++k) {
-      const int64_t r = first + k * stride, y = a.target[r];
-      const int p = k % kRing, parity = (k / kRing) & 1;
-      const uint32_t bar = dev::smem_u32(&joined[0][p]);
-      if (lane == 0) dev::mbar_arrive_expect_tx(bar, cluster * (uint32_t)sizeof(Share));
-      Given in{1.f, 0.f, 0.f, 0.f};
-      bool live = target_ok(y, a, rank == 0 && lane == 0);
-      if (kPolicy) {
-        in = given(a, r);
-        live = live && in.weight != 0.f;
+      const int64_t r = first + k * stride, y = target_next;
+      const Given in = given_next;
+      if (k + 1 < count) {
+        target_next = a.target[r + stride];
+        if (kPolicy) given_next = given(a, r + stride);
       }
+      const int p = k % kRing, parity = (k / kRing) & 1;
+      const uint32_t bar = dev::smem_u32(&joined[p]);
+      if (lane == 0) dev::mbar_arrive_expect_tx(bar, cluster * (uint32_t)sizeof(Share));
+      const bool live = target_ok(y, a, rank == 0 && lane == 0) && in.weight != 0.f;
       if (!wait_cluster(bar, parity, &gave_up, a.status, 502)) break;
       if (live) {
-        double d = lane < cluster ? share[0][p][lane].d : 0.0;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        const Stat sum = join_references<T>(lane < cluster ? Stat{share[p][lane].m, share[p][lane].d} : Stat{kLowest, 0.0}, a.inv_tau);
+        double d = sum.d;
         if (sizeof(T) == 2) d += d * kEx2Shortfall;
-        const float zy = known[k % kInfo].y;
-        float ref = info[k % kInfo].reference, m = known[k % kInfo].x;
+        const float zy = known[k % kInfo];
+        float ref = sum.m;
         // the target's own term
         double own = sizeof(T) == 2 ? exp2((double)zy * (a.inv_tau * 1.4426950408889634) - (double)ref) : exp(((double)zy - (double)ref) * a.inv_tau);
         bool exact = false;
@@ -713,30 +841,30 @@ __global__ void __launch_bounds__(kWorkers + 64, 1) pipe_kernel(const T* logits,
           const int shift = (int)((uint32_t)reinterpret_cast<uintptr_t>(logits + r * ld) & 15u) / (int)sizeof(T);
           const int64_t begin = (int64_t)rank * per * N - shift, end = min(a.V, (int64_t)(rank + 1) * per * N - shift);
           const Stat s = sum_again(logits + r * ld, (int)(begin < 0 ? 0 : begin), (int)end, (int)y, a);
-          const int p2 = again % kRing, parity2 = (again / kRing) & 1;
-          const uint32_t bar2 = dev::smem_u32(&joined[1][p2]);
+          const int p2 = again % 2, parity2 = (again / 2) & 1;
+          const uint32_t bar2 = dev::smem_u32(&joined_again[p2]);
           ++again;
           if (lane == 0) dev::mbar_arrive_expect_tx(bar2, cluster * (uint32_t)sizeof(Share));
           __syncwarp();
-          if (lane < cluster) send_share(dev::map_to_cta(dev::smem_u32(&share[1][p2][rank]), lane), dev::map_to_cta(bar2, lane), Share{s.m, 0.f, s.d});
+          if (lane < cluster) send_share(dev::map_to_cta(dev::smem_u32(&share_again[p2][rank]), lane), dev::map_to_cta(bar2, lane), Share{s.m, 0.f, s.d});
           if (!wait_cluster(bar2, parity2, &gave_up, a.status, 505)) break;
-          const Share got = lane < cluster ? share[1][p2][lane] : Share{kLowest, 0.f, 0.0};
+          const Share got = lane < cluster ? share_again[p2][lane] : Share{kLowest, 0.f, 0.0};
           const Stat t = join_lanes(Stat{got.m, got.d}, 32, a.inv_tau);
-          ref = m = t.m;
+          ref = t.m;
           d = t.d;
-          own = exp(((double)zy - (double)m) * a.inv_tau);
+          own = exp(((double)zy - (double)ref) * a.inv_tau);
         }
         const double logp = -log1p(d / own), all = own + d;
+        // the sum may be beyond 32 bits' range where the reference was far too low
+        const float per_sum = all < 1e38 && all > 1e-37 ? 1.f / (float)all : (float)(1.0 / all);
         if (lane == 0) {
-          const float rest = rest_of<T>(d / all, zy, logp, a.tau);
+          const float rest = rest_of<T>((double)((float)d * per_sum), zy, logp, a.tau);
           if (kPolicy) {
             const float coef = (float)(policy_scalars(a, in, logp, r, rank == 0) * a.inv_tau);
-            bcast[p] = make_float4(coef, (float)(-coef / all), ref, coef * rest);
+            bcast[p] = make_float4(coef, -coef * per_sum, ref, coef * rest);
             exact_form[p] = exact;
           } else if (rank == 0) {
-            // the backward pass takes exp((z - m)/tau) over a sum against the same m
-            const double lse = (exact || sizeof(T) == 4 ? (double)ref * a.inv_tau : (double)ref * 0.6931471805599453) + log(all);
-            put_logp(a, r, logp, make_float4(m, (float)exp((double)m * a.inv_tau - lse), rest, (float)lse));
+            put_logp(a, r, logp, make_float4(ref, exact ? -per_sum : per_sum, rest, (float)((double)zy * a.inv_tau - logp)));
           }
         }
       } else if (rank == 0 && lane == 0) {
@@ -784,19 +912,9 @@ __global__ void __launch_bounds__(kWorkers + 64, 1) pipe_kernel(const T* logits,
             if (sizeof(T) == 2) asm volatile("st.shared.u16 [%0], %1;" ::"r"(e), "h"((unsigned short)0xFF80) : "memory");
             else asm volatile("st.shared.u32 [%0], %1;" ::"r"(e), "r"(0xFF800000u) : "memory");
           }
-          const F2 minus_ref = f2(-row.reference, -row.reference);
-          F2 d = f2(0.f, 0.f);
-          int i = 0;
-#pragma unroll 2
-          for (; i + 1 < part.n; i += 2)
-            d = d + (sum_vec(from_shared<T>(place + i * kStep), minus_ref, c) + sum_vec(from_shared<T>(place + (i + 1) * kStep), minus_ref, c));
-          if (i < part.n) d = d + sum_vec(from_shared<T>(place + i * kStep), minus_ref, c);
-          float lo, hi;
-          split(d, lo, hi);
-          double all = (double)lo + (double)hi;
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-          if (lane == 0) sums[p][warp] = all;
+          Stat mine_sum{row.reference, warp_sum_against<T>(place, part.n, row.reference, c)};
+          if (!(mine_sum.d < kFarAbove)) mine_sum = warp_sum_far<T>(place, part.n, c);
+          if (lane == 0) sums[p][warp] = mine_sum;
         }
         __syncwarp();
         if (lane == 0) dev::mbar_arrive(dev::smem_u32(&summed[p]));
@@ -907,7 +1025,7 @@ __global__ void __launch_bounds__(512) wide_kernel(const T* logits, int64_t ld, 
         const float coef = (float)(policy_scalars(a, in, v.logp, r, true) * a.inv_tau);
         bcast = make_float4(coef, (float)(-coef / t.d), t.m, coef * v.rest);
       } else {
-        put_logp(a, r, v.logp, make_float4(t.m, (float)(1.0 / t.d), v.rest, (float)v.lse));
+        put_logp(a, r, v.logp, make_float4(t.m, (float)(-1.0 / t.d), v.rest, (float)v.lse));
       }
     }
   }
@@ -923,8 +1041,8 @@ __global__ void __launch_bounds__(512) wide_kernel(const T* logits, int64_t ld, 
 
 // ---- gradient of the log-probabilities --------------------------------------------------------------
 // dz = g (onehot - exp((z - m)/tau)/d)/tau: one pass without a reduction, kBwdVecs vectors per thread.
-constexpr int kBwdThreads = 256, kBwdVecs = 4;
-template <typename T>
+constexpr int kBwdVecs = 4;
+template <typename T, int kBwdThreads>
 __global__ void __launch_bounds__(kBwdThreads) logp_bwd_kernel(const T* logits, int64_t ld, RowArgs a, const void* __restrict__ grad_logp, T* out,
                                                                int64_t ld_out, int blocks) {
   constexpr int N = Vec<T>::N;
@@ -944,7 +1062,9 @@ __global__ void __launch_bounds__(kBwdThreads) logp_bwd_kernel(const T* logits, 
     return;
   }
   const float4 st = a.stats[r];
-  const F2 factor = f2(-g * st.y, -g * st.y), minus_m = f2(-st.x, -st.x);
+  const float per_sum = fabsf(st.y);
+  const bool natural = !(st.y > 0.f);
+  const F2 factor = f2(-g * per_sum, -g * per_sum), minus_m = f2(-st.x, -st.x);
   Vec<T> x[kBwdVecs];
 #pragma unroll
   for (int i = 0; i < kBwdVecs; ++i) {
@@ -955,7 +1075,7 @@ __global__ void __launch_bounds__(kBwdThreads) logp_bwd_kernel(const T* logits, 
 #pragma unroll
   for (int i = 0; i < kBwdVecs; ++i) {
     const int v = begin + i * kBwdThreads + threadIdx.x;
-    if (v < row.nvec) row.store(o, v, scaled_exp(x[i], minus_m, factor, a.c), wide);
+    if (v < row.nvec) row.store(o, v, natural ? scaled_exp(x[i], minus_m, factor, a.c) : cotangent_vec(x[i], minus_m, factor, a.c), wide);
   }
   const int at = (int)((y + row.shift) / N) - begin - (int)threadIdx.x;      // its writer puts the target's entry right
   if (at >= 0 && at < kBwdThreads * kBwdVecs && at % kBwdThreads == 0) o[y] = from_float<T>(g * st.z);
@@ -1082,12 +1202,18 @@ static policy::RowArgs row_args(const int64_t* target, int64_t V, int64_t ignore
 }
 
 // Which kernel, cluster and slices.
-//   Rows of at most kSmallRow bytes: held_kernel with one CTA of 128 threads per row, many CTAs per SM.
+//   Rows of at most 16 vectors of 16 bytes a lane (bf16: 4081 logits): short_kernel, a warp per row (200,000 x 1000 bf16: log-
+//     probabilities 111 us, 617 us with a CTA per row).
+//   Rows of at most kSmallRow bytes: held_kernel with one CTA of 128 threads per row, many CTAs per SM (20,000 x 10,000 bf16: loss
+//     186 us, 262 us in the pipeline, whose rows cost as much as 20 to 30 KB however short they are; 16,000: 173 and 188; 20,000:
+//     186 and 186).
 //   Else pipe_kernel with the cluster size whose clusters have the fewest bytes to go through one after the other,
-//     rounds * (slice + kRoundBytes),  rounds = rows / clusters that the device holds at once (8-CTA clusters leave 28 of 148 SMs
-//     empty, 9-CTA clusters 13: the GPCs have 16 to 20 SMs), among those whose slices leave room for three slots (more are taken where they fit).
-//   Rows too wide for that: two slots, or one; beyond it wide_kernel.
-constexpr int64_t kSmallRow = 16 * 1024, kSliceLimit = 221 * 1024, kRoundBytes = 8 * 1024;
+//     rounds * (slice + kRoundBytes),  rounds = rows / clusters that the device holds at once (of 296 places 8-CTA clusters fill
+//     264, 9-CTA clusters 270, 5-CTA clusters 280: the GPCs have 16 to 20 SMs), among those whose slices leave room for two
+//     slots.  kRoundBytes stands for what a row costs however short its slices are.
+//   Rows too wide for that: one slot; beyond it wide_kernel.
+// Two CTAs share an SM's 228 KB: 1 KB each is the system's, and pipe_kernel's own arrays may take 5 KB beside the slices.
+constexpr int64_t kSmallRow = 36 * 1024, kSliceLimit = 108 * 1024, kRoundBytes = 8 * 1024;
 
 template <typename T, bool kPolicy>
 static cudaLaunchConfig_t pipe_config(int cluster, int64_t bytes, cudaLaunchAttribute* at) {
@@ -1102,7 +1228,7 @@ static cudaLaunchConfig_t pipe_config(int cluster, int64_t bytes, cudaLaunchAttr
   return cfg;
 }
 
-// Clusters of pipe_kernel that the device holds at once: one CTA per SM whatever the slices are, so asked once per size.
+// Clusters of pipe_kernel that the device holds at once, with all the shared memory that a CTA may take: asked once per size.
 template <typename T, bool kPolicy>
 static int resident_clusters(int cluster, int* out) {
   static std::atomic<int> known[64][policy::kMaxCluster + 1];
@@ -1131,7 +1257,7 @@ static int launch_pipe(const T* logits, int64_t ld, const policy::RowArgs& a, T*
   }
   const int64_t need = (a.V + 2 * (N - 1)) / N;      // vectors of a row at its worst alignment
   int best = 0, best_resident = 0;
-  for (int slots = 3; slots >= 1 && best == 0; --slots) {
+  for (int slots = policy::kMaxSlots; slots >= 1 && best == 0; --slots) {
     int64_t best_cost = 0;
     for (int c = 1; c <= policy::kMaxCluster; ++c) {
       const int64_t slice = (need + c - 1) / c * 16;
@@ -1146,9 +1272,9 @@ static int launch_pipe(const T* logits, int64_t ld, const policy::RowArgs& a, T*
   *taken = best != 0;
   if (best == 0) return 0;
   const int64_t slice = (need + best - 1) / best * 16;
-  const int slots = (int)(kSliceLimit / slice < policy::kMaxSlots ? kSliceLimit / slice : policy::kMaxSlots);
-  // G may trail S by as many rows as there are slots beside the one being filled; without G only the rings bound it
-  const int lead = kPolicy ? (slots >= 3 ? slots - 2 : slots - 1) : policy::kMaxLead;
+  const int slots = kSliceLimit / slice < policy::kMaxSlots ? 1 : policy::kMaxSlots;
+  // G trails S by a row where there is a second slot to wait in; without G only the rings bound how far the workers run ahead
+  const int lead = kPolicy ? slots - 1 : policy::kMaxLead;
   // whole turns of 32 vectors per warp; the last warps may have none
   const int per_warp = (int)((slice / 16 + policy::kWorkers - 1) / policy::kWorkers) * 32;
   cudaLaunchAttribute at[1];
@@ -1162,6 +1288,7 @@ static int launch_pipe(const T* logits, int64_t ld, const policy::RowArgs& a, T*
 template <typename T, int kThreads, bool kPolicy>
 static int launch_held(const T* logits, int64_t ld, const policy::RowArgs& a, T* out, int64_t ld_out, int64_t rows, int cluster, int64_t bytes,
                        cudaStream_t s) {
+  B2G_KERNEL_SMEM((policy::held_kernel<T, kThreads, kPolicy>), kSmallRow);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * cluster));
   cfg.blockDim = dim3(kThreads);
@@ -1176,10 +1303,21 @@ static int launch_held(const T* logits, int64_t ld, const policy::RowArgs& a, T*
   return 0;
 }
 
+template <typename T, int kVecs, bool kPolicy>
+static int launch_short(const T* logits, int64_t ld, const policy::RowArgs& a, T* out, int64_t ld_out, int64_t rows, cudaStream_t s) {
+  policy::short_kernel<T, kVecs, kPolicy><<<(unsigned)((rows + policy::kShortWarps - 1) / policy::kShortWarps), policy::kShortWarps * 32, 0, s>>>(
+      logits, ld, a, out, ld_out, rows);
+  B2G_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
 template <typename T, bool kPolicy>
 static int launch_rows(const T* logits, int64_t ld, const policy::RowArgs& a, T* out, int64_t ld_out, int64_t rows, cudaStream_t s) {
   constexpr int N = 16 / sizeof(T);
-  const int64_t bytes = (a.V + 2 * (N - 1)) / N * 16;
+  const int64_t need = (a.V + 2 * (N - 1)) / N, bytes = need * 16;
+  if (need <= 32 * 4) return launch_short<T, 4, kPolicy>(logits, ld, a, out, ld_out, rows, s);
+  if (need <= 32 * 8) return launch_short<T, 8, kPolicy>(logits, ld, a, out, ld_out, rows, s);
+  if (need <= 32 * 16) return launch_short<T, 16, kPolicy>(logits, ld, a, out, ld_out, rows, s);
   if (bytes <= kSmallRow) return launch_held<T, 128, kPolicy>(logits, ld, a, out, ld_out, rows, 1, bytes, s);
   bool taken = false;
   if (int rc = launch_pipe<T, kPolicy>(logits, ld, a, out, ld_out, rows, s, &taken)) return rc;
@@ -1188,6 +1326,25 @@ static int launch_rows(const T* logits, int64_t ld, const policy::RowArgs& a, T*
     B2G_CUDA_OK(cudaGetLastError());
   }
   return 0;
+}
+
+// Blocks of 32, 128 or 256 threads, so that a short row does not leave most of one idle.
+template <typename T, int kThreads>
+static int launch_bwd_as(const T* logits, int64_t ld, const policy::RowArgs& a, const void* grad_logp, T* out, int64_t ld_out, int64_t rows,
+                         int64_t need, cudaStream_t s) {
+  const int64_t tile = kThreads * policy::kBwdVecs, blocks = (need + tile - 1) / tile;
+  B2G_REQUIRE(rows * blocks < (1ll << 31), "token_logprobs_bwd: %lld rows of %lld logits are too many for one call", (long long)rows, (long long)a.V);
+  policy::logp_bwd_kernel<T, kThreads><<<(unsigned)(rows * blocks), kThreads, 0, s>>>(logits, ld, a, grad_logp, out, ld_out, (int)blocks);
+  B2G_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+template <typename T>
+static int launch_bwd(const T* logits, int64_t ld, const policy::RowArgs& a, const void* grad_logp, T* out, int64_t ld_out, int64_t rows, cudaStream_t s) {
+  constexpr int N = 16 / sizeof(T);
+  const int64_t need = (a.V + 2 * (N - 1)) / N;
+  if (need <= 32 * policy::kBwdVecs) return launch_bwd_as<T, 32>(logits, ld, a, grad_logp, out, ld_out, rows, need, s);
+  if (need <= 128 * policy::kBwdVecs) return launch_bwd_as<T, 128>(logits, ld, a, grad_logp, out, ld_out, rows, need, s);
+  return launch_bwd_as<T, 256>(logits, ld, a, grad_logp, out, ld_out, rows, need, s);
 }
 
 extern "C" int b2g_token_logprobs(const void* logits, int64_t ld, int logits_dtype, const int64_t* target, void* logp, int logp_dtype, float* stats,
@@ -1215,17 +1372,9 @@ extern "C" int b2g_token_logprobs_bwd(const void* logits, int64_t ld, int logits
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   policy::RowArgs a = row_args(target, V, ignore_index, temperature, nullptr);
   a.logp64 = logp_dtype; a.stats = reinterpret_cast<float4*>(const_cast<float*>(stats));
-  const int n = logits_dtype ? 4 : 8, tile = policy::kBwdThreads * policy::kBwdVecs;
-  const int64_t blocks = ((V + 2 * (n - 1)) / n + tile - 1) / tile;
-  B2G_REQUIRE(rows * blocks < (1ll << 31), "token_logprobs_bwd: %lld rows of %lld logits are too many for one call", (long long)rows, (long long)V);
   if (logits_dtype)
-    policy::logp_bwd_kernel<float><<<(unsigned)(rows * blocks), policy::kBwdThreads, 0, s>>>(
-        static_cast<const float*>(logits), ld, a, grad_logp, static_cast<float*>(grad_logits), ld_grad, (int)blocks);
-  else
-    policy::logp_bwd_kernel<__nv_bfloat16><<<(unsigned)(rows * blocks), policy::kBwdThreads, 0, s>>>(
-        static_cast<const __nv_bfloat16*>(logits), ld, a, grad_logp, static_cast<__nv_bfloat16*>(grad_logits), ld_grad, (int)blocks);
-  B2G_CUDA_OK(cudaGetLastError());
-  return 0;
+    return launch_bwd(static_cast<const float*>(logits), ld, a, grad_logp, static_cast<float*>(grad_logits), ld_grad, rows, s);
+  return launch_bwd(static_cast<const __nv_bfloat16*>(logits), ld, a, grad_logp, static_cast<__nv_bfloat16*>(grad_logits), ld_grad, rows, s);
 }
 
 extern "C" int b2g_policy_loss(const void* logits, int64_t ld, int logits_dtype, const int64_t* target, const float* advantage,
