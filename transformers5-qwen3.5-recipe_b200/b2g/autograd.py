@@ -400,18 +400,21 @@ def _first_order_only(what: str) -> None:
 
 class _RouteExperts(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, bias, top_k, score_function, groups, top_groups, group_experts, renormalize, scaling_factor):
-        weights, indices = ops.route_experts(logits, top_k, bias, score_function, groups, top_groups, group_experts, renormalize, scaling_factor)
+    def forward(ctx, logits, bias, choice, weighting):
+        weights, indices = ops.route_experts(logits, choice[0], bias, weighting[0], *choice[1:], *weighting[1:])
+        ctx.set_materialize_grads(False)         # no zeros for the ids' gradient, which does not exist
         ctx.save_for_backward(logits, weights, indices)
-        ctx.settings = (score_function, renormalize, scaling_factor)
+        ctx.weighting = weighting
         ctx.mark_non_differentiable(indices)
         return weights, indices
 
     @staticmethod
     def backward(ctx, grad_weights, _grad_indices):
         _first_order_only("route_experts")
+        if grad_weights is None:
+            return None, None, None, None
         logits, weights, indices = ctx.saved_tensors
-        return (ops.route_experts_bwd(grad_weights.contiguous(), logits, weights, indices, *ctx.settings),) + (None,) * 8
+        return ops.route_experts_bwd(grad_weights.contiguous(), logits, weights, indices, *ctx.weighting), None, None, None
 
 
 def route_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor] = None, score_function: str = "softmax", groups: int = 1,
@@ -419,7 +422,7 @@ def route_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor]
     """``ops.route_experts`` whose weights carry the gradient to the logits (the bias enters the choice only and gets none)."""
     if not (logits.requires_grad and torch.is_grad_enabled()):
         return ops.route_experts(logits, top_k, bias, score_function, groups, top_groups, group_experts, renormalize, scaling_factor)
-    return _RouteExperts.apply(logits, bias, top_k, score_function, groups, top_groups, group_experts, renormalize, scaling_factor)
+    return _RouteExperts.apply(logits, bias, (top_k, groups, top_groups, group_experts), (score_function, renormalize, scaling_factor))
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -449,8 +452,9 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, temperature: floa
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logp, offsets, ref_logp, beta, label_smoothing, loss_type, average, target, ignore_index):
-        loss, chosen, rejected, coef = ops.preference_loss(logp, offsets, ref_logp, beta, label_smoothing, loss_type, average, target, ignore_index)
+    def forward(ctx, logp, offsets, ref_logp, settings, target, ignore_index):
+        loss, chosen, rejected, coef = ops.preference_loss(logp, offsets, ref_logp, *settings, target, ignore_index)
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(coef, offsets, target)
         ctx.num_tokens, ctx.ignore_index, ctx.dtype = logp.shape[0], ignore_index, logp.dtype
         ctx.mark_non_differentiable(chosen, rejected)
@@ -459,8 +463,10 @@ class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_loss, _grad_chosen, _grad_rejected):
         _first_order_only("preference_loss")
+        if grad_loss is None:
+            return (None,) * 6
         coef, offsets, target = ctx.saved_tensors
-        return (ops.preference_loss_bwd(grad_loss.contiguous(), coef, offsets, ctx.num_tokens, target, ctx.ignore_index, ctx.dtype),) + (None,) * 8
+        return (ops.preference_loss_bwd(grad_loss.contiguous(), coef, offsets, ctx.num_tokens, target, ctx.ignore_index, ctx.dtype),) + (None,) * 5
 
 
 def preference_loss(logp: torch.Tensor, offsets: torch.Tensor, ref_logp: Optional[torch.Tensor] = None, beta: float = 0.1,
@@ -468,4 +474,4 @@ def preference_loss(logp: torch.Tensor, offsets: torch.Tensor, ref_logp: Optiona
                     ignore_index: int = -100) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(loss [pairs], chosen rewards [pairs], rejected rewards [pairs])`` of ``ops.preference_loss``; the loss carries the
     gradient to ``logp``, the rewards are for logging."""
-    return _PreferenceLoss.apply(logp, offsets, ref_logp, float(beta), float(label_smoothing), loss_type, average, target, ignore_index)
+    return _PreferenceLoss.apply(logp, offsets, ref_logp, (float(beta), float(label_smoothing), loss_type, average), target, ignore_index)

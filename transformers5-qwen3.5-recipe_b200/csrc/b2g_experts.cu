@@ -6,7 +6,8 @@
 // One warp per token; lane i holds experts [i * kPer, (i + 1) * kPer), so the lowest lane of a tie holds the lowest expert.
 // The order of c is its order in 64 bits (without a bias: the order of the logits), so the choice does not depend on how an
 // exponential is rounded.  The work is done in 32 bits; where two neighbours of the order lie closer than the 32-bit scores can
-// be wrong and are not equal by construction (same logit, same bias), the warp goes over its token once more in 64 bits.
+// be wrong and are not equal by construction (same logit, same bias), the warp ranks its candidates once more in 64 bits.  Groups
+// that lie so close, and NaN among the logits, send it over the whole token in 64 bits.
 #include "b2g_common.cuh"
 
 namespace b2g {
@@ -209,6 +210,7 @@ struct WarpSpace {
     Pick candidate[32 * kPer];
   };
   Pick sorted[kMaxTopK + 1];
+  double exact[kCandidates];
 };
 
 // The best two of a group's choices.
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
   constexpr float kStep = 2.384185791015625e-7f;      // and 2^-22 of the sums
 
   // c[j]: what expert first + j is chosen by; NaN where there is none to choose
-  float c[kPer], top = -INFINITY, denominator = 1.f;
+  float c[kPer], top = -INFINITY, denominator = 1.f, smax = 1.f;
   load_lane<T, kPer>(row, first, E, wide, NAN, c);
   bool unsure = false;
   if constexpr (kScored) {
@@ -246,7 +248,6 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
     }
     unsure = __any_sync(0xffffffffu, odd);
     top = lanes_max(top);
-    float smax;
     if (fn == kSoftmax) {
       denominator = 0.f;
 #pragma unroll
@@ -324,6 +325,8 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
       if (head == floor_value) head = NAN;
     }
     if (floor_value != floor_value) floor_value = -INFINITY;
+    // so that nothing outside can belong among the first K even if the 32-bit choices are wrong
+    if (biased) floor_value -= 2.f * eps * smax + kStep * 2.f * fabsf(floor_value);
   }
   int n = 0;
 #pragma unroll
@@ -358,7 +361,43 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
     }
     __syncwarp();
     const bool out = lane < K;
-    const Pick p = out ? ws.sorted[lane] : Pick{0.f, 0};
+    Pick p = out ? ws.sorted[lane] : Pick{0.f, 0};
+    if (biased) {
+      bool close = false;
+      if (out && lane + 1 < min(n, ranks)) {
+        const Pick q = ws.sorted[lane + 1];            // a score is at most its choice less its bias, give or take a step
+        const float bp = bias[p.id], bq = bias[q.id];
+        close = !(p.c - q.c > eps * fmaxf(fabsf(p.c - bp), fabsf(q.c - bq)) + kStep * (fabsf(p.c) + fabsf(bp) + fabsf(bq))) &&
+                !(bp == bq && load_logit(row, p.id) == load_logit(row, q.id));
+      }
+      if (__any_sync(0xffffffffu, close)) {            // the candidates once more, in 64 bits
+        double all = 1.0;
+        if (fn == kSoftmax) {
+          float x[kPer];
+          load_lane<T, kPer>(row, first, E, wide, -INFINITY, x);
+          all = 0.0;
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) all += exp((double)x[j] - (double)top);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        }
+        for (int h = lane; h < n; h += 32) {
+          const int id = ws.candidate[h].id;
+          const double x = load_logit(row, id);
+          ws.exact[h] = (fn == kSoftmax ? exp(x - (double)top) / all : score_of(x, fn)) + (double)bias[id];
+        }
+        __syncwarp();
+        for (int h = lane; h < n; h += 32) {
+          const double mine = ws.exact[h];
+          const int id = ws.candidate[h].id;
+          int rank = 0;
+          for (int q = 0; q < n; ++q) rank += ws.exact[q] > mine || (ws.exact[q] == mine && ws.candidate[q].id < id);
+          if (rank < K) ws.sorted[rank] = ws.candidate[h];
+        }
+        __syncwarp();
+        if (out) p = ws.sorted[lane];
+      }
+    }
     const float x = biased || grouped ? load_logit(row, p.id) : p.c;
     float w = 0.f;
     if (fn == kSoftmax) {
@@ -366,31 +405,19 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
     } else {
       w = score_of(x, fn);
     }
-    if (biased) {
-      bool close = false;
-      if (out && lane + 1 < min(n, ranks)) {
-        const Pick q = ws.sorted[lane + 1];            // its score is at most its choice less its bias, give or take a step
-        const float bp = bias[p.id], bq = bias[q.id], xq = load_logit(row, q.id);
-        close = !(p.c - q.c > eps * fmaxf(w, fabsf(q.c - bq)) + kStep * (fabsf(p.c) + fabsf(bq))) && !(x == xq && bp == bq);
+    if (!out) w = 0.f;
+    if (renorm) {
+      if (fn == kSoftmax) {
+        const float m = kScored ? warp_maxf(out ? x : -INFINITY) : __shfl_sync(0xffffffffu, x, 0);
+        w = !out || m == -INFINITY ? 0.f : expf(x - m);
       }
-      unsure = __any_sync(0xffffffffu, close);
+      w = w / (warp_sum(w) + 1e-20f);
     }
-    if (!unsure) {
-      if (!out) w = 0.f;
-      if (renorm) {
-        if (fn == kSoftmax) {
-          const float m = kScored ? warp_maxf(out ? x : -INFINITY) : __shfl_sync(0xffffffffu, x, 0);
-          w = !out || (m == -INFINITY) ? 0.f : expf(x - m);
-        }
-        w = w / (warp_sum(w) + 1e-20f);
-      }
-      if (out) {
-        weights[t * K + lane] = w * alpha;
-        indices[t * K + lane] = p.id;
-      }
+    if (out) {
+      weights[t * K + lane] = w * alpha;
+      indices[t * K + lane] = p.id;
     }
-  }
-  if (unsure) {
+  } else {
     __syncwarp();
     route_in_64_bits<T, kPer>(row, bias, fn, G, M, best, renorm, alpha, weights + t * K, indices + t * K, E, K, ws.value);
   }

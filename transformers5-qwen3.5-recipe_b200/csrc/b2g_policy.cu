@@ -1082,39 +1082,16 @@ __global__ void __launch_bounds__(kBwdThreads) logp_bwd_kernel(const T* logits, 
 }
 
 // ---- preference loss ------------------------------------------------------------------------------
-constexpr int kPairThreads = 256;
-
-// Sums of 64 bits over one sequence's counted tokens.
-template <typename L>
-__device__ __forceinline__ void sequence_sum(const L* logp, const float* ref, const int64_t* target, int64_t begin, int64_t end,
-                                             int64_t ignore_index, double& sum, double& count) {
-  __shared__ double ps[kPairThreads / 32], pc[kPairThreads / 32];
-  double s = 0.0;
-  long long n = 0;
-  for (int64_t i = begin + threadIdx.x; i < end; i += kPairThreads) {
-    if (target && target[i] == ignore_index) continue;
-    s += ref ? (double)logp[i] - (double)ref[i] : (double)logp[i];
-    ++n;
-  }
-  double cnt = (double)n;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-    cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) { ps[threadIdx.x >> 5] = s; pc[threadIdx.x >> 5] = cnt; }
-  __syncthreads();
-  sum = count = 0.0;
-  for (int i = 0; i < kPairThreads / 32; ++i) { sum += ps[i]; count += pc[i]; }
-}
+// Latency, not bytes: a pair is a few thousand tokens.  A CTA of 1024 threads per pair, half of it on either sequence, and a
+// cluster of up to eight where the sequences are long on average; kAtOnce loads of each array are under way per thread.
+constexpr int kPairThreads = 1024, kHalf = kPairThreads / 2, kAtOnce = 4, kPairClusterMax = 8;
 
 // The bounds of sequence s, brought into [0, N]; a bound that had to be moved is reported.
 __device__ __forceinline__ void bounds(const int64_t* offsets, int64_t s, int64_t N, int64_t& begin, int64_t& end, int* status) {
   const int64_t b = offsets[s], e = offsets[s + 1];
   begin = b < 0 ? 0 : (b > N ? N : b);
   end = e < begin ? begin : (e > N ? N : e);
-  if ((b != begin || e != end) && threadIdx.x == 0 && status) atomicCAS(status, 0, 905);
+  if ((b != begin || e != end) && threadIdx.x % kHalf == 0 && status) atomicCAS(status, 0, 905);
 }
 
 __device__ __forceinline__ double log_sigmoid(double u) { return fmin(u, 0.0) - log1p(exp(-fabs(u))); }
@@ -1124,19 +1101,61 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(const L* __restrict_
                                                             const int64_t* __restrict__ target, const int64_t* __restrict__ offsets, int64_t N,
                                                             int64_t P, int64_t ignore_index, float beta, float smoothing, int squared, int average,
                                                             float* __restrict__ loss, float* __restrict__ chosen, float* __restrict__ rejected,
-                                                            float* __restrict__ coef, int* status) {
-  const int64_t p = blockIdx.x;
-  double sum[2], count[2];
-  for (int h = 0; h < 2; ++h) {
-    int64_t begin, end;
-    bounds(offsets, p + h * P, N, begin, end, status);
-    sequence_sum(logp, ref, target, begin, end, ignore_index, sum[h], count[h]);
-    if (!average) count[h] = 1.0;
-    count[h] = fmax(count[h], 1.0);
-    sum[h] /= count[h];
+                                                            float* __restrict__ coef, int* status, int cluster) {
+  constexpr int kHalfWarps = kHalf / 32;
+  __shared__ double warp_sum[kPairThreads / 32];
+  __shared__ int warp_count[kPairThreads / 32];
+  __shared__ double2 part[kPairClusterMax][2];       // of the cluster's first CTA: every CTA's sum and count of either sequence
+  const int rank = blockIdx.x % cluster, half = threadIdx.x / kHalf, thread = threadIdx.x % kHalf, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t p = blockIdx.x / cluster;
+  int64_t begin, end;
+  bounds(offsets, p + half * P, N, begin, end, status);
+  double s = 0.0;                                    // differences and sums in 64 bits
+  int n = 0;
+  const int64_t step = (int64_t)cluster * kHalf;
+  for (int64_t i = begin + (int64_t)rank * kHalf + thread; i < end; i += step * kAtOnce) {
+    int64_t y[kAtOnce];
+    L l[kAtOnce];
+    float f[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int64_t at = i + u * step;
+      const bool in = at < end;
+      y[u] = in ? (target ? target[at] : ignore_index + 1) : ignore_index;
+      l[u] = in ? logp[at] : (L)0;
+      f[u] = in && ref ? ref[at] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (y[u] != ignore_index) {                    // what stands in ignored places is not looked at
+        s += (double)l[u] - (double)f[u];
+        ++n;
+      }
+    }
   }
-  if (threadIdx.x == 0) {
-    const double b = beta, gap = sum[0] - sum[1], u = b * gap, e = smoothing;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
+  }
+  if (lane == 0) { warp_sum[warp] = s; warp_count[warp] = n; }
+  __syncthreads();
+  if (threadIdx.x < 2) {                             // thread h: sequence h
+    double sum = 0.0, count = 0.0;
+    for (int i = 0; i < kHalfWarps; ++i) { sum += warp_sum[threadIdx.x * kHalfWarps + i]; count += (double)warp_count[threadIdx.x * kHalfWarps + i]; }
+    const uint32_t to = dev::map_to_cta(dev::smem_u32(&part[rank][threadIdx.x]), 0);
+    asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(to), "d"(sum), "d"(count) : "memory");
+  }
+  dev::cluster_sync_all();
+  if (rank == 0 && threadIdx.x == 0) {
+    double value[2], count[2];
+    for (int h = 0; h < 2; ++h) {
+      value[h] = count[h] = 0.0;
+      for (int i = 0; i < cluster; ++i) { value[h] += part[i][h].x; count[h] += part[i][h].y; }
+      count[h] = average ? fmax(count[h], 1.0) : 1.0;
+      value[h] /= count[h];
+    }
+    const double b = beta, gap = value[0] - value[1], u = b * gap, e = smoothing;
     double l, slope;     // slope = d loss / d gap
     if (squared) {
       const double h = gap - 0.5 / b;
@@ -1147,33 +1166,56 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(const L* __restrict_
       slope = b * (e / (1.0 + exp(-u)) - (1.0 - e) / (1.0 + exp(u)));
     }
     loss[p] = (float)l;
-    chosen[p] = (float)(b * sum[0]);
-    rejected[p] = (float)(b * sum[1]);
+    chosen[p] = (float)(b * value[0]);
+    rejected[p] = (float)(b * value[1]);
     coef[p] = (float)(slope / count[0]);
     coef[P + p] = (float)(-slope / count[1]);
   }
 }
 
-// grad_logp[i] = grad_loss[pair] * coef[sequence] for counted tokens of a sequence, 0 elsewhere.  The sequence of a token is
-// found by bisection in the offsets.
+// grad_logp[i] = grad_loss[pair] * coef[sequence] for counted tokens of a sequence, 0 elsewhere.  A thread's first token finds its
+// sequence by bisection, in a copy of the offsets on chip where they fit; its others follow from there.
+constexpr int kPairBwdThreads = 256, kPairBwdTokens = 4, kOffsetsOnChip = 2049;
 template <typename L>
-__global__ void __launch_bounds__(256) pair_bwd_kernel(const float* __restrict__ grad_loss, const float* __restrict__ coef,
-                                                       const int64_t* __restrict__ target, const int64_t* __restrict__ offsets,
-                                                       L* __restrict__ grad_logp, int64_t N, int64_t P, int64_t ignore_index) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= N) return;
-  int64_t lo = 0, hi = 2 * P + 1;         // the number of offsets <= i
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (offsets[mid] <= i) lo = mid + 1;
-    else hi = mid;
+__global__ void __launch_bounds__(kPairBwdThreads) pair_bwd_kernel(const float* __restrict__ grad_loss, const float* __restrict__ coef,
+                                                                   const int64_t* __restrict__ target, const int64_t* __restrict__ offsets,
+                                                                   L* __restrict__ grad_logp, int64_t N, int64_t P, int64_t ignore_index) {
+  __shared__ int64_t on_chip[kOffsetsOnChip];
+  const int64_t entries = 2 * P + 1;
+  const bool copied = entries <= kOffsetsOnChip;
+  if (copied) {
+    for (int i = threadIdx.x; i < (int)entries; i += kPairBwdThreads) on_chip[i] = offsets[i];
+    __syncthreads();
   }
-  float g = 0.f;
-  if (lo >= 1 && lo <= 2 * P && !(target && target[i] == ignore_index)) {
-    const int64_t s = lo - 1;
-    g = grad_loss[s < P ? s : s - P] * coef[s];
+  const int64_t tile = (int64_t)blockIdx.x * (kPairBwdThreads * kPairBwdTokens);
+  int64_t y[kPairBwdTokens];
+#pragma unroll
+  for (int u = 0; u < kPairBwdTokens; ++u) {
+    const int64_t i = tile + u * kPairBwdThreads + threadIdx.x;
+    y[u] = i < N && target ? target[i] : ignore_index + 1;
   }
-  grad_logp[i] = g;
+  auto offset = [&](int64_t k) { return copied ? on_chip[k] : offsets[k]; };
+  int64_t lo = 0;                          // the number of offsets <= i
+#pragma unroll
+  for (int u = 0; u < kPairBwdTokens; ++u) {
+    const int64_t i = tile + u * kPairBwdThreads + threadIdx.x;
+    if (i >= N) return;
+    // most tiles lie within one sequence
+    if (u == 0 || (lo < entries && offset(lo) <= i)) {
+      int64_t hi = entries;
+      while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (offset(mid) <= i) lo = mid + 1;
+        else hi = mid;
+      }
+    }
+    float g = 0.f;
+    if (lo >= 1 && lo <= 2 * P && y[u] != ignore_index) {
+      const int64_t s = lo - 1;
+      g = grad_loss[s < P ? s : s - P] * coef[s];
+    }
+    grad_logp[i] = g;
+  }
 }
 
 }  // namespace policy
@@ -1399,7 +1441,7 @@ extern "C" int b2g_policy_loss(const void* logits, int64_t ld, int logits_dtype,
 extern "C" int b2g_preference_loss(const void* logp, int logp_dtype, const float* ref_logp, const int64_t* target, const int64_t* offsets, int64_t N,
                                    int64_t pairs, int64_t ignore_index, float beta, float label_smoothing, int loss_type, int average, float* loss,
                                    float* chosen, float* rejected, float* coef, int* status, void* stream) {
-  B2G_REQUIRE(N >= 0 && pairs >= 0 && pairs < (1ll << 30), "preference_loss: bad shape N=%lld pairs=%lld", (long long)N, (long long)pairs);
+  B2G_REQUIRE(N >= 0 && pairs >= 0 && pairs < (1ll << 28), "preference_loss: bad shape N=%lld pairs=%lld", (long long)N, (long long)pairs);
   B2G_REQUIRE(logp_dtype == 0 || logp_dtype == 1, "preference_loss: logp_dtype must be 0 (fp32) or 1 (fp64)");
   B2G_REQUIRE(beta > 0.f && beta <= 3.4e38f, "preference_loss: beta must be positive and finite");
   B2G_REQUIRE(label_smoothing >= 0.f && label_smoothing < 0.5f, "preference_loss: label_smoothing outside [0, 0.5)");
@@ -1407,16 +1449,24 @@ extern "C" int b2g_preference_loss(const void* logp, int logp_dtype, const float
   B2G_REQUIRE(loss_type == 0 || label_smoothing == 0.f, "preference_loss: label smoothing belongs to the sigmoid loss");
   if (pairs == 0) return 0;
   B2G_REQUIRE((logp || N == 0) && offsets && loss && chosen && rejected && coef, "preference_loss: null pointer");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // a CTA goes through 2048 tokens of either sequence in one turn of its loads
+  int cluster = 1;
+  while (cluster < policy::kPairClusterMax && N / (2 * pairs) > 2048 * cluster) cluster *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(pairs * cluster));
+  cfg.blockDim = dim3(policy::kPairThreads);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
   if (logp_dtype)
-    policy::pair_kernel<<<(unsigned)pairs, policy::kPairThreads, 0, s>>>(static_cast<const double*>(logp), ref_logp, target, offsets, N, pairs,
-                                                                         ignore_index, beta, label_smoothing, loss_type, average, loss, chosen, rejected,
-                                                                         coef, status);
+    B2G_CUDA_OK(cudaLaunchKernelEx(&cfg, policy::pair_kernel<double>, static_cast<const double*>(logp), ref_logp, target, offsets, N, pairs, ignore_index,
+                                   beta, label_smoothing, loss_type, average, loss, chosen, rejected, coef, status, cluster));
   else
-    policy::pair_kernel<<<(unsigned)pairs, policy::kPairThreads, 0, s>>>(static_cast<const float*>(logp), ref_logp, target, offsets, N, pairs,
-                                                                         ignore_index, beta, label_smoothing, loss_type, average, loss, chosen, rejected,
-                                                                         coef, status);
-  B2G_CUDA_OK(cudaGetLastError());
+    B2G_CUDA_OK(cudaLaunchKernelEx(&cfg, policy::pair_kernel<float>, static_cast<const float*>(logp), ref_logp, target, offsets, N, pairs, ignore_index,
+                                   beta, label_smoothing, loss_type, average, loss, chosen, rejected, coef, status, cluster));
   return 0;
 }
 
@@ -1427,11 +1477,12 @@ extern "C" int b2g_preference_loss_bwd(const float* grad_loss, const float* coef
   if (N == 0) return 0;
   B2G_REQUIRE((grad_loss && coef || pairs == 0) && offsets && grad_logp, "preference_loss_bwd: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned blocks = (unsigned)((N + 255) / 256);
+  const int64_t tile = policy::kPairBwdThreads * policy::kPairBwdTokens;
+  const unsigned blocks = (unsigned)((N + tile - 1) / tile);
   if (logp_dtype)
-    policy::pair_bwd_kernel<<<blocks, 256, 0, s>>>(grad_loss, coef, target, offsets, static_cast<double*>(grad_logp), N, pairs, ignore_index);
+    policy::pair_bwd_kernel<<<blocks, policy::kPairBwdThreads, 0, s>>>(grad_loss, coef, target, offsets, static_cast<double*>(grad_logp), N, pairs, ignore_index);
   else
-    policy::pair_bwd_kernel<<<blocks, 256, 0, s>>>(grad_loss, coef, target, offsets, static_cast<float*>(grad_logp), N, pairs, ignore_index);
+    policy::pair_bwd_kernel<<<blocks, policy::kPairBwdThreads, 0, s>>>(grad_loss, coef, target, offsets, static_cast<float*>(grad_logp), N, pairs, ignore_index);
   B2G_CUDA_OK(cudaGetLastError());
   return 0;
 }

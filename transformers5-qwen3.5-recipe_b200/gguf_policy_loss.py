@@ -102,6 +102,7 @@ class _PackedPolicyLoss(torch.autograd.Function):
                 grad[a:b] = torch.ops.b2g.mmq_grad_input(logits, payload, quant_type, rows.shape[1])
         if wanted:
             ctx.save_for_backward(grad)
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(logp, kl)
         return loss.sum(), logp, kl
 
@@ -109,6 +110,8 @@ class _PackedPolicyLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, _grad_logp, _grad_kl):
         if torch.is_grad_enabled():
             raise RuntimeError("Packed LM-head losses do not support higher-order gradients")
+        if grad_loss is None:
+            return (None,) * 11
         (grad,) = ctx.saved_tensors
         return (grad * grad_loss.to(grad.dtype),) + (None,) * 10
 
