@@ -6,8 +6,8 @@
 // One warp per token; lane i holds experts [i * kPer, (i + 1) * kPer), so the lowest lane of a tie holds the lowest expert.
 // The order of c is its order in 64 bits (without a bias: the order of the logits), so the choice does not depend on how an
 // exponential is rounded.  The work is done in 32 bits; where two neighbours of the order lie closer than the 32-bit scores can
-// be wrong and are not equal by construction (same logit, same bias), the warp ranks its candidates once more in 64 bits.  Groups
-// that lie so close, and NaN among the logits, send it over the whole token in 64 bits.
+// be wrong and are not equal by construction (same logit, same bias), the warp ranks its candidates, or its groups, once more in
+// 64 bits.  NaN among the logits send it over the whole token in 64 bits.
 #include "b2g_common.cuh"
 
 namespace b2g {
@@ -53,68 +53,87 @@ __device__ __forceinline__ float load_logit(const T* p, int64_t i) {
   else return p[i];
 }
 
-// The whole route of one token in 64 bits, by one warp.  The choices live in `value` (32 * kPer doubles of shared memory) and
-// everything else is computed again where it is needed: few registers, because the 32-bit pass would have to keep as many free.
+// One token's scores in 64 bits: of a warp whose lanes hold its experts.
 template <typename T, int kPer>
-__device__ __noinline__ void route_in_64_bits(const T* row, const float* bias, int fn, int G, int M, int best, int renorm, float alpha,
-                                              float* weights, int64_t* indices, int E, int K, double* value) {
-  const int lane = threadIdx.x & 31, first = lane * kPer, mine = max(0, min(kPer, E - first));
-  double top = -INFINITY, sum = 0.0;
-  if (fn == kSoftmax) {
+struct Exact {
+  const T* row;
+  const float* bias;
+  int fn;
+  double top, sum;
+  __device__ Exact(const T* row_, const float* bias_, int fn_, int E) : row(row_), bias(bias_), fn(fn_), top(-INFINITY), sum(0.0) {
+    if (fn != kSoftmax) return;
+    const int first = (threadIdx.x & 31) * kPer, mine = max(0, min(kPer, E - first));
 #pragma unroll 1
     for (int j = 0; j < mine; ++j) top = fmax(top, (double)load_logit(row, first + j));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll 1
-    for (int j = 0; j < mine; ++j) {
-      const double x = load_logit(row, first + j);
-      sum += top == -INFINITY && x == x ? 0.0 : exp(x - top);
-    }
+    for (int j = 0; j < mine; ++j) sum += part((double)load_logit(row, first + j));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  auto score = [&](double x) {
+  __device__ double part(double x) const { return top == -INFINITY && x == x ? 0.0 : exp(x - top); }
+  __device__ double score(double x) const {
     if (fn != kSoftmax) return score_of(x, fn);
-    const double e = top == -INFINITY && x == x ? 0.0 : exp(x - top);
+    const double e = part(x);
     return e == 0.0 ? 0.0 : e / sum;
-  };
+  }
+};
+
+// The best M of G groups, as a bit mask, in 64 bits.  `value` holds 32 * kPer doubles of shared memory.
+template <typename T, int kPer>
+__device__ __noinline__ unsigned groups_in_64_bits(const T* row, const float* bias, int fn, int G, int M, int best, int E, double* value) {
+  const Exact<T, kPer> exact(row, bias, fn, E);
+  const int lane = threadIdx.x & 31, first = lane * kPer, mine = max(0, min(kPer, E - first)), per = E / G;
+#pragma unroll 2
+  for (int j = 0; j < mine; ++j) {
+    const double v = exact.score((double)load_logit(row, first + j));
+    value[first + j] = bias ? v + (double)bias[first + j] : v;
+  }
+  __syncwarp();
+  unsigned long long worth = 0ull;
+  if (lane < G) {
+    double a = -INFINITY, b = -INFINITY;
+    int at = lane % per;                       // lanes start apart, so that they meet few of one another's banks
+#pragma unroll 2
+    for (int i = 0; i < per; ++i) {
+      const double v = value[lane * per + at];
+      at = at + 1 == per ? 0 : at + 1;
+      if (v > a || v != v) { b = a; a = v; }
+      else if (v > b) b = v;
+    }
+    worth = key_of(best == 2 && per > 1 ? a + b : a);
+  }
+  unsigned kept = 0u;
+#pragma unroll 1
+  for (int r = 0; r < M; ++r) {
+    const unsigned long long all = warp_max(worth);
+    const int g = __ffs(__ballot_sync(0xffffffffu, worth == all)) - 1;
+    kept |= 1u << g;
+    if (lane == g) worth = 0ull;
+  }
+  __syncwarp();
+  return kept;
+}
+
+// The whole route of one token in 64 bits, by one warp.  The choices live in `value` (32 * kPer doubles of shared memory) and
+// everything else is computed again where it is needed: few registers, because the 32-bit pass would have to keep as many free.
+template <typename T, int kPer>
+__device__ __noinline__ void route_in_64_bits(const T* row, const float* bias, int fn, int G, int M, int best, int renorm, float alpha,
+                                              float* weights, int64_t* indices, int E, int K, double* value) {
+  const Exact<T, kPer> exact(row, bias, fn, E);
+  const int lane = threadIdx.x & 31, first = lane * kPer, mine = max(0, min(kPer, E - first));
   uint32_t gone = 0u;       // bit j: expert first + j has been chosen, or its group dropped
   if (M < G) {
+    const unsigned kept = groups_in_64_bits<T, kPer>(row, bias, fn, G, M, best, E, value);
     const int per = E / G;
-#pragma unroll 1
-    for (int j = 0; j < mine; ++j) {
-      const double v = score((double)load_logit(row, first + j));
-      value[first + j] = bias ? v + (double)bias[first + j] : v;
-    }
-    __syncwarp();
-    unsigned long long worth = 0ull;
-    if (lane < G) {
-      double a = -INFINITY, b = -INFINITY;
-#pragma unroll 1
-      for (int i = 0; i < per; ++i) {
-        const double v = value[lane * per + i];
-        if (v > a || v != v) { b = a; a = v; }
-        else if (v > b) b = v;
-      }
-      worth = key_of(best == 2 && per > 1 ? a + b : a);
-    }
-    unsigned kept = 0u;
-#pragma unroll 1
-    for (int r = 0; r < M; ++r) {
-      const unsigned long long all = warp_max(worth);
-      const int g = __ffs(__ballot_sync(0xffffffffu, worth == all)) - 1;
-      kept |= 1u << g;
-      if (lane == g) worth = 0ull;
-    }
-    __syncwarp();
-#pragma unroll 1
     for (int j = 0; j < mine; ++j)
       if (!((kept >> ((first + j) / per)) & 1u)) gone |= 1u << j;
   }
 #pragma unroll 1
   for (int j = 0; j < mine; ++j) {
     const double x = load_logit(row, first + j);
-    value[first + j] = bias ? score(x) + (double)bias[first + j] : x;
+    value[first + j] = bias ? exact.score(x) + (double)bias[first + j] : x;
   }
   __syncwarp();
   int id = 0;         // lane r keeps the r-th choice
@@ -142,7 +161,7 @@ __device__ __noinline__ void route_in_64_bits(const T* row, const float* bias, i
     for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (out) w = m == -INFINITY && raw == raw ? 0.0 : exp(raw - m);
   } else if (out) {
-    w = score(raw);
+    w = exact.score(raw);
   }
   if (renorm) {
     double total = w;
@@ -218,11 +237,14 @@ struct Two { float a, b; };
 __device__ __forceinline__ Two add_to(Two t, float v) { return Two{fmaxf(t.a, v), fmaxf(t.b, fminf(t.a, v))}; }
 __device__ __forceinline__ Two merge(Two t, Two u) { return Two{fmaxf(t.a, u.a), fmaxf(fminf(t.a, u.a), fmaxf(t.b, u.b))}; }
 
+// per = E / G; lane_shift: log2 of the lanes that hold a group where groups are whole powers of two of lanes, else -1 (the host
+// divides once; eight divisions a lane cost more than the groups' arithmetic).
 // kScored: the choice needs the scores (a bias, groups) or the weights need the whole row's (softmax that is not renormalised).
 template <typename T, int kPer, bool kScored>
 __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ bias, int fn,
-                                                            int G, int M, int best, int renorm, float alpha, float* __restrict__ weights,
-                                                            int64_t* __restrict__ indices, int64_t tokens, int E, int K) {
+                                                            int G, int M, int best, int per, int lane_shift, int renorm, float alpha,
+                                                            float* __restrict__ weights, int64_t* __restrict__ indices, int64_t tokens, int E,
+                                                            int K) {
   __shared__ WarpSpace<kPer> space[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = lane * kPer;
   const int64_t t = (int64_t)blockIdx.x * kWarps + warp;
@@ -236,17 +258,19 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
 
   // c[j]: what expert first + j is chosen by; NaN where there is none to choose
   float c[kPer], top = -INFINITY, denominator = 1.f, smax = 1.f;
-  load_lane<T, kPer>(row, first, E, wide, NAN, c);
+  load_lane<T, kPer>(row, first, E, wide, kScored ? -INFINITY : NAN, c);
+  const bool ragged = first + kPer > E;
   bool unsure = false;
   if constexpr (kScored) {
     float s[kPer];
-    bool odd = false;                                  // NaN among the logits: left to the 64-bit pass
+    float sum = c[0];
+    top = c[0];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      odd = odd || (c[j] != c[j] && first + j < E);
+    for (int j = 1; j < kPer; ++j) {
+      sum += c[j];
       top = fmaxf(top, c[j]);
     }
-    unsure = __any_sync(0xffffffffu, odd);
+    unsure = __any_sync(0xffffffffu, sum != sum);      // NaN among the logits (or infinities of both signs): left to the 64-bit pass
     top = lanes_max(top);
     if (fn == kSoftmax) {
       denominator = 0.f;
@@ -266,20 +290,18 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
     }
     if (biased) {
       float b[kPer];
-      load_lane<float, kPer>(bias, first, E, (reinterpret_cast<uintptr_t>(bias) & 15) == 0, NAN, b);
+      load_lane<float, kPer>(bias, first, E, (reinterpret_cast<uintptr_t>(bias) & 15) == 0, 0.f, b);
 #pragma unroll
       for (int j = 0; j < kPer; ++j) s[j] = c[j] = s[j] + b[j];
     }
     if (grouped) {                                     // s: what the groups are compared by
-      const int per = E / G, lanes = per / kPer;
-      const bool on_lanes = lanes * kPer == per && (lanes & (lanes - 1)) == 0;
       Two two{-INFINITY, -INFINITY};
       int group = lane;
-      if (on_lanes) {                                  // a power of two of whole lanes per group: its last lane speaks for it
+      if (lane_shift >= 0) {                           // its first lane speaks for a group
 #pragma unroll
         for (int j = 0; j < kPer; ++j) two = add_to(two, s[j]);
-        for (int o = 1; o < lanes; o *= 2) two = merge(two, Two{__shfl_xor_sync(0xffffffffu, two.a, o), __shfl_xor_sync(0xffffffffu, two.b, o)});
-        group = lane % lanes == 0 ? lane / lanes : G;
+        for (int o = 1; o < 1 << lane_shift; o *= 2) two = merge(two, Two{__shfl_xor_sync(0xffffffffu, two.a, o), __shfl_xor_sync(0xffffffffu, two.b, o)});
+        group = (lane & ((1 << lane_shift) - 1)) == 0 ? lane >> lane_shift : G;
       } else {
 #pragma unroll
         for (int j = 0; j < kPer; ++j) ws.choice[first + j] = s[j];
@@ -304,12 +326,28 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
           last = all;
           if (lane == src) worth = NAN;
         } else {
-          unsure = unsure || !(last - all > 2.f * eps * smax + kStep * fabsf(last));
+          if (!(last - all > 2.f * eps * smax + kStep * fabsf(last)) && !unsure)
+            kept = groups_in_64_bits<T, kPer>(row, bias, fn, G, M, best, E, ws.value);
         }
       }
+      if (lane_shift >= 0) {
+        const bool stays = kept >> (lane >> lane_shift) & 1u;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) c[j] = stays ? c[j] : NAN;
+      } else {
+        int g = first / per, left = (g + 1) * per - first;      // group, and how many of its experts are still to come
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          if (left == 0) { ++g; left = per; }
+          --left;
+          if (!(kept >> (g & 31) & 1u)) c[j] = NAN;
+        }
+      }
+    }
+    if (ragged) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j)
-        if (first + j < E && !((kept >> ((first + j) / per)) & 1u)) c[j] = NAN;
+        if (first + j >= E) c[j] = NAN;
     }
   }
 
@@ -426,25 +464,31 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
 // dl from dw.  With u_j = w_j / alpha and dot = sum_i g_i w_i:  renormalised ds_j s_j = u_j (alpha g_j - dot), else ds_j s_j = g_j w_j;
 // the slopes of the score functions relative to the score are 1 - sigmoid (sigmoid), sigmoid / (2 softplus) (sqrtsoftplus) and
 // 1 (softmax, whose common denominator cancels when renormalised and otherwise gives every expert - s_e * dot).
-template <typename T, int kPer>
+// A warp takes kTokens tokens at once, 32 / kTokens lanes on the choices of each, and then writes their rows one after the other:
+// with one token a warp spent most of its time waiting for three short loads (65536 x 256 bf16, top 8: 16 us, 13.5 us with four).
+template <typename T, int kPer, int kTokens>
 __global__ void __launch_bounds__(kWarps * 32) route_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ grad_w,
                                                                 const float* __restrict__ weights, const int64_t* __restrict__ indices, int fn,
                                                                 int renorm, float alpha, T* __restrict__ grad, int64_t tokens, int E, int K) {
-  constexpr int N = 16 / sizeof(T);
-  __shared__ __align__(16) float value[kWarps][32 * kPer];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = lane * kPer;
-  const int64_t t = (int64_t)blockIdx.x * kWarps + warp;
-  if (t >= tokens) return;
-  const T* row = logits + t * ld;
-  const bool in = lane < K;
-  const float g = in ? grad_w[t * K + lane] : 0.f, w = in ? weights[t * K + lane] : 0.f;
-  const int64_t e64 = in ? indices[t * K + lane] : -1;
+  constexpr int N = 16 / sizeof(T), kLanes = 32 / kTokens;
+  __shared__ __align__(16) float value[kWarps][kTokens][32 * kPer];
+  __shared__ float dots[kWarps][kTokens];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = lane * kPer, mine = lane / kLanes, slot = lane % kLanes;
+  const int64_t t0 = ((int64_t)blockIdx.x * kWarps + warp) * kTokens, t = t0 + mine;
+  if (t0 >= tokens) return;
+  const bool in = t < tokens && slot < K;
+  const float g = in ? grad_w[t * K + slot] : 0.f, w = in ? weights[t * K + slot] : 0.f;
+  const int64_t e64 = in ? indices[t * K + slot] : -1;
   const bool ok = e64 >= 0 && e64 < E;
   const int e = ok ? (int)e64 : 0;
-  const float raw = ok && fn != kSoftmax ? load_logit(row, e) : 0.f;
+  const float raw = ok && fn != kSoftmax ? load_logit(logits + t * ld, e) : 0.f;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) value[warp][first + j] = 0.f;
-  const float dot = warp_sum(g * w);
+  for (int u = 0; u < kTokens; ++u)
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) value[warp][u][first + j] = 0.f;
+  float dot = g * w;
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
   float d = renorm ? (w / alpha) * (alpha * g - dot) : g * w;
   if (fn != kSoftmax) {
     const float n = expf(-fabsf(raw));
@@ -452,48 +496,58 @@ __global__ void __launch_bounds__(kWarps * 32) route_bwd_kernel(const T* __restr
     else d *= raw < -16.f ? 0.5f : (raw >= 0.f ? 1.f : n) / ((1.f + n) * 2.f * (fmaxf(raw, 0.f) + log1pf(n)));
   }
   __syncwarp();
-  if (ok) value[warp][e] = d;
+  if (ok) value[warp][mine][e] = d;
+  if (slot == 0) dots[warp][mine] = dot;
   __syncwarp();
-  float v[kPer];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) v[j] = value[warp][first + j];
-  if (fn == kSoftmax && !renorm) {
-    float x[kPer], sum = 0.f;
-    load_lane<T, kPer>(row, first, E, (reinterpret_cast<uintptr_t>(row) & 15) == 0, -INFINITY, x);
-    float top = x[0];
+  for (int u = 0; u < kTokens; ++u) {
+    if (t0 + u >= tokens) return;
+    float v[kPer];
 #pragma unroll
-    for (int j = 1; j < kPer; ++j) top = fmaxf(top, x[j]);
-    top = warp_maxf(top);
+    for (int j = 0; j < kPer; ++j) v[j] = value[warp][u][first + j];
+    if (fn == kSoftmax && !renorm) {
+      const T* row = logits + (t0 + u) * ld;
+      const float of_row = dots[warp][u];
+      float x[kPer], sum = 0.f;
+      load_lane<T, kPer>(row, first, E, (reinterpret_cast<uintptr_t>(row) & 15) == 0, -INFINITY, x);
+      float top = x[0];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      x[j] = top == -INFINITY && x[j] == x[j] ? 0.f : expf(x[j] - top);
-      sum += x[j];
-    }
-    sum = warp_sum(sum);
+      for (int j = 1; j < kPer; ++j) top = fmaxf(top, x[j]);
+      top = warp_maxf(top);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] -= x[j] == 0.f ? 0.f : x[j] / sum * dot;
-  }
-  T* out = grad + t * (int64_t)E;
-  if constexpr (kPer % N == 0) {
-    if (first + kPer <= E && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
-#pragma unroll
-      for (int i = 0; i < kPer; i += N) {
-        uint4 q;
-        if constexpr (sizeof(T) == 2)
-          q = make_uint4(dev::pack_bf16(v[i], v[i + 1]), dev::pack_bf16(v[i + 2], v[i + 3]), dev::pack_bf16(v[i + 4], v[i + 5]),
-                         dev::pack_bf16(v[i + 6], v[i + 7]));
-        else
-          q = make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
-        *reinterpret_cast<uint4*>(out + first + i) = q;
+      for (int j = 0; j < kPer; ++j) {
+        x[j] = top == -INFINITY && x[j] == x[j] ? 0.f : expf(x[j] - top);
+        sum += x[j];
       }
-      return;
-    }
-  }
+      sum = warp_sum(sum);
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    if (first + j < E) {
-      if constexpr (sizeof(T) == 2) out[first + j] = __float2bfloat16_rn(v[j]);
-      else out[first + j] = v[j];
+      for (int j = 0; j < kPer; ++j) v[j] -= x[j] == 0.f ? 0.f : x[j] / sum * of_row;
+    }
+    T* out = grad + (t0 + u) * (int64_t)E;
+    bool written = false;
+    if constexpr (kPer % N == 0) {
+      if (first + kPer <= E && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+        written = true;
+#pragma unroll
+        for (int i = 0; i < kPer; i += N) {
+          uint4 q;
+          if constexpr (sizeof(T) == 2)
+            q = make_uint4(dev::pack_bf16(v[i], v[i + 1]), dev::pack_bf16(v[i + 2], v[i + 3]), dev::pack_bf16(v[i + 4], v[i + 5]),
+                           dev::pack_bf16(v[i + 6], v[i + 7]));
+          else
+            q = make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
+          *reinterpret_cast<uint4*>(out + first + i) = q;
+        }
+      }
+    }
+    if (!written) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (first + j < E) {
+          if constexpr (sizeof(T) == 2) out[first + j] = __float2bfloat16_rn(v[j]);
+          else out[first + j] = v[j];
+        }
+      }
     }
   }
 }
@@ -540,9 +594,15 @@ extern "C" int b2g_route_experts(const void* logits, int64_t ld, int logits_dtyp
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int blocks = (int)((T + experts::kWarps - 1) / experts::kWarps);
   const bool scored = bias || top_groups < groups || (score_fn == experts::kSoftmax && !renormalize);
+  const int per_group = E / groups;
+  auto lane_shift = [&](int per_lane) {
+    for (int shift = 0; shift <= 5; ++shift)
+      if (per_group == per_lane << shift) return shift;
+    return -1;
+  };
 #define B2G_ROUTE_AS(TYPE, PER, SCORED)                                                                                                \
   experts::route_kernel<TYPE, PER, SCORED><<<blocks, experts::kWarps * 32, 0, s>>>(static_cast<const TYPE*>(logits), ld, bias, score_fn, groups, \
-      top_groups, group_experts, renormalize, scaling, weights, indices, T, E, top_k)
+      top_groups, group_experts, per_group, lane_shift(PER), renormalize, scaling, weights, indices, T, E, top_k)
 #define B2G_ROUTE(PER)                                                   \
   do {                                                                   \
     if (logits_dtype) {                                                  \
@@ -565,14 +625,22 @@ extern "C" int b2g_route_experts_bwd(const void* logits, int64_t ld, int logits_
   if (T == 0) return 0;
   B2G_REQUIRE(grad_weights && weights && indices && grad_logits, "route_experts_bwd: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int blocks = (int)((T + experts::kWarps - 1) / experts::kWarps);
-#define B2G_ROUTE_BWD(PER)                                                                                                                 \
-  if (logits_dtype)                                                                                                                        \
-    experts::route_bwd_kernel<float, PER><<<blocks, experts::kWarps * 32, 0, s>>>(static_cast<const float*>(logits), ld, grad_weights, weights, \
-        indices, score_fn, renormalize, scaling, static_cast<float*>(grad_logits), T, E, top_k);                                           \
-  else                                                                                                                                     \
-    experts::route_bwd_kernel<__nv_bfloat16, PER><<<blocks, experts::kWarps * 32, 0, s>>>(static_cast<const __nv_bfloat16*>(logits), ld,   \
-        grad_weights, weights, indices, score_fn, renormalize, scaling, static_cast<__nv_bfloat16*>(grad_logits), T, E, top_k)
+  // four tokens a warp where their choices fit its lanes and there are tokens for all SMs
+  const int tokens = top_k <= 8 && T >= 8192 ? 4 : 1;
+  const int blocks = (int)((T + experts::kWarps * tokens - 1) / (experts::kWarps * tokens));
+#define B2G_ROUTE_BWD_AS(TYPE, PER, TOKENS)                                                                                                \
+  experts::route_bwd_kernel<TYPE, PER, TOKENS><<<blocks, experts::kWarps * 32, 0, s>>>(static_cast<const TYPE*>(logits), ld, grad_weights, weights, \
+      indices, score_fn, renormalize, scaling, static_cast<TYPE*>(grad_logits), T, E, top_k)
+#define B2G_ROUTE_BWD(PER)                                              \
+  do {                                                                  \
+    if (logits_dtype) {                                                 \
+      if (tokens == 4) B2G_ROUTE_BWD_AS(float, PER, 4);                 \
+      else B2G_ROUTE_BWD_AS(float, PER, 1);                             \
+    } else {                                                            \
+      if (tokens == 4) B2G_ROUTE_BWD_AS(__nv_bfloat16, PER, 4);         \
+      else B2G_ROUTE_BWD_AS(__nv_bfloat16, PER, 1);                     \
+    }                                                                   \
+  } while (0)
   B2G_BY_EXPERTS(E, B2G_ROUTE_BWD);
   B2G_CUDA_OK(cudaGetLastError());
   return 0;
