@@ -11,7 +11,7 @@
  *     ([rows, K / block * block_bytes]); quant types use the GGML ids (8 = Q8_0, 10 = Q2_K,
  *     11 = Q3_K, 12 = Q4_K, 13 = Q5_K, 14 = Q6_K, 16 = IQ2_XXS, 22 = IQ2_S).
  *   - `status` (nullable) is a device int32 the kernels write a non-zero code into when a bounded
- *     device-side wait runs out (1xx-4xx) or an input is out of range (901 receive buffer too small, 902 label
+ *     device-side wait runs out (1xx-5xx) or an input is out of range (901 receive buffer too small, 902 label
  *     outside the vocabulary, 903 expert id outside [0, E), 904 expert offsets beyond the row count, 905 sequence offsets
  *     that decrease or leave the tokens); it is never written on a healthy run and only the first code is kept.
  *

@@ -75,9 +75,9 @@ __device__ __forceinline__ F2 exp_from(F2 z, F2 minus_m, const Scale& c) {
     return f2(expf(lo), expf(hi));
   }
 }
-// The sum without ex2's shortfall; the largest term is exp(0), which is exact.
+// The sum without ex2's shortfall.
 template <typename T>
-__device__ __forceinline__ double whole_sum(double d) { return sizeof(T) == 2 ? d + (d - 1.0) * kEx2Shortfall : d; }
+__device__ __forceinline__ double whole_sum(double d) { return sizeof(T) == 2 ? d * (1.0 + kEx2Shortfall) : d; }
 
 // Sixteen bytes of logits as floats, and back.
 template <typename T>
@@ -97,6 +97,14 @@ struct Vec {
   __device__ __forceinline__ void packed_again() {
 #pragma unroll
     for (int i = 0; i < 4; ++i) asm volatile("" : "+r"(w[i]));
+  }
+  // -inf in place of value j
+  __device__ __forceinline__ void take_out(int j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (sizeof(T) == 4) w[i] = i == j ? 0xFF800000u : w[i];
+      else w[i] = i != j >> 1 ? w[i] : (j & 1) ? (w[i] & 0xFFFFu) | 0xFF800000u : (w[i] & 0xFFFF0000u) | 0xFF80u;
+    }
   }
   __device__ __forceinline__ void set_nothing() {   // -inf everywhere: the maximum and the sum do not see it
 #pragma unroll
@@ -139,29 +147,6 @@ __device__ __forceinline__ Vec<T> scaled_exp(const Vec<T>& x, F2 minus_m, F2 fac
     }
   }
   return r;
-}
-
-// 2^(z c - reference) as pairs: two fused steps, the exponent rounded where it is small.
-__device__ __forceinline__ F2 ex2_pair(F2 t) {
-  float lo, hi;
-  split(t, lo, hi);
-  return f2(ex2(lo), ex2(hi));
-}
-template <typename T>
-__device__ __forceinline__ Vec<T> cotangent_vec(const Vec<T>& x, F2 minus_ref, F2 factor, const Scale& c) {
-  if constexpr (sizeof(T) == 4) {
-    return scaled_exp(x, minus_ref, factor, c);
-  } else {
-    Vec<T> r;
-    const F2 h = f2(c.hi, c.hi);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float lo, hi;
-      split(ex2_pair(fma2(x.pair(i), h, minus_ref)) * factor, lo, hi);
-      r.w[i] = dev::pack_bf16(lo, hi);
-    }
-    return r;
-  }
 }
 
 // A row as 16-byte vectors of the memory it lies in: vector v holds the columns [v * N - shift, (v + 1) * N - shift), so the
@@ -239,10 +224,7 @@ struct RowArgs {
   // log-probabilities
   void* logp;          // fp32, or fp64 when logp64
   int logp64;
-  // What the backward pass of the log-probabilities reads: what the exponentials are against, 1/sum, 1 - p of the target, lse.
-  // A positive 1/sum stands for the pipeline's form (16-bit logits: 2^(z log2(e)/tau - reference)), a negative one for
-  // exp((z - m)/tau).
-  float4* stats;
+  float4* stats;       // what the backward pass of the log-probabilities reads: m, 1/sum of exp((z - m)/tau), 1 - p of the target, lse
   // policy loss
   const float *advantage, *old_logp, *ref_logp, *weight;
   float clip_low, clip_high, kl_coef;
@@ -273,18 +255,6 @@ __device__ __forceinline__ float rest_of(double exact, float zy, double logp, fl
   return fabsf(lse) < 16384.f ? 1.f - expf(z - lse) : (float)exact;
 }
 
-// What a row's maximum, sum and target logit say.
-struct Scalars { double lse, logp; float rest; };
-template <typename T>
-__device__ __forceinline__ Scalars row_scalars(float m, double d, float zy, const RowArgs& a) {
-  Scalars s;
-  const double log_d = log(d);
-  s.lse = (double)m * a.inv_tau + log_d;
-  s.logp = ((double)zy - (double)m) * a.inv_tau - log_d;
-  s.rest = rest_of<T>(-expm1(s.logp), zy, s.logp, a.tau);
-  return s;
-}
-
 __device__ __forceinline__ void put_logp(const RowArgs& a, int64_t row, double logp, float4 stats) {
   if (a.logp64) static_cast<double*>(a.logp)[row] = logp;
   else static_cast<float*>(a.logp)[row] = (float)logp;
@@ -311,25 +281,55 @@ __device__ __forceinline__ float policy_scalars(const RowArgs& a, const Given& i
   return (float)(in.weight * slope);
 }
 
-// A maximum and the sum of exponentials against it.  The maximum starts at the type's lowest value, not at -inf, so that -inf
-// logits (a masked vocabulary) meet a finite maximum: exp(-inf - lowest) = 0.
+// What the exponentials of a row, or of a part of it, were taken against, and their sum WITHOUT the target's own term.  A
+// reference starts at the type's lowest value, not at -inf, so that -inf logits (a masked vocabulary) meet a finite one:
+// exp(-inf - lowest) = 0.
 struct Stat { float m; double d; };
 
-// The joint statistic of `count` lanes (a power of two), in every one of them.
-__device__ __forceinline__ Stat join_lanes(Stat s, int count, double inv_tau) {
+// The joint sum of `count` lanes (a power of two), in every one of them.
+template <int kCount>
+__device__ __forceinline__ Stat join_lanes(Stat s, double inv_tau) {
   float m = s.m;
-  for (int o = count / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (s.m != m) s.d *= exp(((double)s.m - (double)m) * inv_tau);
-  s.m = m;
-  for (int o = count / 2; o > 0; o >>= 1) s.d += __shfl_xor_sync(0xffffffffu, s.d, o);
-  return s;
+#pragma unroll
+  for (int o = kCount / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (s.d != 0.0 && s.m != m) s.d *= exp(((double)s.m - (double)m) * inv_tau);
+#pragma unroll
+  for (int o = kCount / 2; o > 0; o >>= 1) s.d += __shfl_xor_sync(0xffffffffu, s.d, o);
+  return Stat{m, s.d};
+}
+
+// The scalars of a live row.  The target's own term is added in 64 bits: where it dominates, nothing of the small rest is lost to
+// its rounding, and 1 - p is the rest's share without a cancellation.  Writes them (`write`) and, for the policy loss, returns the
+// coefficient of the cotangent, what to multiply the exponentials by, their reference and the target's entry.
+template <typename T, bool kPolicy>
+__device__ __forceinline__ float4 conclude(const RowArgs& a, const Stat& t, float zy, const Given& in, int64_t r, bool write) {
+  const double d = whole_sum<T>(t.d), above = ((double)zy - (double)t.m) * a.inv_tau, own = exp(above), all = own + d;
+  const double logp = own > d ? -log1p(d / own) : above - log(all);
+  const float per_sum = 1.f / (float)all, rest = rest_of<T>((double)((float)d * per_sum), zy, logp, a.tau);
+  if (!kPolicy) {
+    if (write) put_logp(a, r, logp, make_float4(t.m, per_sum, rest, (float)((double)zy * a.inv_tau - logp)));
+    return make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const float coef = (float)(policy_scalars(a, in, logp, r, write) * a.inv_tau);
+  return make_float4(coef, -coef * per_sum, t.m, coef * rest);
+}
+
+// A row that takes no part.
+template <bool kPolicy>
+__device__ __forceinline__ void conclude_nothing(const RowArgs& a, int64_t r) {
+  if (kPolicy) {
+    a.loss[r] = 0.f;
+    a.kl[r] = 0.f;
+    static_cast<float*>(a.logp)[r] = 0.f;
+  } else {
+    put_logp(a, r, 0.0, make_float4(0.f, 0.f, 0.f, 0.f));
+  }
 }
 
 // ---- rows held on chip ----------------------------------------------------------------------------
-// A cluster of 1, 2, 4 or 8 CTAs per row.  Every thread copies its vectors of the CTA's slice to shared memory (cp.async, no
-// registers) and is the only one that reads them back, so no barrier stands between the copy and the three passes over it:
-// maximum (while later groups of the copy are on their way), sum, cotangent.  Maximum and sum are joined over the cluster
-// through distributed shared memory.  The row crosses HBM once.
+// One CTA per row.  Every thread copies its vectors to shared memory (cp.async, no registers) and is the only one that reads
+// them back, so no barrier stands between the copy and the three passes over it: maximum (while later groups of the copy are on
+// their way), sum, cotangent.  The row crosses HBM once.
 constexpr int kGroups = 4;
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -362,52 +362,46 @@ __device__ __forceinline__ float vec_max(const Vec<T>& x, float m) {
   }
 }
 
-template <typename T, int kThreads, bool kPolicy>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) held_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out,
-                                                                         int cluster) {
-  constexpr int N = Vec<T>::N, kWarps = kThreads / 32;
-  extern __shared__ __align__(16) uint8_t slice[];
+constexpr int kHeldThreads = 128;
+
+template <typename T, bool kPolicy>
+__global__ void __launch_bounds__(kHeldThreads, 8) held_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out) {
+  constexpr int kWarps = kHeldThreads / 32, kStep = kHeldThreads * 16;
+  extern __shared__ __align__(16) uint8_t held[];
   __shared__ Stat warp_stat[kWarps];
-  __shared__ Stat slot[8];
   __shared__ float4 bcast;
-  const int rank = blockIdx.x % cluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t r = blockIdx.x / cluster, y = a.target[r];
-  const bool first = rank == 0 && threadIdx.x == 0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r = blockIdx.x, y = a.target[r];
   const Row<T> row(logits + r * ld, a.V);
   T* const o = kPolicy ? out + r * ld_out : nullptr;
   const bool wide = kPolicy && same_alignment(row.x, (const T*)o);
-  const int per = (row.nvec + cluster - 1) / cluster, begin = rank * per, end = min(begin + per, row.nvec);
-
-  bool live = target_ok(y, a, first);
+  bool live = target_ok(y, a, threadIdx.x == 0);
   Given in{1.f, 0.f, 0.f, 0.f};
   if (kPolicy) {
     in = given(a, r);
     live = live && in.weight != 0.f;
   }
-  if (!live) {      // the same for every CTA of the cluster
-    if (first) {
-      if (kPolicy) { a.loss[r] = 0.f; a.kl[r] = 0.f; static_cast<float*>(a.logp)[r] = 0.f; }
-      else put_logp(a, r, 0.0, make_float4(0.f, 0.f, 0.f, 0.f));
-    }
+  if (!live) {
+    if (threadIdx.x == 0) conclude_nothing<kPolicy>(a, r);
     if (kPolicy)
-      for (int v = begin + threadIdx.x; v < end; v += kThreads) row.store(o, v, zeros<T>(), wide);
+      for (int v = threadIdx.x; v < row.nvec; v += kHeldThreads) row.store(o, v, zeros<T>(), wide);
     return;
   }
 
-  // this thread's vectors: begin + threadIdx.x + i * kThreads, i < n, at mine + i * kThreads * 16
-  const int v0 = begin + threadIdx.x, n = v0 < end ? (end - v0 + kThreads - 1) / kThreads : 0;
-  const uint32_t mine = dev::smem_u32(slice) + threadIdx.x * 16;
-  const int group = (per + kThreads * kGroups - 1) / (kThreads * kGroups);
+  // this thread's vectors: threadIdx.x + i * kHeldThreads, i < n, at mine + i * kStep
+  const int n = row.nvec > (int)threadIdx.x ? (row.nvec - 1 - (int)threadIdx.x) / kHeldThreads + 1 : 0;
+  const uint32_t mine = dev::smem_u32(held) + threadIdx.x * 16;
+  const int group = (row.nvec + kHeldThreads * kGroups - 1) / (kHeldThreads * kGroups);
   const T* const base = row.x - row.shift;          // vector v lies at base + v * N
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
     const int stop = min(n, (g + 1) * group);
 #pragma unroll 4
     for (int i = g * group; i < stop; ++i) {
-      const int v = v0 + i * kThreads;
-      const uint32_t at = mine + i * (kThreads * 16);
+      const int v = threadIdx.x + i * kHeldThreads;
+      const uint32_t at = mine + i * kStep;
       if (row.full(v)) {
-        copy16(at, base + (int64_t)v * N);
+        copy16(at, base + (int64_t)v * Row<T>::N);
       } else {
         const Vec<T> x = row.load(v);
         dev::sts128(at, x.w[0], x.w[1], x.w[2], x.w[3]);
@@ -415,13 +409,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) held_kernel(const T
     }
     copy_commit();
   }
-  const float zy = to_float(row.x[y]);      // before any CTA of the row can overwrite it
-
-  float m = kLowest;
+  const float zy = to_float(row.x[y]);
+  float m = fmaxf(kLowest, zy);
   auto max_of = [&](int g) {
     const int stop = min(n, (g + 1) * group);
 #pragma unroll 4
-    for (int i = g * group; i < stop; ++i) m = vec_max(from_shared<T>(mine + i * (kThreads * 16)), m);
+    for (int i = g * group; i < stop; ++i) m = vec_max(from_shared<T>(mine + i * kStep), m);
   };
   copy_wait<3>(); max_of(0);
   copy_wait<2>(); max_of(1);
@@ -430,6 +423,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) held_kernel(const T
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
 
+  // the target's term is added in the end
+  const int vy = (int)((y + row.shift) / Row<T>::N);
+  const bool writer = vy % kHeldThreads == threadIdx.x;
+  if (writer) {
+    const uint32_t at = mine + vy / kHeldThreads * kStep;
+    Vec<T> x = from_shared<T>(at);
+    x.take_out((int)((y + row.shift) % Row<T>::N));
+    dev::sts128(at, x.w[0], x.w[1], x.w[2], x.w[3]);
+  }
   // Every warp sums against its own maximum, so no barrier comes first.  The terms of two vectors are summed in 32 bits,
   // everything above them in 64.
   const Scale c = a.c;
@@ -439,56 +441,34 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) held_kernel(const T
     int i = 0;
 #pragma unroll 2
     for (; i + 1 < n; i += 2)
-      d += (double)sum_of(exp_sum(from_shared<T>(mine + i * (kThreads * 16)), minus_m, c) +
-                          exp_sum(from_shared<T>(mine + (i + 1) * (kThreads * 16)), minus_m, c));
-    if (i < n) d += (double)sum_of(exp_sum(from_shared<T>(mine + i * (kThreads * 16)), minus_m, c));
+      d += (double)sum_of(exp_sum(from_shared<T>(mine + i * kStep), minus_m, c) + exp_sum(from_shared<T>(mine + (i + 1) * kStep), minus_m, c));
+    if (i < n) d += (double)sum_of(exp_sum(from_shared<T>(mine + i * kStep), minus_m, c));
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
   if (lane == 0) warp_stat[warp] = Stat{m, d};
   __syncthreads();
   if (warp == 0) {
-    Stat t = join_lanes(lane < kWarps ? warp_stat[lane] : Stat{kLowest, 0.0}, kWarps, a.inv_tau);
-    t.m = __shfl_sync(0xffffffffu, t.m, 0);   // a CTA of few warps has the sum in fewer lanes than the cluster has CTAs
-    t.d = __shfl_sync(0xffffffffu, t.d, 0);
-    if (lane < cluster) {                     // lane k gives this CTA's share to CTA k
-      const uint32_t to = dev::map_to_cta(dev::smem_u32(&slot[rank]), lane);
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(t.m) : "memory");
-      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to + 8), "d"(t.d) : "memory");
-    }
-  }
-  dev::cluster_sync_all();
-  if (warp == 0) {
-    Stat t = join_lanes(lane < cluster ? slot[lane] : Stat{kLowest, 0.0}, cluster, a.inv_tau);
-    if (lane == 0) {
-      t.d = whole_sum<T>(t.d);
-      const Scalars v = row_scalars<T>(t.m, t.d, zy, a);
-      if (kPolicy) {
-        const float coef = (float)(policy_scalars(a, in, v.logp, r, rank == 0) * a.inv_tau);
-        bcast = make_float4(coef, (float)(-coef / t.d), t.m, coef * v.rest);
-      } else if (rank == 0) {
-        put_logp(a, r, v.logp, make_float4(t.m, (float)(-1.0 / t.d), v.rest, (float)v.lse));
-      }
-    }
+    const Stat t = join_lanes<kWarps>(lane < kWarps ? warp_stat[lane] : Stat{kLowest, 0.0}, a.inv_tau);
+    if (lane == 0) bcast = conclude<T, kPolicy>(a, t, zy, in, r, true);
   }
   if (!kPolicy) return;
   __syncthreads();
-  const float coef = bcast.x;
-  if (coef == 0.f) {                          // clipped: nothing of the row is wanted
-    for (int i = 0; i < n; ++i) row.store(o, v0 + i * kThreads, zeros<T>(), wide);
+  const float4 b = bcast;
+  if (b.x == 0.f) {                           // clipped: nothing of the row is wanted
+    for (int i = 0; i < n; ++i) row.store(o, threadIdx.x + i * kHeldThreads, zeros<T>(), wide);
     return;
   }
-  const F2 factor = f2(bcast.y, bcast.y), minus_m = f2(-bcast.z, -bcast.z);
+  const F2 factor = f2(b.y, b.y), minus_m = f2(-b.z, -b.z);
   T* const to = o - row.shift;
 #pragma unroll 2
   for (int i = 0; i < n; ++i) {
-    const int v = v0 + i * kThreads;
-    const Vec<T> g = scaled_exp(from_shared<T>(mine + i * (kThreads * 16)), minus_m, factor, c);
-    if (wide && row.full(v)) __stcs(reinterpret_cast<uint4*>(to + (int64_t)v * N), make_uint4(g.w[0], g.w[1], g.w[2], g.w[3]));
+    const int v = threadIdx.x + i * kHeldThreads;
+    const Vec<T> g = scaled_exp(from_shared<T>(mine + i * kStep), minus_m, factor, c);
+    if (wide && row.full(v)) __stcs(reinterpret_cast<uint4*>(to + (int64_t)v * Row<T>::N), make_uint4(g.w[0], g.w[1], g.w[2], g.w[3]));
     else row.store(o, v, g, wide);
   }
-  const int vy = (int)((y + row.shift) / N);  // its writer puts the target's entry right
-  if (vy >= v0 && vy < end && (vy - v0) % kThreads == 0) o[y] = from_float<T>(bcast.w);
+  if (writer) o[y] = from_float<T>(b.w);      // its writer puts the target's entry right
 }
 
 // ---- short rows --------------------------------------------------------------------------------------
@@ -511,10 +491,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const T* logits
     live = live && in.weight != 0.f;
   }
   if (!live) {
-    if (lane == 0) {
-      if (kPolicy) { a.loss[r] = 0.f; a.kl[r] = 0.f; static_cast<float*>(a.logp)[r] = 0.f; }
-      else put_logp(a, r, 0.0, make_float4(0.f, 0.f, 0.f, 0.f));
-    }
+    if (lane == 0) conclude_nothing<kPolicy>(a, r);
     if (kPolicy)
       for (int v = lane; v < row.nvec; v += 32) row.store(o, v, zeros<T>(), wide);
     return;
@@ -528,38 +505,50 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const T* logits
     else x[i].set_nothing();
   }
   const float zy = to_float(row.x[y]);
+  const int vy = (int)((y + row.shift) / Vec<T>::N), jy = (int)((y + row.shift) % Vec<T>::N);
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) m = vec_max(x[i], m);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+  // the target's term is added in the end: -inf in its place, by masks made once (x is in registers, whose index must be static)
+  Vec<T> keep, put = zeros<T>();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) keep.w[i] = ~0u;
+  put.take_out(jy);
+  if (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keep.w[i] = put.w[i] >> 16 ? 0xFFFFu : put.w[i] ? 0xFFFF0000u : ~0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keep.w[i] = put.w[i] ? 0u : ~0u;
+  }
   double d = 0.0;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
+    if (lane + i * 32 == vy) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[i].w[k] = (x[i].w[k] & keep.w[k]) | put.w[k];
+    }
     x[i].packed_again();
     d += (double)sum_of(exp_sum(x[i], f2(-m, -m), a.c));
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-  d = whole_sum<T>(d);
-  const Scalars v = row_scalars<T>(m, d, zy, a);
-  if (!kPolicy) {
-    if (lane == 0) put_logp(a, r, v.logp, make_float4(m, (float)(-1.0 / d), v.rest, (float)v.lse));
-    return;
-  }
-  const float coef = (float)(policy_scalars(a, in, v.logp, r, lane == 0) * a.inv_tau), k = (float)(-coef / d);
-  const int vy = (int)((y + row.shift) / Vec<T>::N);
+  const float4 b = conclude<T, kPolicy>(a, Stat{m, d}, zy, in, r, lane == 0);
+  if constexpr (kPolicy) {
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int u = lane + i * 32;
-    x[i].packed_again();
-    if (u < row.nvec) row.store(o, u, coef == 0.f ? zeros<T>() : scaled_exp(x[i], f2(-m, -m), f2(k, k), a.c), wide);
+    for (int i = 0; i < kVecs; ++i) {
+      const int u = lane + i * 32;
+      x[i].packed_again();
+      if (u < row.nvec) row.store(o, u, b.x == 0.f ? zeros<T>() : scaled_exp(x[i], f2(-m, -m), f2(b.y, b.y), a.c), wide);
+    }
+    if (b.x != 0.f && vy % 32 == lane) o[y] = from_float<T>(b.w);      // its writer puts the target's entry right
   }
-  if (coef != 0.f && vy % 32 == lane) o[y] = from_float<T>(coef * v.rest);      // its writer puts the target's entry right
 }
 
 // ---- rows in a pipeline ------------------------------------------------------------------------------
 // Clusters that stay and go from row to row, two CTAs on every SM (two whose phases differ keep memory and the special-function
-// unit busier than one of twice the size: 1024 x 248320 bf16 in 215 against 233 us), each with `slots` slices of rows in shared
+// unit busier than one of twice the size: 1024 x 248320 bf16 in 218 against 233 us), each with `slots` slices of rows in shared
 // memory.  13 warps work, two more do everything that is latency.  For every row k:
 //   the first of them reads 128 samples and the target's logit, and publishes their maximum as the row's reference: a sum of
 //     exponentials needs no maximum, only a number near it, so the workers need no pass for one and their sums simply add up;
@@ -569,14 +558,10 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const T* logits
 //   the first warp adds them up and sends the CTA's share to the others of the cluster (asynchronous remote stores that count on
 //     their barrier); the second adds the shares, finishes the row's scalars and lets the workers know;
 //   G(k), the cotangent, `lead` rows after S(k): the workers never wait for the exchange.
-// The target's own term is added in 64 bits: where it dominates, nothing of the small rest is lost to its rounding, and 1 - p
-// is the rest's share without a cancellation.
 // A warp's vectors are its own: it fetches them (one bulk copy per row, issued by one lane: as 16-byte copies of every lane they
 // took the load-store unit as long as the arithmetic), reads them in S and in G, and fetches those of the row `slots` further
 // on into the same place.
-// A row whose sum is no number, or 0 (NaN, +inf, a vocabulary masked throughout by the type's lowest value) is summed again by
-// the scalar warps alone, and G then takes the exact form of the exponent.
-// What bounds it: two exponentials per logit at 16 per cycle and SM (126 us of the 215), then HBM (155 us); the two overlap
+// What bounds it: two exponentials per logit at 16 per cycle and SM (126 us of the 218), then HBM (155 us); the two overlap
 // only between CTAs.  Replacing one exponential in four by a polynomial on the fp32 pipe was slower (231 us): the loops issue
 // 12 instructions per logit, and the polynomial adds six to every one that it replaces.
 // All waits are bounded; a CTA whose wait ran out stops working, and all CTAs of a cluster leave together.
@@ -651,39 +636,7 @@ struct Part {
 // What the workers need to know of a row: what to sum against, and its target, or -1 where it takes no part.
 struct Info { float reference; int y; };
 
-// What the workers sum against: bf16 in units of log2 (any number serves, so its rounding costs nothing), fp32 as a logit.
-template <typename T>
-__device__ __forceinline__ float reference_of(float m, const Scale& c) {
-  return sizeof(T) == 2 ? fminf(fmaxf(m * c.hi, -3e38f), 3e38f) : fmaxf(m, kLowest);
-}
-template <typename T>
-__device__ __forceinline__ F2 sum_vec(const Vec<T>& x, F2 minus_ref, const Scale& c) {
-  constexpr int P = Vec<T>::N / 2;
-  F2 e[P];
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    if constexpr (sizeof(T) == 2) e[i] = ex2_pair(fma2(x.pair(i), f2(c.lo, c.lo), fma2(x.pair(i), f2(c.hi, c.hi), minus_ref)));
-    else e[i] = exp_from<T, true>(x.pair(i), minus_ref, c);
-  }
-#pragma unroll
-  for (int s = P / 2; s > 0; s >>= 1)
-#pragma unroll
-    for (int i = 0; i < s; ++i) e[i] = e[i] + e[i + s];
-  return e[0];
-}
 constexpr double kFarAbove = 16384.0;      // 2^14
-// The joint sum of a warp's lanes, whose references differ only where one of them met a logit far above the others'.
-template <typename T>
-__device__ __forceinline__ Stat join_references(Stat s, double inv_tau) {
-  float m = s.m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (s.d != 0.0 && s.m != m) s.d *= sizeof(T) == 2 ? exp2((double)s.m - (double)m) : exp(((double)s.m - (double)m) * inv_tau);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s.d += __shfl_xor_sync(0xffffffffu, s.d, o);
-  return Stat{m, s.d};
-}
-
 // A warp's sum over its vectors in shared memory, n of this lane's 512 bytes apart.
 template <typename T>
 __device__ __forceinline__ double warp_sum_against(uint32_t place, int n, float ref, const Scale& c) {
@@ -693,8 +646,8 @@ __device__ __forceinline__ double warp_sum_against(uint32_t place, int n, float 
   int i = 0;
 #pragma unroll 2
   for (; i + 1 < n; i += 2)
-    d = d + (sum_vec(from_shared<T>(place + i * kStep), minus_ref, c) + sum_vec(from_shared<T>(place + (i + 1) * kStep), minus_ref, c));
-  if (i < n) d = d + sum_vec(from_shared<T>(place + i * kStep), minus_ref, c);
+    d = d + (exp_sum(from_shared<T>(place + i * kStep), minus_ref, c) + exp_sum(from_shared<T>(place + (i + 1) * kStep), minus_ref, c));
+  if (i < n) d = d + exp_sum(from_shared<T>(place + i * kStep), minus_ref, c);
   float lo, hi;
   split(d, lo, hi);
   double all = (double)lo + (double)hi;
@@ -709,24 +662,7 @@ __device__ __noinline__ Stat warp_sum_far(uint32_t place, int n, Scale c) {
   for (int i = 0; i < n; ++i) m = vec_max(from_shared<T>(place + i * 512), m);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float ref = reference_of<T>(m, c);
-  return Stat{ref, warp_sum_against<T>(place, n, ref, c)};
-}
-
-// One warp's sum over columns [begin, end) of a row but for column y, against their maximum.
-template <typename T>
-__device__ __noinline__ Stat sum_again(const T* x, int begin, int end, int y, const RowArgs& a) {
-  const int lane = threadIdx.x & 31;
-  float m = kLowest;
-  for (int i = begin + lane; i < end; i += 32) m = fmaxf(m, to_float(x[i]));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  double d = 0.0;
-  for (int i = begin + lane; i < end; i += 32)
-    if (i != y) d += exp(((double)to_float(x[i]) - (double)m) * a.inv_tau);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-  return Stat{m, d};
+  return Stat{m, warp_sum_against<T>(place, n, m, c)};
 }
 
 template <typename T, bool kPolicy>
@@ -736,13 +672,11 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
   extern __shared__ __align__(16) uint8_t space[];
   __shared__ uint64_t arrived[kMaxSlots][kWorkerWarps];      // one per slot and warp: a warp's copies are its own
   __shared__ __align__(16) Share share[kRing][kMaxCluster];
-  __shared__ __align__(16) Share share_again[2][kMaxCluster];   // a CTA sends its next one only after all have sent the one before
   __shared__ Stat sums[kRing][kWorkerWarps];
   __shared__ __align__(8) Info info[kInfo];
   __shared__ float known[kInfo];                 // the target's logit
   __shared__ float4 bcast[kRing];
-  __shared__ int exact_form[kRing];
-  __shared__ uint64_t referred[kInfo], summed[kRing], joined[kRing], joined_again[2], ready[kRing];
+  __shared__ uint64_t referred[kInfo], summed[kRing], joined[kRing], ready[kRing];
   __shared__ int gave_up;
   const int rank = blockIdx.x % cluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t first = blockIdx.x / cluster, stride = gridDim.x / cluster;
@@ -756,13 +690,11 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
       dev::mbar_init(dev::smem_u32(&joined[i]), 1);
       dev::mbar_init(dev::smem_u32(&ready[i]), 1);
     }
-    for (int i = 0; i < 2; ++i) dev::mbar_init(dev::smem_u32(&joined_again[i]), 1);
     dev::fence_barrier_init();
   }
   dev::cluster_sync_all();          // nobody sends to a barrier that is not there yet
 
   if (warp == kWorkerWarps) {       // references, and the CTA's share
-    const Scale c = a.c;
     const int64_t apart = a.V / (32 * kSamples);
     float sample[kSamples], target_logit = 0.f;
     int y_ahead = -1;
@@ -791,7 +723,7 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (lane == 0) {
-        info[k % kInfo] = Info{reference_of<T>(m, c), y_ahead};
+        info[k % kInfo] = Info{m, y_ahead};
         known[k % kInfo] = target_logit;
         dev::mbar_arrive(dev::smem_u32(&referred[k % kInfo]));
       }
@@ -805,13 +737,12 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
       look_at(k + kAhead);
       if (!dev::mbar_wait(dev::smem_u32(&summed[p]), parity, &gave_up, a.status, 501)) break;
       // of a row that takes no part nobody looks at it
-      const Stat t = join_references<T>(lane < kWorkerWarps ? sums[p][lane] : Stat{kLowest, 0.0}, a.inv_tau);
+      const Stat t = join_lanes<32>(lane < kWorkerWarps ? sums[p][lane] : Stat{kLowest, 0.0}, a.inv_tau);
       if (lane < cluster)
         send_share(dev::map_to_cta(dev::smem_u32(&share[p][rank]), lane), dev::map_to_cta(dev::smem_u32(&joined[p]), lane), Share{t.m, 0.f, t.d});
       refer(k + kAhead);
     }
   } else if (warp == kWorkerWarps + 1) {       // the row's scalars
-    int again = 0;                  // rows that needed the second exchange
     int64_t target_next = a.target[first];
     Given given_next{1.f, 0.f, 0.f, 0.f};
     if (kPolicy) given_next = given(a, first);
@@ -828,48 +759,13 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
       const bool live = target_ok(y, a, rank == 0 && lane == 0) && in.weight != 0.f;
       if (!wait_cluster(bar, parity, &gave_up, a.status, 502)) break;
       if (live) {
-        const Stat sum = join_references<T>(lane < cluster ? Stat{share[p][lane].m, share[p][lane].d} : Stat{kLowest, 0.0}, a.inv_tau);
-        double d = sum.d;
-        if (sizeof(T) == 2) d += d * kEx2Shortfall;
-        const float zy = known[k % kInfo];
-        float ref = sum.m;
-        // the target's own term
-        double own = sizeof(T) == 2 ? exp2((double)zy * (a.inv_tau * 1.4426950408889634) - (double)ref) : exp(((double)zy - (double)ref) * a.inv_tau);
-        bool exact = false;
-        if (!(own + d > 0.0 && own + d < 1e300)) {             // the same for every CTA: they added the same numbers
-          exact = true;
-          const int shift = (int)((uint32_t)reinterpret_cast<uintptr_t>(logits + r * ld) & 15u) / (int)sizeof(T);
-          const int64_t begin = (int64_t)rank * per * N - shift, end = min(a.V, (int64_t)(rank + 1) * per * N - shift);
-          const Stat s = sum_again(logits + r * ld, (int)(begin < 0 ? 0 : begin), (int)end, (int)y, a);
-          const int p2 = again % 2, parity2 = (again / 2) & 1;
-          const uint32_t bar2 = dev::smem_u32(&joined_again[p2]);
-          ++again;
-          if (lane == 0) dev::mbar_arrive_expect_tx(bar2, cluster * (uint32_t)sizeof(Share));
-          __syncwarp();
-          if (lane < cluster) send_share(dev::map_to_cta(dev::smem_u32(&share_again[p2][rank]), lane), dev::map_to_cta(bar2, lane), Share{s.m, 0.f, s.d});
-          if (!wait_cluster(bar2, parity2, &gave_up, a.status, 505)) break;
-          const Share got = lane < cluster ? share_again[p2][lane] : Share{kLowest, 0.f, 0.0};
-          const Stat t = join_lanes(Stat{got.m, got.d}, 32, a.inv_tau);
-          ref = t.m;
-          d = t.d;
-          own = exp(((double)zy - (double)ref) * a.inv_tau);
-        }
-        const double logp = -log1p(d / own), all = own + d;
-        // the sum may be beyond 32 bits' range where the reference was far too low
-        const float per_sum = all < 1e38 && all > 1e-37 ? 1.f / (float)all : (float)(1.0 / all);
+        const Stat sum = join_lanes<32>(lane < cluster ? Stat{share[p][lane].m, share[p][lane].d} : Stat{kLowest, 0.0}, a.inv_tau);
         if (lane == 0) {
-          const float rest = rest_of<T>((double)((float)d * per_sum), zy, logp, a.tau);
-          if (kPolicy) {
-            const float coef = (float)(policy_scalars(a, in, logp, r, rank == 0) * a.inv_tau);
-            bcast[p] = make_float4(coef, -coef * per_sum, ref, coef * rest);
-            exact_form[p] = exact;
-          } else if (rank == 0) {
-            put_logp(a, r, logp, make_float4(ref, exact ? -per_sum : per_sum, rest, (float)((double)zy * a.inv_tau - logp)));
-          }
+          const float4 b = conclude<T, kPolicy>(a, sum, known[k % kInfo], in, r, rank == 0);
+          if (kPolicy) bcast[p] = b;
         }
       } else if (rank == 0 && lane == 0) {
-        if (kPolicy) { a.loss[r] = 0.f; a.kl[r] = 0.f; static_cast<float*>(a.logp)[r] = 0.f; }
-        else put_logp(a, r, 0.0, make_float4(0.f, 0.f, 0.f, 0.f));
+        conclude_nothing<kPolicy>(a, r);
       }
       __syncwarp();
       if (lane == 0) dev::mbar_arrive(dev::smem_u32(&ready[p]));
@@ -947,12 +843,8 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
             for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, zeros<T>());
           } else {
             const F2 factor = f2(b.y, b.y), minus_ref = f2(-b.z, -b.z);
-            if (exact_form[p]) {
-              for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled_exp(from_shared<T>(place + i * kStep), minus_ref, factor, c));
-            } else {
 #pragma unroll 2
-              for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, cotangent_vec(from_shared<T>(place + i * kStep), minus_ref, factor, c));
-            }
+            for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled_exp(from_shared<T>(place + i * kStep), minus_ref, factor, c));
             if (part.owns(y, begin, lane) >= 0) o[y] = from_float<T>(b.w);              // its writer puts the target's entry right
           }
         }
@@ -996,10 +888,7 @@ __global__ void __launch_bounds__(512) wide_kernel(const T* logits, int64_t ld, 
     live = live && in.weight != 0.f;
   }
   if (!live) {
-    if (threadIdx.x == 0) {
-      if (kPolicy) { a.loss[r] = 0.f; a.kl[r] = 0.f; static_cast<float*>(a.logp)[r] = 0.f; }
-      else put_logp(a, r, 0.0, make_float4(0.f, 0.f, 0.f, 0.f));
-    }
+    if (threadIdx.x == 0) conclude_nothing<kPolicy>(a, r);
     if (kPolicy)
       for (int v = threadIdx.x; v < row.nvec; v += kThreads) row.store(o, v, zeros<T>(), wide);
     return;
@@ -1009,34 +898,29 @@ __global__ void __launch_bounds__(512) wide_kernel(const T* logits, int64_t ld, 
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
   const Scale c = a.c;
+  const float zy = to_float(row.x[y]);
+  const int vy = (int)((y + row.shift) / N), jy = (int)((y + row.shift) % N);
   double d = 0.0;
-  for (int v = threadIdx.x; v < row.nvec; v += kThreads) d += (double)sum_of(exp_sum(row.load(v), f2(-m, -m), c));
+  for (int v = threadIdx.x; v < row.nvec; v += kThreads) {
+    Vec<T> x = row.load(v);
+    if (v == vy) x.take_out(jy);                // the target's term is added in the end
+    d += (double)sum_of(exp_sum(x, f2(-m, -m), c));
+  }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
   if (lane == 0) warp_stat[warp] = Stat{m, d};
-  const float zy = to_float(row.x[y]);
   __syncthreads();
   if (warp == 0) {
-    Stat t = join_lanes(lane < kWarps ? warp_stat[lane] : Stat{kLowest, 0.0}, kWarps, a.inv_tau);
-    if (lane == 0) {
-      t.d = whole_sum<T>(t.d);
-      const Scalars v = row_scalars<T>(t.m, t.d, zy, a);
-      if (kPolicy) {
-        const float coef = (float)(policy_scalars(a, in, v.logp, r, true) * a.inv_tau);
-        bcast = make_float4(coef, (float)(-coef / t.d), t.m, coef * v.rest);
-      } else {
-        put_logp(a, r, v.logp, make_float4(t.m, (float)(-1.0 / t.d), v.rest, (float)v.lse));
-      }
-    }
+    const Stat t = join_lanes<kWarps>(lane < kWarps ? warp_stat[lane] : Stat{kLowest, 0.0}, a.inv_tau);
+    if (lane == 0) bcast = conclude<T, kPolicy>(a, t, zy, in, r, true);
   }
   if (!kPolicy) return;
   __syncthreads();
-  const float coef = bcast.x;
-  const F2 factor = f2(bcast.y, bcast.y), minus_m = f2(-bcast.z, -bcast.z);
+  const float4 b = bcast;
+  const F2 factor = f2(b.y, b.y), minus_m = f2(-b.z, -b.z);
   for (int v = threadIdx.x; v < row.nvec; v += kThreads)
-    row.store(o, v, coef == 0.f ? zeros<T>() : scaled_exp(row.load(v), minus_m, factor, c), wide);
-  const int vy = (int)((y + row.shift) / N);
-  if (coef != 0.f && vy % kThreads == threadIdx.x) o[y] = from_float<T>(bcast.w);
+    row.store(o, v, b.x == 0.f ? zeros<T>() : scaled_exp(row.load(v), minus_m, factor, c), wide);
+  if (b.x != 0.f && vy % kThreads == threadIdx.x) o[y] = from_float<T>(b.w);
 }
 
 // ---- gradient of the log-probabilities --------------------------------------------------------------
@@ -1062,9 +946,7 @@ __global__ void __launch_bounds__(kBwdThreads) logp_bwd_kernel(const T* logits, 
     return;
   }
   const float4 st = a.stats[r];
-  const float per_sum = fabsf(st.y);
-  const bool natural = !(st.y > 0.f);
-  const F2 factor = f2(-g * per_sum, -g * per_sum), minus_m = f2(-st.x, -st.x);
+  const F2 factor = f2(-g * st.y, -g * st.y), minus_m = f2(-st.x, -st.x);
   Vec<T> x[kBwdVecs];
 #pragma unroll
   for (int i = 0; i < kBwdVecs; ++i) {
@@ -1075,7 +957,7 @@ __global__ void __launch_bounds__(kBwdThreads) logp_bwd_kernel(const T* logits, 
 #pragma unroll
   for (int i = 0; i < kBwdVecs; ++i) {
     const int v = begin + i * kBwdThreads + threadIdx.x;
-    if (v < row.nvec) row.store(o, v, natural ? scaled_exp(x[i], minus_m, factor, a.c) : cotangent_vec(x[i], minus_m, factor, a.c), wide);
+    if (v < row.nvec) row.store(o, v, scaled_exp(x[i], minus_m, factor, a.c), wide);
   }
   const int at = (int)((y + row.shift) / N) - begin - (int)threadIdx.x;      // its writer puts the target's entry right
   if (at >= 0 && at < kBwdThreads * kBwdVecs && at % kBwdThreads == 0) o[y] = from_float<T>(g * st.z);
@@ -1245,10 +1127,10 @@ static policy::RowArgs row_args(const int64_t* target, int64_t V, int64_t ignore
 
 // Which kernel, cluster and slices.
 //   Rows of at most 16 vectors of 16 bytes a lane (bf16: 4081 logits): short_kernel, a warp per row (200,000 x 1000 bf16: log-
-//     probabilities 111 us, 617 us with a CTA per row).
+//     probabilities 123 us, 617 us with a CTA per row).
 //   Rows of at most kSmallRow bytes: held_kernel with one CTA of 128 threads per row, many CTAs per SM (20,000 x 10,000 bf16: loss
-//     186 us, 262 us in the pipeline, whose rows cost as much as 20 to 30 KB however short they are; 16,000: 173 and 188; 20,000:
-//     186 and 186).
+//     183 us, 262 us in the pipeline, whose rows cost as much as 20 to 30 KB however short they are; 16,000: 161 and 188; 20,000:
+//     186 and 189).
 //   Else pipe_kernel with the cluster size whose clusters have the fewest bytes to go through one after the other,
 //     rounds * (slice + kRoundBytes),  rounds = rows / clusters that the device holds at once (of 296 places 8-CTA clusters fill
 //     264, 9-CTA clusters 270, 5-CTA clusters 280: the GPCs have 16 to 20 SMs), among those whose slices leave room for two
@@ -1327,21 +1209,11 @@ static int launch_pipe(const T* logits, int64_t ld, const policy::RowArgs& a, T*
   return 0;
 }
 
-template <typename T, int kThreads, bool kPolicy>
-static int launch_held(const T* logits, int64_t ld, const policy::RowArgs& a, T* out, int64_t ld_out, int64_t rows, int cluster, int64_t bytes,
-                       cudaStream_t s) {
-  B2G_KERNEL_SMEM((policy::held_kernel<T, kThreads, kPolicy>), kSmallRow);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)bytes;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  B2G_CUDA_OK(cudaLaunchKernelEx(&cfg, policy::held_kernel<T, kThreads, kPolicy>, logits, ld, a, out, ld_out, cluster));
+template <typename T, bool kPolicy>
+static int launch_held(const T* logits, int64_t ld, const policy::RowArgs& a, T* out, int64_t ld_out, int64_t rows, int64_t bytes, cudaStream_t s) {
+  B2G_KERNEL_SMEM((policy::held_kernel<T, kPolicy>), kSmallRow);
+  policy::held_kernel<T, kPolicy><<<(unsigned)rows, policy::kHeldThreads, (size_t)bytes, s>>>(logits, ld, a, out, ld_out);
+  B2G_CUDA_OK(cudaGetLastError());
   return 0;
 }
 
@@ -1360,7 +1232,7 @@ static int launch_rows(const T* logits, int64_t ld, const policy::RowArgs& a, T*
   if (need <= 32 * 4) return launch_short<T, 4, kPolicy>(logits, ld, a, out, ld_out, rows, s);
   if (need <= 32 * 8) return launch_short<T, 8, kPolicy>(logits, ld, a, out, ld_out, rows, s);
   if (need <= 32 * 16) return launch_short<T, 16, kPolicy>(logits, ld, a, out, ld_out, rows, s);
-  if (bytes <= kSmallRow) return launch_held<T, 128, kPolicy>(logits, ld, a, out, ld_out, rows, 1, bytes, s);
+  if (bytes <= kSmallRow) return launch_held<T, kPolicy>(logits, ld, a, out, ld_out, rows, bytes, s);
   bool taken = false;
   if (int rc = launch_pipe<T, kPolicy>(logits, ld, a, out, ld_out, rows, s, &taken)) return rc;
   if (!taken) {
