@@ -122,7 +122,7 @@ B2G_API int b2g_cross_entropy_inplace(void* logits, int64_t ld, const int64_t* t
  *   logp[row] = z[target] / temperature - log sum_i exp(z[i] / temperature)
  * in fp32 or fp64 (logp_dtype 0 | 1: sums over long sequences keep their digits in fp64).  stats[row] (4 floats, 16-byte
  * aligned) = {max z, 1 / sum_i exp((z[i] - max z) / temperature), 1 - p of the target, log-sum-exp} is what the gradient reads.  A row whose target is
- * ignore_index gets logp 0 and its logits are not looked at; a target outside [0, V) is reported (status 902) and treated the
+ * ignore_index gets logp 0 whatever its logits are; a target outside [0, V) is reported (status 902) and treated the
  * same way.  -inf logits have probability zero; a live row that holds NaN or +inf, or nothing but -inf, gives NaN.
  * This entry has no counterpart in the reference (its losses are supervised only). */
 B2G_API int b2g_token_logprobs(const void* logits, int64_t ld, int logits_dtype, const int64_t* target, void* logp, int logp_dtype, float* stats,
@@ -139,15 +139,15 @@ B2G_API int b2g_token_logprobs_bwd(const void* logits, int64_t ld, int logits_dt
  * old_logp is null), d = ref_logp - logp, A = advantage and w = weight (1 when null):
  *   loss = w * ( -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * kl ),   kl = e^d - d - 1 (0 without ref_logp)
  *   grad_logits = (d loss / d logp) * (onehot - softmax) / temperature   in the logits' type, possibly in place.
- * A row takes part when its target is in [0, V) and its weight is not 0; every other row gives zeros in all four outputs and
- * nothing else of it is read.  A target that is neither ignore_index nor in [0, V) is reported (status 902).
+ * A row takes part when its target is in [0, V) and its weight is not 0; every other row gives zeros in all four outputs
+ * whatever else it holds.  A target that is neither ignore_index nor in [0, V) is reported (status 902).
  * This entry has no counterpart in the reference. */
 B2G_API int b2g_policy_loss(const void* logits, int64_t ld, int logits_dtype, const int64_t* target, const float* advantage,
                     const float* old_logp, const float* ref_logp, const float* weight, float clip_low, float clip_high, float kl_coef,
                     float temperature, float* loss, float* logp, float* kl, void* grad_logits, int64_t ld_grad, int64_t rows, int64_t V,
                     int64_t ignore_index, int* status, void* stream);
 
-/* Preference loss on pairs of sequences.  logp (fp32 or fp64: logp_dtype 0 | 1), ref_logp (fp32, nullable) and target (nullable) hold N tokens; sequence s is the
+/* Preference loss on pairs of sequences.  logp and ref_logp (nullable; either in fp32 or fp64: *_dtype 0 | 1) and target (nullable) hold N tokens; sequence s is the
  * tokens [offsets[s], offsets[s + 1]) and offsets has 2 * pairs + 1 entries: the `pairs` chosen sequences, then the rejected
  * ones in the same order.  L_s = sum (average: mean) of logp - ref_logp over the tokens whose target is not ignore_index, an
  * empty sequence gives 0; with gap = L_chosen - L_rejected
@@ -155,8 +155,8 @@ B2G_API int b2g_policy_loss(const void* logits, int64_t ld, int logits_dtype, co
  *   loss_type 1: loss = (gap - 1 / (2 beta))^2
  * chosen / rejected = beta * L_s (rewards, [pairs]); coef[2 * pairs] = d loss / d logp of a counted token of each sequence.
  * Offsets that decrease or leave [0, N] are brought into range and reported (status 905).  This entry has no counterpart in the reference. */
-B2G_API int b2g_preference_loss(const void* logp, int logp_dtype, const float* ref_logp, const int64_t* target, const int64_t* offsets, int64_t N,
-                        int64_t pairs, int64_t ignore_index, float beta, float label_smoothing, int loss_type, int average, float* loss, float* chosen,
+B2G_API int b2g_preference_loss(const void* logp, int logp_dtype, const void* ref_logp, int ref_dtype, const int64_t* target,
+                        const int64_t* offsets, int64_t N, int64_t pairs, int64_t ignore_index, float beta, float label_smoothing, int loss_type, int average, float* loss, float* chosen,
                         float* rejected, float* coef, int* status, void* stream);
 
 /* grad_logp[i] = grad_loss[pair] * coef[sequence] for counted tokens, 0 for ignored tokens and tokens of no sequence,

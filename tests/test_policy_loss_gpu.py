@@ -379,6 +379,19 @@ def test_preference_loss(cuda, lengths, average, kind, smoothing, dtype):
         assert bool((grad.cpu()[~counted] == 0).all())
 
 
+def test_preference_types_of_the_reference(cuda):
+    """The reference's log-probabilities in either type: the same numbers give the same result, whatever they are held in."""
+    from b2g import ops
+
+    logp, rf, target, ends = _pairs([300, 5, 0, 77], 41)
+    on = dict(target=target.to(cuda), average=True)
+    for a in (logp, logp.double()):
+        got = [ops.preference_loss(a.to(cuda), ends.to(cuda), ref_logp=b.to(cuda), **on) for b in (rf, rf.double())]
+        assert all(torch.equal(x, y) for x, y in zip(*got))
+    with pytest.raises(TypeError, match="ref_logp"):
+        ops.preference_loss(logp.to(cuda), ends.to(cuda), ref_logp=rf.bfloat16().to(cuda))
+
+
 def test_preference_gradient_against_differences(cuda):
     from b2g import autograd as ag
 

@@ -33,7 +33,7 @@ def test_no_rows_is_no_work(lib):
     assert lib.b2g_token_logprobs(None, 8, 0, None, None, 0, None, 0, 8, f(1.0), -100, None, None) == 0
     assert lib.b2g_token_logprobs_bwd(None, 8, 0, None, None, None, 0, None, 8, 0, 8, f(1.0), -100, None) == 0
     assert lib.b2g_policy_loss(None, 8, 0, None, None, None, None, None, f(0.2), f(0.2), f(0), f(1), None, None, None, None, 8, 0, 8, -100, None, None) == 0
-    assert lib.b2g_preference_loss(None, 0, None, None, None, 0, 0, -100, f(0.1), f(0), 0, 0, None, None, None, None, None, None) == 0
+    assert lib.b2g_preference_loss(None, 0, None, 0, None, None, 0, 0, -100, f(0.1), f(0), 0, 0, None, None, None, None, None, None) == 0
     assert lib.b2g_preference_loss_bwd(None, None, None, None, None, 0, 0, 0, -100, None) == 0
 
 
@@ -52,7 +52,7 @@ def test_loss_entries(lib):
     assert lib.b2g_token_logprobs(None, 8, 0, None, None, 2, None, 2, 8, f(1.0), -100, None, None) == -1 and b"logp_dtype" in lib.b2g_last_error()
 
     def pairs(beta=0.1, smooth=0.0, kind=0, pairs_=2, dtype=0):
-        rc = lib.b2g_preference_loss(None, dtype, None, None, None, 4, pairs_, -100, f(beta), f(smooth), kind, 0, None, None, None, None, None, None)
+        rc = lib.b2g_preference_loss(None, dtype, None, 0, None, None, 4, pairs_, -100, f(beta), f(smooth), kind, 0, None, None, None, None, None, None)
         return rc, lib.b2g_last_error()
 
     for kw, what in ((dict(beta=0.0), b"beta"), (dict(smooth=0.5), b"label_smoothing"), (dict(kind=2), b"loss_type"), (dict(kind=1, smooth=0.1), b"smoothing"),

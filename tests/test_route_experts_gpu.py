@@ -237,3 +237,35 @@ def test_refusals(cuda):
     (first,) = torch.autograd.grad(_route(y, 4)[0].sum(), y, create_graph=False)
     with pytest.raises(RuntimeError, match="higher-order"):
         torch.autograd.grad(_route(y, 4)[0].sum(), y, create_graph=True)
+
+
+@pytest.mark.parametrize("fn", ["softmax", "sigmoid", "sqrtsoftplus"])
+def test_a_single_renormalised_choice_has_no_gradient(cuda, fn):
+    """Its weight is the scaling factor whatever its score is; what is left of the gradient is below 1e-16 of the cotangent."""
+    g = torch.Generator().manual_seed(13)
+    for dtype in (torch.bfloat16, torch.float32):
+        for alpha in (1.0, 1.5, 2.7):
+            x = (torch.randn(200, 24, generator=g) * 2).to(dtype).to(cuda).requires_grad_(True)
+            w, _ = _route(x, 1, score_function=fn, scaling_factor=alpha)
+            assert bool((w == torch.tensor(alpha)).all())
+            cot = torch.randn(200, 1, generator=g).to(cuda)
+            (grad,) = torch.autograd.grad(w, x, cot)
+            assert float(grad.float().abs().max()) < 1e-15 * float(cot.abs().max())
+
+
+def test_gradient_where_one_expert_has_nearly_all_the_weight(cuda):
+    """fp32 logits, a row dominated by one of its choices: 1 - w is 1e-5 ... 1e-9 there, and the gradient is proportional to it.
+    Softmax takes it from fp32 weights (off by half a step of 1), the other scores from the logits in 64 bits."""
+    g = torch.Generator().manual_seed(14)
+    logits = torch.randn(100, 32, generator=g) - 14.0
+    logits[:, 3] = 2.0
+    for fn, tol in (("sigmoid", 2.0 ** -22), ("sqrtsoftplus", 2.0 ** -22)):
+        x = logits.to(cuda).requires_grad_(True)
+        w, idx = _route(x, 4, score_function=fn)
+        cot = torch.randn(100, 4, generator=g)
+        (grad,) = torch.autograd.grad(w, x, cot.to(cuda))
+        x64 = logits.double().requires_grad_(True)
+        (want,) = torch.autograd.grad(ref.weights(x64, idx.cpu(), fn, True, 1.0), x64, cot.double())
+        off = (grad.cpu().double() - want).abs()
+        scale = want.abs().amax(1, keepdim=True)
+        assert bool((off <= tol * want.abs() + 2.0 ** -40 * scale).all()), fn

@@ -28,7 +28,7 @@ SIGNATURES = {
     "b2g_token_logprobs_bwd": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _f32, _i64, _vp]),
     "b2g_policy_loss": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp,
                                _vp]),
-    "b2g_preference_loss": (_i32, [_vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b2g_preference_loss": (_i32, [_vp, _i32, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _f32, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "b2g_preference_loss_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp]),
     "b2g_lora_down": (_i32, [_vp, _vp, _i32, _f32, _vp, _vp, _i64, _i64, _i32, _vp]),
     "b2g_lora_wgrad_workspace_bytes": (_i64, [_i64, _i64]),

@@ -457,7 +457,7 @@ def preference_loss(logp: torch.Tensor, offsets: torch.Tensor, ref_logp: Optiona
                     ignore_index: int = -100):
     """Preference loss of pairs of sequences: ``(loss [pairs], chosen [pairs], rejected [pairs], coef [2 * pairs])``.
 
-    Sequence ``s`` is the tokens ``offsets[s]:offsets[s + 1]`` of ``logp``; the chosen sequences come first, the rejected ones
+    ``logp`` and ``ref_logp`` are fp32 or fp64 (sums are in fp64).  Sequence ``s`` is the tokens ``offsets[s]:offsets[s + 1]``; the chosen sequences come first, the rejected ones
     follow in the same order.  ``L_s`` is the sum (``average``: the mean) of ``logp - ref_logp`` over the tokens whose
     ``target`` is not ``ignore_index`` (all of them without ``target``), 0 for a sequence without tokens.  ``"sigmoid"``:
     ``-(1 - label_smoothing) log sigmoid(beta gap) - label_smoothing log sigmoid(-beta gap)``, ``gap = L_chosen - L_rejected``;
@@ -470,7 +470,10 @@ def preference_loss(logp: torch.Tensor, offsets: torch.Tensor, ref_logp: Optiona
         raise ValueError(f"logp must be a vector, got {tuple(logp.shape)}")
     n = logp.shape[0]
     pairs = _pair_shapes(n, logp, offsets, target)
-    _row_vector(ref_logp, logp, n, torch.float32, "ref_logp")
+    if ref_logp is not None:
+        if ref_logp.dtype not in _LOGP_DTYPES:
+            raise TypeError(f"ref_logp must be fp32 or fp64, got {ref_logp.dtype}")
+        _row_vector(ref_logp, logp, n, ref_logp.dtype, "ref_logp")
     if loss_type not in _PAIR_LOSSES:
         raise ValueError(f"loss_type must be one of {sorted(_PAIR_LOSSES)}, got {loss_type!r}")
     if not 0.0 < beta < float("inf"):
@@ -479,7 +482,8 @@ def preference_loss(logp: torch.Tensor, offsets: torch.Tensor, ref_logp: Optiona
         raise ValueError(f"label_smoothing must lie in [0, 0.5) and belongs to the sigmoid loss, got {label_smoothing}")
     loss, chosen, rejected = torch.empty(3, pairs, dtype=torch.float32, device=logp.device).unbind(0)
     coef = torch.empty(2 * pairs, dtype=torch.float32, device=logp.device)
-    _launch("b2g_preference_loss", logp, _a(logp), int(logp.dtype == torch.float64), _a(ref_logp), _a(target), _a(offsets), n, pairs,
+    _launch("b2g_preference_loss", logp, _a(logp), int(logp.dtype == torch.float64), _a(ref_logp),
+            int(ref_logp is not None and ref_logp.dtype == torch.float64), _a(target), _a(offsets), n, pairs,
             int(ignore_index), float(beta), float(label_smoothing), _PAIR_LOSSES[loss_type], int(bool(average)), _a(loss), _a(chosen),
             _a(rejected), _a(coef), _a(status_word(logp.device)))
     return loss, chosen, rejected, coef

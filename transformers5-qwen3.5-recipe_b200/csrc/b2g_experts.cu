@@ -464,6 +464,8 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
 // dl from dw.  With u_j = w_j / alpha and dot = sum_i g_i w_i:  renormalised ds_j s_j = u_j (alpha g_j - dot), else ds_j s_j = g_j w_j;
 // the slopes of the score functions relative to the score are 1 - sigmoid (sigmoid), sigmoid / (2 softplus) (sqrtsoftplus) and
 // 1 (softmax, whose common denominator cancels when renormalised and otherwise gives every expert - s_e * dot).
+// The choices' own terms are in 64 bits, and each product is rounded before the difference: alpha g_j - dot cancels where one
+// expert has nearly all the weight, and with a single choice it is 0 and has to come out as 0.
 // A warp takes kTokens tokens at once, 32 / kTokens lanes on the choices of each, and then writes their rows one after the other:
 // with one token a warp spent most of its time waiting for three short loads (65536 x 256 bf16, top 8: 16 us, 13.5 us with four).
 template <typename T, int kPer, int kTokens>
@@ -486,18 +488,34 @@ __global__ void __launch_bounds__(kWarps * 32) route_bwd_kernel(const T* __restr
   for (int u = 0; u < kTokens; ++u)
 #pragma unroll
     for (int j = 0; j < kPer; ++j) value[warp][u][first + j] = 0.f;
-  float dot = g * w;
+  const double g64 = g, raw64 = raw;
+  double own = 0.0, part = w, total = 1.0;           // a score, its weight, and what it was divided by
+  if (fn != kSoftmax) {
+    own = ok ? score_of(raw64, fn) : 0.0;
+    if (renorm) {
+      total = own;
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      total += 1e-20;
+    }
+    part = __dmul_rn((double)alpha, own) / total;
+  }
+  double dot = __dmul_rn(g64, part);
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-  float d = renorm ? (w / alpha) * (alpha * g - dot) : g * w;
-  if (fn != kSoftmax) {
-    const float n = expf(-fabsf(raw));
-    if (fn == kSigmoid) d *= (raw >= 0.f ? n : 1.f) / (1.f + n);
-    else d *= raw < -16.f ? 0.5f : (raw >= 0.f ? 1.f : n) / ((1.f + n) * 2.f * (fmaxf(raw, 0.f) + log1pf(n)));
+  double slope = __dmul_rn((double)alpha, g64);      // dL/ds
+  if (renorm) slope = __dadd_rn(slope, -dot) / total;
+  double d;
+  if (fn == kSoftmax) {
+    d = slope * (part / (double)alpha);              // not renormalised: alpha g s, and the row's share below
+  } else {
+    const double sig = 1.0 / (1.0 + exp(-raw64));
+    if (fn == kSigmoid) d = slope * (sig * (1.0 / (1.0 + exp(raw64))));
+    else d = raw64 < -600.0 ? slope * 0.5 * own : slope * (sig / (2.0 * own));      // far below 0 both are e^(x/2) / 2
   }
   __syncwarp();
-  if (ok) value[warp][mine][e] = d;
-  if (slot == 0) dots[warp][mine] = dot;
+  if (ok) value[warp][mine][e] = (float)d;
+  if (slot == 0) dots[warp][mine] = (float)dot;
   __syncwarp();
 #pragma unroll
   for (int u = 0; u < kTokens; ++u) {

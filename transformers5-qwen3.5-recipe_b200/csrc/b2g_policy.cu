@@ -978,8 +978,8 @@ __device__ __forceinline__ void bounds(const int64_t* offsets, int64_t s, int64_
 
 __device__ __forceinline__ double log_sigmoid(double u) { return fmin(u, 0.0) - log1p(exp(-fabs(u))); }
 
-template <typename L>
-__global__ void __launch_bounds__(kPairThreads) pair_kernel(const L* __restrict__ logp, const float* __restrict__ ref,
+template <typename L, typename R>
+__global__ void __launch_bounds__(kPairThreads) pair_kernel(const L* __restrict__ logp, const R* __restrict__ ref,
                                                             const int64_t* __restrict__ target, const int64_t* __restrict__ offsets, int64_t N,
                                                             int64_t P, int64_t ignore_index, float beta, float smoothing, int squared, int average,
                                                             float* __restrict__ loss, float* __restrict__ chosen, float* __restrict__ rejected,
@@ -998,14 +998,14 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(const L* __restrict_
   for (int64_t i = begin + (int64_t)rank * kHalf + thread; i < end; i += step * kAtOnce) {
     int64_t y[kAtOnce];
     L l[kAtOnce];
-    float f[kAtOnce];
+    R f[kAtOnce];
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
       const int64_t at = i + u * step;
       const bool in = at < end;
-      y[u] = in ? (target ? target[at] : ignore_index + 1) : ignore_index;
+      y[u] = in ? (target ? target[at] : ~ignore_index) : ignore_index;
       l[u] = in ? logp[at] : (L)0;
-      f[u] = in && ref ? ref[at] : 0.f;
+      f[u] = in && ref ? ref[at] : (R)0;
     }
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
@@ -1074,7 +1074,7 @@ __global__ void __launch_bounds__(kPairBwdThreads) pair_bwd_kernel(const float* 
 #pragma unroll
   for (int u = 0; u < kPairBwdTokens; ++u) {
     const int64_t i = tile + u * kPairBwdThreads + threadIdx.x;
-    y[u] = i < N && target ? target[i] : ignore_index + 1;
+    y[u] = i < N && target ? target[i] : ~ignore_index;
   }
   auto offset = [&](int64_t k) { return copied ? on_chip[k] : offsets[k]; };
   int64_t lo = 0;                          // the number of offsets <= i
@@ -1310,11 +1310,12 @@ extern "C" int b2g_policy_loss(const void* logits, int64_t ld, int logits_dtype,
   return launch_rows<__nv_bfloat16, true>(static_cast<const __nv_bfloat16*>(logits), ld, a, static_cast<__nv_bfloat16*>(grad_logits), ld_grad, rows, s);
 }
 
-extern "C" int b2g_preference_loss(const void* logp, int logp_dtype, const float* ref_logp, const int64_t* target, const int64_t* offsets, int64_t N,
+extern "C" int b2g_preference_loss(const void* logp, int logp_dtype, const void* ref_logp, int ref_dtype, const int64_t* target, const int64_t* offsets, int64_t N,
                                    int64_t pairs, int64_t ignore_index, float beta, float label_smoothing, int loss_type, int average, float* loss,
                                    float* chosen, float* rejected, float* coef, int* status, void* stream) {
   B2G_REQUIRE(N >= 0 && pairs >= 0 && pairs < (1ll << 28), "preference_loss: bad shape N=%lld pairs=%lld", (long long)N, (long long)pairs);
   B2G_REQUIRE(logp_dtype == 0 || logp_dtype == 1, "preference_loss: logp_dtype must be 0 (fp32) or 1 (fp64)");
+  B2G_REQUIRE(ref_dtype == 0 || ref_dtype == 1, "preference_loss: ref_dtype must be 0 (fp32) or 1 (fp64)");
   B2G_REQUIRE(beta > 0.f && beta <= 3.4e38f, "preference_loss: beta must be positive and finite");
   B2G_REQUIRE(label_smoothing >= 0.f && label_smoothing < 0.5f, "preference_loss: label_smoothing outside [0, 0.5)");
   B2G_REQUIRE(loss_type == 0 || loss_type == 1, "preference_loss: loss_type must be 0 (sigmoid) or 1 (squared)");
@@ -1333,12 +1334,17 @@ extern "C" int b2g_preference_loss(const void* logp, int logp_dtype, const float
   at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (logp_dtype)
-    B2G_CUDA_OK(cudaLaunchKernelEx(&cfg, policy::pair_kernel<double>, static_cast<const double*>(logp), ref_logp, target, offsets, N, pairs, ignore_index,
-                                   beta, label_smoothing, loss_type, average, loss, chosen, rejected, coef, status, cluster));
-  else
-    B2G_CUDA_OK(cudaLaunchKernelEx(&cfg, policy::pair_kernel<float>, static_cast<const float*>(logp), ref_logp, target, offsets, N, pairs, ignore_index,
-                                   beta, label_smoothing, loss_type, average, loss, chosen, rejected, coef, status, cluster));
+#define B2G_PAIRS(L, R)                                                                                                                      \
+  B2G_CUDA_OK(cudaLaunchKernelEx(&cfg, policy::pair_kernel<L, R>, static_cast<const L*>(logp), static_cast<const R*>(ref_logp), target, offsets, N, \
+                                 pairs, ignore_index, beta, label_smoothing, loss_type, average, loss, chosen, rejected, coef, status, cluster))
+  if (logp_dtype) {
+    if (ref_dtype) B2G_PAIRS(double, double);
+    else B2G_PAIRS(double, float);
+  } else {
+    if (ref_dtype) B2G_PAIRS(float, double);
+    else B2G_PAIRS(float, float);
+  }
+#undef B2G_PAIRS
   return 0;
 }
 
