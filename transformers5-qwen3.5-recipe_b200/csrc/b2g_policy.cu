@@ -780,28 +780,30 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
     Part<T> part(x0, V, begin, limit, lane);            // of the row at hand
     auto look_up = [&](int k) { return info[k % kInfo]; };
     auto wait_for = [&](int k) { return dev::mbar_wait(dev::smem_u32(&referred[k % kInfo]), (k / kInfo) & 1, &gave_up, a.status, 504); };
-    bool fine = true;
     uint32_t phase = 0u;            // bit i: parity of the next arrival in slot i
-    for (int k = 0; k < min(slots, count) && fine; ++k) {
-      fine = wait_for(k);
+    // the first rows are fetched before anybody knows whether they take part: a call of few rows is all latency
+    for (int k = 0; k < min(slots, count); ++k) {
       const T* const x = x0 + k * pitch;
       if (!steady) part = Part<T>(x, V, begin, limit, lane);
-      if (look_up(k).y >= 0 && lane == 0) part.fetch(x, begin, base + k * slot_bytes, dev::smem_u32(&arrived[k][warp]), a.V);
+      if (lane == 0) part.fetch(x, begin, base + k * slot_bytes, dev::smem_u32(&arrived[k][warp]), a.V);
       __syncwarp();
     }
     int s_slot = 0, g_slot = 0;
-    for (int k = 0; k < count + lead && fine; ++k) {
+    for (int k = 0; k < count + lead; ++k) {
       const int j = k - lead, q = (kPolicy ? j : k) + slots;      // G's row, and the row that takes the place freed in this turn
       int slot = s_slot;                                          // the place at hand
       if (k < count) {
         const int p = k % kRing;
+        if (k < slots && !wait_for(k)) break;
         const Info row = look_up(k);
-        if (row.y >= 0) {
-          if (!steady) part = Part<T>(x0 + k * pitch, V, begin, limit, lane);
-          const uint32_t place = base + s_slot * slot_bytes + lane * 16;
+        if (row.y >= 0 || k < slots) {
           if (!dev::mbar_wait(dev::smem_u32(&arrived[s_slot][warp]), phase >> s_slot & 1u, &gave_up, a.status, 506)) break;
           phase ^= 1u << s_slot;
           __syncwarp();                                 // partial vectors are lane 0's ordinary stores
+        }
+        if (row.y >= 0) {
+          if (!steady) part = Part<T>(x0 + k * pitch, V, begin, limit, lane);
+          const uint32_t place = base + s_slot * slot_bytes + lane * 16;
           const int mine = part.owns(row.y, begin, lane);
           if (mine >= 0) {                              // the target's term is the scalar warp's
             const uint32_t e = place + mine * kStep + ((row.y + part.shift) % N) * (uint32_t)sizeof(T);
@@ -870,7 +872,7 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
 
 // ---- rows of any width ----------------------------------------------------------------------------
 // One CTA per row that reads it twice (maximum, then sum) and, for the policy loss, a third time: vocabularies wider than a
-// cluster's registers hold.
+// cluster's shared memory holds.
 template <typename T, bool kPolicy>
 __global__ void __launch_bounds__(512) wide_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out) {
   constexpr int N = Vec<T>::N, kThreads = 512, kWarps = kThreads / 32;
