@@ -570,3 +570,20 @@ def test_many_rows_of_every_path_repeat_bit_for_bit(cuda):
             one = ops.policy_loss(x[r:r + 1], t[r:r + 1], adv[r:r + 1])
             assert torch.equal(one[1], want[1][r:r + 1]) or abs(float(one[1] - want[1][r])) <= 2 * ref.lse_error(vocab)
             torch.testing.assert_close(one[3].float(), want[3][r:r + 1].float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+def test_results_are_changed_in_place_like_any_tensor(cuda):
+    from b2g import autograd as ag
+
+    logp, _, target, ends = _pairs([4, 3, 2, 5], 5, dtype=torch.float32)
+    x = logp.to(cuda).requires_grad_(True)
+    plain, _, _ = ag.preference_loss(x, ends.to(cuda), target=target.to(cuda))
+    (want,) = torch.autograd.grad((plain * 3.0 * plain.detach() * 3.0).sum(), x)
+    loss, chosen, rejected = ag.preference_loss(x, ends.to(cuda), target=target.to(cuda))
+    loss.mul_(3.0)
+    y = (loss * loss.detach().clone()).sum()
+    chosen.neg_()
+    rejected.zero_()
+    (got,) = torch.autograd.grad(y, x)
+    # the same products in another order: four roundings of fp32 on either side
+    assert bool(((got - want).abs() <= 8 * 2.0 ** -24 * want.abs()).all())

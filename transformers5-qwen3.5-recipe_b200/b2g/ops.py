@@ -434,7 +434,7 @@ def policy_loss(logits: torch.Tensor, target: torch.Tensor, advantage: torch.Ten
     if kl_coef != 0.0 and ref_logp is None:
         raise ValueError("policy_loss: a KL term needs ref_logp")
     out = _cotangent_out(logits, out, "policy_loss")
-    loss, logp, kl = torch.empty(3, rows, dtype=torch.float32, device=logits.device).unbind(0)
+    loss, logp, kl = (torch.empty(rows, dtype=torch.float32, device=logits.device) for _ in range(3))
     _launch("b2g_policy_loss", logits, _a(logits), ld, int(logits.dtype == torch.float32), _a(target), _a(advantage), _a(old_logp), _a(ref_logp),
             _a(weight), float(clip_low), float(clip_high), float(kl_coef), temperature, _a(loss), _a(logp), _a(kl), _a(out),
             out.stride(0) if rows > 1 else v, rows, v, int(ignore_index), _a(status_word(logits.device)))
@@ -457,8 +457,8 @@ def preference_loss(logp: torch.Tensor, offsets: torch.Tensor, ref_logp: Optiona
                     ignore_index: int = -100):
     """Preference loss of pairs of sequences: ``(loss [pairs], chosen [pairs], rejected [pairs], coef [2 * pairs])``.
 
-    ``logp`` and ``ref_logp`` are fp32 or fp64 (sums are in fp64).  Sequence ``s`` is the tokens ``offsets[s]:offsets[s + 1]``; the chosen sequences come first, the rejected ones
-    follow in the same order.  ``L_s`` is the sum (``average``: the mean) of ``logp - ref_logp`` over the tokens whose
+    ``logp`` and ``ref_logp`` are fp32 or fp64 (sums are in fp64).  Sequence ``s`` is the tokens ``offsets[s]:offsets[s + 1]``; the
+    chosen sequences come first, the rejected ones follow in the same order.  ``L_s`` is the sum (``average``: the mean) of ``logp - ref_logp`` over the tokens whose
     ``target`` is not ``ignore_index`` (all of them without ``target``), 0 for a sequence without tokens.  ``"sigmoid"``:
     ``-(1 - label_smoothing) log sigmoid(beta gap) - label_smoothing log sigmoid(-beta gap)``, ``gap = L_chosen - L_rejected``;
     ``"squared"``: ``(gap - 1 / (2 beta))^2``.  ``chosen`` and ``rejected`` are the rewards ``beta L_s``; ``coef`` is the gradient
@@ -480,7 +480,8 @@ def preference_loss(logp: torch.Tensor, offsets: torch.Tensor, ref_logp: Optiona
         raise ValueError(f"beta must be positive and finite, got {beta}")
     if not 0.0 <= label_smoothing < 0.5 or (label_smoothing and loss_type != "sigmoid"):
         raise ValueError(f"label_smoothing must lie in [0, 0.5) and belongs to the sigmoid loss, got {label_smoothing}")
-    loss, chosen, rejected = torch.empty(3, pairs, dtype=torch.float32, device=logp.device).unbind(0)
+    # not views of one tensor: autograd refuses to have those changed in place
+    loss, chosen, rejected = (torch.empty(pairs, dtype=torch.float32, device=logp.device) for _ in range(3))
     coef = torch.empty(2 * pairs, dtype=torch.float32, device=logp.device)
     _launch("b2g_preference_loss", logp, _a(logp), int(logp.dtype == torch.float64), _a(ref_logp),
             int(ref_logp is not None and ref_logp.dtype == torch.float64), _a(target), _a(offsets), n, pairs,

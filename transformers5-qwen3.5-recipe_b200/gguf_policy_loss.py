@@ -88,7 +88,7 @@ class _PackedPolicyLoss(torch.autograd.Function):
     def forward(ctx, rows, payload, target, advantage, old_logp, ref_logp, weight, quant_type, vocab, chunk_size, settings):
         n = rows.shape[0]
         wanted = ctx.needs_input_grad[0]
-        loss, logp, kl = torch.empty(3, n, dtype=torch.float32, device=rows.device).unbind(0)
+        loss, logp, kl = (torch.empty(n, dtype=torch.float32, device=rows.device) for _ in range(3))
         grad = torch.empty_like(rows) if wanted else None
 
         def part(t, a, b):
