@@ -172,3 +172,19 @@ def test_a_post_training_step_through_router_experts_and_head(cuda):
     for a, b in zip(grads, want):
         assert dense_ref.rel_l2(a, b.cpu().double()) < 1e-2
     ops.check_status()
+
+
+def test_the_gradient_is_scaled_in_32_bits(cuda):
+    import gguf_policy_loss as gp
+
+    head, _ = _head(cuda, 1032, 2048, go.Q6_K, 5)
+    g, h, target = _case(1032, 2048, 40, 6)
+    adv = torch.randn(40, generator=g).to(cuda)
+
+    def grad(scale):
+        x = h.to(cuda).requires_grad_(True)
+        (gp.packed_policy_loss(x, head, target.to(cuda), adv)[0] * scale).backward()
+        return x.grad
+
+    third = torch.tensor(1.0 / 3.0)
+    assert torch.equal(grad(float(third)), (grad(1.0).float() * third.to(cuda)).bfloat16())

@@ -113,7 +113,7 @@ class _PackedPolicyLoss(torch.autograd.Function):
         if grad_loss is None:
             return (None,) * 11
         (grad,) = ctx.saved_tensors
-        return (grad * grad_loss.to(grad.dtype),) + (None,) * 10
+        return (grad.float().mul_(grad_loss).to(grad.dtype),) + (None,) * 10      # a bf16 factor would be off by 2^-9 everywhere
 
 
 def packed_token_logprobs(hidden_states: torch.Tensor, lm_head, target: torch.Tensor, *, temperature: float = 1.0, ignore_index: int = -100,
@@ -140,6 +140,8 @@ def packed_policy_loss(hidden_states: torch.Tensor, lm_head, target: torch.Tenso
         if t is not None and (t.shape != target.shape or t.dtype != torch.float32):
             raise ValueError(f"{name} must be fp32 with shape {tuple(target.shape)}, got {t.dtype} {tuple(t.shape)}")
         per_token.append(None if t is None else t.detach().reshape(-1).contiguous())
+    if not torch.is_grad_enabled():
+        rows = rows.detach()                  # nobody will ask for the input gradient
     settings = dict(clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef, temperature=temperature, ignore_index=ignore_index)
     loss, logp, kl = _PackedPolicyLoss.apply(rows, payload, flat, *per_token, quant_type, vocab, int(chunk_size), settings)
     return loss, logp.reshape(target.shape), kl.reshape(target.shape)
