@@ -587,3 +587,16 @@ def test_results_are_changed_in_place_like_any_tensor(cuda):
     (got,) = torch.autograd.grad(y, x)
     # the same products in another order: four roundings of fp32 on either side
     assert bool(((got - want).abs() <= 8 * 2.0 ** -24 * want.abs()).all())
+
+
+def test_tokens_that_cannot_occur(cuda):
+    """A sequence with a token of probability 0: the loss is 0 where it is the rejected one, infinite where it is the chosen one."""
+    from b2g import ops
+
+    logp = torch.tensor([-1.0, -2.0, -math.inf, -3.0, -0.5, -math.inf, -2.0, -1.0], device=cuda)
+    ends = torch.tensor([0, 2, 4, 6, 8], device=cuda)       # chosen: finite, impossible; rejected: impossible, finite
+    loss, chosen, rejected, coef = ops.preference_loss(logp, ends)
+    assert loss.tolist() == [0.0, math.inf] and rejected[0] == -math.inf and chosen[1] == -math.inf
+    grad = ops.preference_loss_bwd(torch.ones(2, device=cuda), coef, ends, 8)
+    beta = float(torch.tensor(0.1))
+    assert grad.tolist() == [0.0, 0.0, -beta, -beta, 0.0, 0.0, beta, beta]

@@ -1046,7 +1046,8 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(const L* __restrict_
       l = h * h;
       slope = 2.0 * h;
     } else {
-      l = -(1.0 - e) * log_sigmoid(u) - e * log_sigmoid(-u);
+      l = -(1.0 - e) * log_sigmoid(u);
+      if (e > 0.0) l -= e * log_sigmoid(-u);         // a rejected token that cannot occur makes it infinite; without smoothing it is no matter
       slope = b * (e / (1.0 + exp(-u)) - (1.0 - e) / (1.0 + exp(u)));
     }
     loss[p] = (float)l;
