@@ -548,8 +548,8 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const T* logits
 
 // ---- rows in a pipeline ------------------------------------------------------------------------------
 // Clusters that stay and go from row to row, two CTAs on every SM (two whose phases differ keep memory and the special-function
-// unit busier than one of twice the size: 1024 x 248320 bf16 in 218 against 233 us), each with `slots` slices of rows in shared
-// memory.  13 warps work, two more do everything that is latency.  For every row k:
+// unit busier than one of twice the size: 1024 x 248320 bf16 in 218 against 233 us).  13 warps work, two more do everything that
+// is latency.  For every row k:
 //   the first of them reads 128 samples and the target's logit, and publishes their maximum as the row's reference: a sum of
 //     exponentials needs no maximum, only a number near it, so the workers need no pass for one and their sums simply add up;
 //   S(k): the workers' sums of exp((z - reference)/tau) over everything but the target, one number per warp.  A warp whose sum
@@ -557,17 +557,24 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const T* logits
 //     coarsely there, and overflow at 128) sums once more, against its own maximum;
 //   the first warp adds them up and sends the CTA's share to the others of the cluster (asynchronous remote stores that count on
 //     their barrier); the second adds the shares, finishes the row's scalars and lets the workers know;
-//   G(k), the cotangent, `lead` rows after S(k): the workers never wait for the exchange.
-// A warp's vectors are its own: it fetches them (one bulk copy per row, issued by one lane: as 16-byte copies of every lane they
-// took the load-store unit as long as the arithmetic), reads them in S and in G, and fetches those of the row `slots` further
-// on into the same place.
-// What bounds it: two exponentials per logit at 16 per cycle and SM (126 us of the 218), then HBM (155 us); the two overlap
-// only between CTAs.  Replacing one exponential in four by a polynomial on the fp32 pipe was slower (231 us): the loops issue
-// 12 instructions per logit, and the polynomial adds six to every one that it replaces.
+//   G(k), the policy loss's cotangent, `lead` rows after S(k): the workers never wait for the exchange.
+// Policy loss: a CTA holds `slots` slices of rows.  A warp's vectors are its own: it fetches them (one bulk copy per row, issued
+// by one lane: as 16-byte copies of every lane they took the load-store unit as long as the arithmetic), reads them in S and in G,
+// and fetches those of the row `slots` further on into the same place.  One copy per CTA and row, by a warp that waits until all
+// are done with the slot, 240 against 219 us; a slice that passes twice, the second time from L2, 233 us.
+//   Bound: two exponentials per logit at 16 per cycle and SM (126 us of the 218), then HBM (155 us); the two overlap only between
+//   CTAs.  Replacing one exponential in four by a polynomial on the fp32 pipe was slower (231 us): the loops issue 12 instructions
+//   per logit, and the polynomial adds six to every one that it replaces.
+// Log-probabilities: nothing is wanted twice, so a slice passes through the slots in chunks of kTurns vectors a lane, which a warp
+// of its own copies, 52 KB at a time (a bulk copy costs some 40 ns beside its bytes: with 4 KB copies by every warp 105 us in
+// place of 97, 1024 x 248320 bf16 with a tenth of the rows left out).
+//   Bound: HBM (70 us; the same kernel without its arithmetic takes 6 us less).
 // All waits are bounded; a CTA whose wait ran out stops working, and all CTAs of a cluster leave together.
-constexpr int kWorkerWarps = 13, kWorkers = kWorkerWarps * 32, kRing = 8, kMaxCluster = 10, kMaxSlots = 2, kMaxLead = 3, kAhead = 7, kInfo = 16, kSamples = 4;
+constexpr int kWorkerWarps = 13, kWorkers = kWorkerWarps * 32, kRing = 8, kMaxCluster = 10, kMaxLead = 3, kAhead = 7, kInfo = 16, kSamples = 4;
+constexpr int kMaxSlots = 2;                                             // policy loss
+constexpr int kStages = 2, kTurns = 8, kChunk = kWorkers * kTurns;       // log-probabilities
 
-struct Share { float m, unused; double d; };       // what a CTA sends: its sum and what it is against
+struct Share { float m, unused; double d; };       // what a CTA sends: its sum and what it is against (16 bytes: one store)
 
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int where) {
   for (uint32_t spin = 0; spin < B2G_SPIN_LIMIT; ++spin) {
@@ -618,13 +625,13 @@ struct Part {
   // One lane: the whole vectors as one bulk copy that counts on `bar`, the partial ones by hand.  `at`: place of vector `begin`.
   __device__ __forceinline__ void fetch(const T* x, int begin, uint32_t at, uint32_t bar, int64_t V) const {
     const int whole = max(0, full_end - full_begin);
+    for (int v = begin; v < min(full_begin, end); ++v) fetch_edge(x, V, v, at + (v - begin) * 16);
+    for (int v = max(full_end, full_begin); v < end; ++v) fetch_edge(x, V, v, at + (v - begin) * 16);
     dev::mbar_arrive_expect_tx(bar, (uint32_t)whole * 16);
     if (whole)
       asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at + (full_begin - begin) * 16),
                    "l"(x - shift + (int64_t)full_begin * N), "r"(whole * 16), "r"(bar)
                    : "memory");
-    for (int v = begin; v < min(full_begin, end); ++v) fetch_edge(x, V, v, at + (v - begin) * 16);
-    for (int v = max(full_end, full_begin); v < end; ++v) fetch_edge(x, V, v, at + (v - begin) * 16);
   }
   // index i of this lane's vector that holds column y, or -1
   __device__ __forceinline__ int owns(int y, int begin, int lane) const {
@@ -637,10 +644,9 @@ struct Part {
 struct Info { float reference; int y; };
 
 constexpr double kFarAbove = 16384.0;      // 2^14
-// A warp's sum over its vectors in shared memory, n of this lane's 512 bytes apart.
-template <typename T>
-__device__ __forceinline__ double warp_sum_against(uint32_t place, int n, float ref, const Scale& c) {
-  constexpr int kStep = 32 * 16;
+// A lane's sum over its n vectors in shared memory, kStep bytes apart, and the warp's.
+template <typename T, int kStep>
+__device__ __forceinline__ double lane_sum_against(uint32_t place, int n, float ref, const Scale& c) {
   const F2 minus_ref = f2(-ref, -ref);
   F2 d = f2(0.f, 0.f);
   int i = 0;
@@ -650,27 +656,55 @@ __device__ __forceinline__ double warp_sum_against(uint32_t place, int n, float 
   if (i < n) d = d + exp_sum(from_shared<T>(place + i * kStep), minus_ref, c);
   float lo, hi;
   split(d, lo, hi);
-  double all = (double)lo + (double)hi;
+  return (double)lo + (double)hi;
+}
+__device__ __forceinline__ double warp_total(double d) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-  return all;
+  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  return d;
+}
+template <typename T, int kStep>
+__device__ __forceinline__ double warp_sum_against(uint32_t place, int n, float ref, const Scale& c) {
+  return warp_total(lane_sum_against<T, kStep>(place, n, ref, c));
 }
 // The same against its own maximum; out of line, it is rare.
-template <typename T>
+template <typename T, int kStep>
 __device__ __noinline__ Stat warp_sum_far(uint32_t place, int n, Scale c) {
   float m = kLowest;
-  for (int i = 0; i < n; ++i) m = vec_max(from_shared<T>(place + i * 512), m);
+  for (int i = 0; i < n; ++i) m = vec_max(from_shared<T>(place + i * kStep), m);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return Stat{m, warp_sum_against<T>(place, n, m, c)};
+  return Stat{m, warp_sum_against<T, kStep>(place, n, m, c)};
 }
 
+__device__ __forceinline__ Stat join_two(Stat a, Stat b, double inv_tau) {
+  const float m = fmaxf(a.m, b.m);
+  if (a.d != 0.0 && a.m != m) a.d *= exp(((double)a.m - (double)m) * inv_tau);
+  if (b.d != 0.0 && b.m != m) b.d *= exp(((double)b.m - (double)m) * inv_tau);
+  return Stat{m, a.d + b.d};
+}
+// -inf in place of value j of the vector at `at`
+template <typename T>
+__device__ __forceinline__ void hide(uint32_t at, int j) {
+  if (sizeof(T) == 2) asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + j * 2), "h"((unsigned short)0xFF80) : "memory");
+  else asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + j * 4), "r"(0xFF800000u) : "memory");
+}
+// A wait has run out: the copies that are still on their way have nowhere to go once the CTA has left.
+__device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
+  for (uint32_t spin = 0; spin < (1u << 16) && !dev::mbar_try_wait(bar, parity); ++spin) {}
+}
+
+template <bool kPolicy>
+constexpr int kPipeThreads = kWorkers + (kPolicy ? 64 : 96);      // two CTAs of either have the 64 registers a thread that an SM holds for them
+
 template <typename T, bool kPolicy>
-__global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out, int64_t rows,
+__global__ void __launch_bounds__(kPipeThreads<kPolicy>, 2) pipe_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out, int64_t rows,
                                                                 int cluster, int slots, int lead, int per, int per_warp) {
   constexpr int N = Vec<T>::N, kStep = 32 * 16;
   extern __shared__ __align__(16) uint8_t space[];
-  __shared__ uint64_t arrived[kMaxSlots][kWorkerWarps];      // one per slot and warp: a warp's copies are its own
+  // policy loss: one per slot and warp, whose copies are its own; log-probabilities: one per slot, and every warp is done with it
+  constexpr int kPlaces = kPolicy ? kMaxSlots : kStages, kOwners = kPolicy ? kWorkerWarps : 1;
+  __shared__ uint64_t arrived[kPlaces][kOwners], emptied[kPlaces];
   __shared__ __align__(16) Share share[kRing][kMaxCluster];
   __shared__ Stat sums[kRing][kWorkerWarps];
   __shared__ __align__(8) Info info[kInfo];
@@ -684,7 +718,8 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
   if (threadIdx.x == 0) {
     gave_up = 0;
     for (int i = 0; i < kInfo; ++i) dev::mbar_init(dev::smem_u32(&referred[i]), 1);
-    for (int i = 0; i < kMaxSlots * kWorkerWarps; ++i) dev::mbar_init(dev::smem_u32(&arrived[0][i]), 1);
+    for (int i = 0; i < kPlaces * kOwners; ++i) dev::mbar_init(dev::smem_u32(&arrived[i / kOwners][i % kOwners]), 1);
+    for (int i = 0; i < kPlaces; ++i) dev::mbar_init(dev::smem_u32(&emptied[i]), kWorkerWarps);
     for (int i = 0; i < kRing; ++i) {
       dev::mbar_init(dev::smem_u32(&summed[i]), kWorkerWarps);
       dev::mbar_init(dev::smem_u32(&joined[i]), 1);
@@ -770,6 +805,80 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
       __syncwarp();
       if (lane == 0) dev::mbar_arrive(dev::smem_u32(&ready[p]));
     }
+  } else if (!kPolicy && warp == kWorkerWarps + 2) {       // the copies
+    const int begin = rank * per, limit = begin + per, chunks = (per + kChunk - 1) / kChunk;
+    const T* x = logits + first * ld;
+    uint32_t turn = 0u, slot = 0u;             // times round the slots, and slots filled in this one
+    bool fine = true;
+    for (int k = 0; k < count && fine; ++k, x += stride * ld) {
+      // the first chunks are fetched before anybody knows whether their rows take part: a call of few rows is all latency
+      bool live = true;
+      if (turn) {
+        fine = dev::mbar_wait(dev::smem_u32(&referred[k % kInfo]), (k / kInfo) & 1, &gave_up, a.status, 504);
+        live = fine && info[k % kInfo].y >= 0;
+      }
+      for (int i = 0; i < chunks && fine; ++i) {
+        if (turn) fine = dev::mbar_wait(dev::smem_u32(&emptied[slot]), (turn - 1u) & 1u, &gave_up, a.status, 505);
+        if (!fine) break;
+        if (lane == 0) {
+          const uint32_t bar = dev::smem_u32(&arrived[slot][0]);
+          const int from = begin + i * kChunk;
+          dev::fence_proxy_async_smem();       // of partial vectors that stood in the slot
+          if (live) Part<T>(x, (uint32_t)a.V, from, min(limit, from + kChunk), 0).fetch(x, from, dev::smem_u32(space) + slot * (kChunk * 16), bar, a.V);
+          else dev::mbar_arrive(bar);
+        }
+        __syncwarp();
+        if (++slot == kStages) { slot = 0u; ++turn; }
+      }
+    }
+    if (gave_up)
+      for (uint32_t i = 0; i < kStages; ++i)       // the last time round that filled slot i
+        if (turn || i < slot) drain(dev::smem_u32(&arrived[i][0]), (i < slot ? turn : turn - 1u) & 1u);
+  } else if constexpr (!kPolicy) {
+    constexpr int kTurn = kWorkers * 16;
+    const int begin = rank * per, limit = begin + per, mine = warp * 32 + lane;      // every kWorkers-th vector of a chunk from `mine` on
+    const uint32_t base = dev::smem_u32(space) + mine * 16;
+    const Scale c = a.c;
+    const T* x = logits + first * ld;
+    uint32_t slot = 0u, parity = 0u;
+    bool fine = true;
+    for (int k = 0; k < count && fine; ++k, x += stride * ld) {
+      fine = dev::mbar_wait(dev::smem_u32(&referred[k % kInfo]), (k / kInfo) & 1, &gave_up, a.status, 504);
+      if (!fine) break;
+      const Info row = info[k % kInfo];
+      const Part<T> part(x, (uint32_t)a.V, begin, limit, 0);
+      const int owner = row.y >= 0 ? (int)((uint32_t)(row.y + part.shift) / N) : -1;      // the vector that holds the target
+      double d = 0.0;
+      Stat far{kLowest, 0.0};
+      for (int from = begin; from < limit; from += kChunk) {
+        fine = dev::mbar_wait(dev::smem_u32(&arrived[slot][0]), parity, &gave_up, a.status, 506);
+        if (!fine) break;
+        if (row.y >= 0) {
+          const uint32_t place = base + slot * (kChunk * 16);
+          const int at = owner - from - mine;           // the target's term is the scalar warp's
+          if (at >= 0 && at < kChunk && at % kWorkers == 0 && owner < limit) hide<T>(place + at * 16, (row.y + part.shift) % N);
+          const int left = part.end - from - mine, n = left > 0 ? min(kTurns, (left - 1) / kWorkers + 1) : 0;
+          const double one = lane_sum_against<T, kTurn>(place, n, row.reference, c);
+          if (__any_sync(0xffffffffu, !(one < kFarAbove))) far = join_two(far, warp_sum_far<T, kTurn>(place, n, c), a.inv_tau);
+          else d += one;
+          dev::fence_proxy_async_smem();                // the next copy into the slot comes after what has been done in it
+        }
+        __syncwarp();
+        if (lane == 0) dev::mbar_arrive(dev::smem_u32(&emptied[slot]));
+        if (++slot == kStages) { slot = 0u; parity ^= 1u; }
+      }
+      if (!fine) break;
+      if (row.y >= 0) {
+        Stat sum{row.reference, warp_total(d)};
+        if (far.d != 0.0) sum = join_two(sum, far, a.inv_tau);
+        if (lane == 0) sums[k % kRing][warp] = sum;
+      }
+      __syncwarp();
+      if (lane == 0) dev::mbar_arrive(dev::smem_u32(&summed[k % kRing]));
+      // the rings bound how far the workers run ahead
+      const int j = k - kMaxLead;
+      if (j >= 0) fine = dev::mbar_wait(dev::smem_u32(&ready[j % kRing]), (j / kRing) & 1, &gave_up, a.status, 503);
+    }
   } else {
     const int begin = rank * per + warp * per_warp, limit = min((rank + 1) * per, begin + per_warp), slot_bytes = per * 16;
     const uint32_t base = dev::smem_u32(space) + warp * per_warp * 16, V = (uint32_t)a.V;
@@ -790,8 +899,8 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
     }
     int s_slot = 0, g_slot = 0;
     for (int k = 0; k < count + lead; ++k) {
-      const int j = k - lead, q = (kPolicy ? j : k) + slots;      // G's row, and the row that takes the place freed in this turn
-      int slot = s_slot;                                          // the place at hand
+      const int j = k - lead, q = j + slots;      // G's row, and the row that takes the place freed in this turn
+      int slot = s_slot;                          // the place at hand
       if (k < count) {
         const int p = k % kRing;
         if (k < slots && !wait_for(k)) break;
@@ -805,13 +914,9 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
           if (!steady) part = Part<T>(x0 + k * pitch, V, begin, limit, lane);
           const uint32_t place = base + s_slot * slot_bytes + lane * 16;
           const int mine = part.owns(row.y, begin, lane);
-          if (mine >= 0) {                              // the target's term is the scalar warp's
-            const uint32_t e = place + mine * kStep + ((row.y + part.shift) % N) * (uint32_t)sizeof(T);
-            if (sizeof(T) == 2) asm volatile("st.shared.u16 [%0], %1;" ::"r"(e), "h"((unsigned short)0xFF80) : "memory");
-            else asm volatile("st.shared.u32 [%0], %1;" ::"r"(e), "r"(0xFF800000u) : "memory");
-          }
-          Stat mine_sum{row.reference, warp_sum_against<T>(place, part.n, row.reference, c)};
-          if (!(mine_sum.d < kFarAbove)) mine_sum = warp_sum_far<T>(place, part.n, c);
+          if (mine >= 0) hide<T>(place + mine * kStep, (row.y + part.shift) % N);      // the target's term is the scalar warp's
+          Stat mine_sum{row.reference, warp_sum_against<T, kStep>(place, part.n, row.reference, c)};
+          if (!(mine_sum.d < kFarAbove)) mine_sum = warp_sum_far<T, kStep>(place, part.n, c);
           if (lane == 0) sums[p][warp] = mine_sum;
         }
         __syncwarp();
@@ -827,28 +932,26 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
       if (j >= 0) {
         const int p = j % kRing;
         if (!dev::mbar_wait(dev::smem_u32(&ready[p]), (j / kRing) & 1, &gave_up, a.status, 503)) break;
-        if (kPolicy) {
-          slot = g_slot;
-          const int y = look_up(j).y;
-          const float4 b = y >= 0 ? bcast[p] : make_float4(0.f, 0.f, 0.f, 0.f);
-          const T* const x = x0 + j * pitch;
-          T* const o = out + (first + j * stride) * ld_out;
-          if (!steady) part = Part<T>(x, V, begin, limit, lane);
-          const uint32_t place = base + g_slot * slot_bytes + lane * 16;
-          T* const to = o - part.shift;
-          const bool wide = same_alignment(x, (const T*)o);
-          auto put = [&](int v, const Vec<T>& w) {
-            if (wide && part.full(v)) __stcs(reinterpret_cast<uint4*>(to + (int64_t)v * N), make_uint4(w.w[0], w.w[1], w.w[2], w.w[3]));
-            else store_edge(x, a.V, v, o, w);
-          };
-          if (b.x == 0.f) {                     // a clipped token, a row that takes no part: nothing of the logits is wanted
-            for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, zeros<T>());
-          } else {
-            const F2 factor = f2(b.y, b.y), minus_ref = f2(-b.z, -b.z);
+        slot = g_slot;
+        const int y = look_up(j).y;
+        const float4 b = y >= 0 ? bcast[p] : make_float4(0.f, 0.f, 0.f, 0.f);
+        const T* const x = x0 + j * pitch;
+        T* const o = out + (first + j * stride) * ld_out;
+        if (!steady) part = Part<T>(x, V, begin, limit, lane);
+        const uint32_t place = base + g_slot * slot_bytes + lane * 16;
+        T* const to = o - part.shift;
+        const bool wide = same_alignment(x, (const T*)o);
+        auto put = [&](int v, const Vec<T>& w) {
+          if (wide && part.full(v)) __stcs(reinterpret_cast<uint4*>(to + (int64_t)v * N), make_uint4(w.w[0], w.w[1], w.w[2], w.w[3]));
+          else store_edge(x, a.V, v, o, w);
+        };
+        if (b.x == 0.f) {                     // a clipped token, a row that takes no part: nothing of the logits is wanted
+          for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, zeros<T>());
+        } else {
+          const F2 factor = f2(b.y, b.y), minus_ref = f2(-b.z, -b.z);
 #pragma unroll 2
-            for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled_exp(from_shared<T>(place + i * kStep), minus_ref, factor, c));
-            if (part.owns(y, begin, lane) >= 0) o[y] = from_float<T>(b.w);              // its writer puts the target's entry right
-          }
+          for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled_exp(from_shared<T>(place + i * kStep), minus_ref, factor, c));
+          if (part.owns(y, begin, lane) >= 0) o[y] = from_float<T>(b.w);              // its writer puts the target's entry right
         }
         if (++g_slot == slots) g_slot = 0;
       }
@@ -861,19 +964,16 @@ __global__ void __launch_bounds__(kWorkers + 64, 2) pipe_kernel(const T* logits,
         __syncwarp();
       }
     }
-    // the copies that are still on their way when a wait ran out have nowhere to go once the CTA has left
-    if (gave_up) {
-      for (int i = 0; i < slots; ++i)
-        for (uint32_t spin = 0; spin < (1u << 16) && !dev::mbar_try_wait(dev::smem_u32(&arrived[i][warp]), phase >> i & 1u); ++spin) {}
-    }
+    if (gave_up)
+      for (int i = 0; i < slots; ++i) drain(dev::smem_u32(&arrived[i][warp]), phase >> i & 1u);
   }
   dev::cluster_sync_all();          // no CTA's memory goes before what was sent to it has come
 }
 
 // ---- rows of any width ----------------------------------------------------------------------------
-// One CTA per row that reads it twice (maximum, then sum) and, for the policy loss, a third time: vocabularies wider than a
-// cluster's shared memory holds.
-template <typename T, bool kPolicy>
+// Policy loss: one CTA per row that reads it three times (maximum, sum, cotangent), vocabularies wider than a cluster's shared
+// memory holds.
+template <typename T>
 __global__ void __launch_bounds__(512) wide_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out) {
   constexpr int N = Vec<T>::N, kThreads = 512, kWarps = kThreads / 32;
   __shared__ Stat warp_stat[kWarps];
@@ -881,18 +981,12 @@ __global__ void __launch_bounds__(512) wide_kernel(const T* logits, int64_t ld, 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t r = blockIdx.x, y = a.target[r];
   const Row<T> row(logits + r * ld, a.V);
-  T* const o = kPolicy ? out + r * ld_out : nullptr;
-  const bool wide = kPolicy && same_alignment(row.x, (const T*)o);
-  bool live = target_ok(y, a, threadIdx.x == 0);
-  Given in{1.f, 0.f, 0.f, 0.f};
-  if (kPolicy) {
-    in = given(a, r);
-    live = live && in.weight != 0.f;
-  }
-  if (!live) {
-    if (threadIdx.x == 0) conclude_nothing<kPolicy>(a, r);
-    if (kPolicy)
-      for (int v = threadIdx.x; v < row.nvec; v += kThreads) row.store(o, v, zeros<T>(), wide);
+  T* const o = out + r * ld_out;
+  const bool wide = same_alignment(row.x, (const T*)o);
+  const Given in = given(a, r);
+  if (!target_ok(y, a, threadIdx.x == 0) || in.weight == 0.f) {
+    if (threadIdx.x == 0) conclude_nothing<true>(a, r);
+    for (int v = threadIdx.x; v < row.nvec; v += kThreads) row.store(o, v, zeros<T>(), wide);
     return;
   }
   float m = kLowest;
@@ -914,9 +1008,8 @@ __global__ void __launch_bounds__(512) wide_kernel(const T* logits, int64_t ld, 
   __syncthreads();
   if (warp == 0) {
     const Stat t = join_lanes<kWarps>(lane < kWarps ? warp_stat[lane] : Stat{kLowest, 0.0}, a.inv_tau);
-    if (lane == 0) bcast = conclude<T, kPolicy>(a, t, zy, in, r, true);
+    if (lane == 0) bcast = conclude<T, true>(a, t, zy, in, r, true);
   }
-  if (!kPolicy) return;
   __syncthreads();
   const float4 b = bcast;
   const F2 factor = f2(b.y, b.y), minus_m = f2(-b.z, -b.z);
@@ -1136,17 +1229,19 @@ static policy::RowArgs row_args(const int64_t* target, int64_t V, int64_t ignore
 //     186 and 189).
 //   Else pipe_kernel with the cluster size whose clusters have the fewest bytes to go through one after the other,
 //     rounds * (slice + kRoundBytes),  rounds = rows / clusters that the device holds at once (of 296 places 8-CTA clusters fill
-//     264, 9-CTA clusters 270, 5-CTA clusters 280: the GPCs have 16 to 20 SMs), among those whose slices leave room for two
-//     slots.  kRoundBytes stands for what a row costs however short its slices are.
-//   Rows too wide for that: one slot; beyond it wide_kernel.
+//     264, 9-CTA clusters 270, 5-CTA clusters 280: the GPCs have 16 to 20 SMs), for the policy loss among those whose slices
+//     leave room for two slots.  kRoundBytes stands for what a row costs however short its slices are.
+//   Policy loss of rows too wide for that: one slot; beyond it wide_kernel.
 // Two CTAs share an SM's 228 KB: 1 KB each is the system's, and pipe_kernel's own arrays may take 5 KB beside the slices.
 constexpr int64_t kSmallRow = 36 * 1024, kSliceLimit = 108 * 1024, kRoundBytes = 8 * 1024;
+constexpr int64_t kStreamBytes = policy::kStages * policy::kChunk * 16;
+static_assert(kStreamBytes <= kSliceLimit, "two CTAs share an SM");
 
 template <typename T, bool kPolicy>
 static cudaLaunchConfig_t pipe_config(int cluster, int64_t bytes, cudaLaunchAttribute* at) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cluster);
-  cfg.blockDim = dim3(policy::kWorkers + 64);
+  cfg.blockDim = dim3(policy::kPipeThreads<kPolicy>);
   cfg.dynamicSmemBytes = (size_t)bytes;
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
@@ -1188,7 +1283,7 @@ static int launch_pipe(const T* logits, int64_t ld, const policy::RowArgs& a, T*
     int64_t best_cost = 0;
     for (int c = 1; c <= policy::kMaxCluster; ++c) {
       const int64_t slice = (need + c - 1) / c * 16;
-      if (slice * slots > kSliceLimit) continue;
+      if (kPolicy && slice * slots > kSliceLimit) continue;
       int resident = 0;
       if (int rc = resident_clusters<T, kPolicy>(c, &resident)) return rc;
       if (resident == 0) continue;
@@ -1199,13 +1294,12 @@ static int launch_pipe(const T* logits, int64_t ld, const policy::RowArgs& a, T*
   *taken = best != 0;
   if (best == 0) return 0;
   const int64_t slice = (need + best - 1) / best * 16;
-  const int slots = kSliceLimit / slice < policy::kMaxSlots ? 1 : policy::kMaxSlots;
-  // G trails S by a row where there is a second slot to wait in; without G only the rings bound how far the workers run ahead
-  const int lead = kPolicy ? slots - 1 : policy::kMaxLead;
+  const int slots = !kPolicy || kSliceLimit / slice < policy::kMaxSlots ? 1 : policy::kMaxSlots;
+  const int lead = slots - 1;      // G trails S by a row where there is a second slot to wait in
   // whole turns of 32 vectors per warp; the last warps may have none
   const int per_warp = (int)((slice / 16 + policy::kWorkers - 1) / policy::kWorkers) * 32;
   cudaLaunchAttribute at[1];
-  cudaLaunchConfig_t cfg = pipe_config<T, kPolicy>(best, slice * slots, at);
+  cudaLaunchConfig_t cfg = pipe_config<T, kPolicy>(best, kPolicy ? slice * slots : kStreamBytes, at);
   cfg.gridDim = dim3((unsigned)((rows < best_resident ? rows : best_resident) * best));
   cfg.stream = s;
   B2G_CUDA_OK(cudaLaunchKernelEx(&cfg, policy::pipe_kernel<T, kPolicy>, logits, ld, a, out, ld_out, rows, best, slots, lead, (int)(slice / 16), per_warp));
@@ -1239,8 +1333,12 @@ static int launch_rows(const T* logits, int64_t ld, const policy::RowArgs& a, T*
   bool taken = false;
   if (int rc = launch_pipe<T, kPolicy>(logits, ld, a, out, ld_out, rows, s, &taken)) return rc;
   if (!taken) {
-    policy::wide_kernel<T, kPolicy><<<(unsigned)rows, 512, 0, s>>>(logits, ld, a, out, ld_out);
-    B2G_CUDA_OK(cudaGetLastError());
+    if constexpr (kPolicy) {
+      policy::wide_kernel<T><<<(unsigned)rows, 512, 0, s>>>(logits, ld, a, out, ld_out);
+      B2G_CUDA_OK(cudaGetLastError());
+    } else {
+      B2G_REQUIRE(taken, "the device has no room for a CTA of %d threads", policy::kPipeThreads<kPolicy>);
+    }
   }
   return 0;
 }
