@@ -1230,10 +1230,11 @@ static policy::RowArgs row_args(const int64_t* target, int64_t V, int64_t ignore
 //   Else pipe_kernel with the cluster size whose clusters have the fewest bytes to go through one after the other,
 //     rounds * (slice + kRoundBytes),  rounds = rows / clusters that the device holds at once (of 296 places 8-CTA clusters fill
 //     264, 9-CTA clusters 270, 5-CTA clusters 280: the GPCs have 16 to 20 SMs), for the policy loss among those whose slices
-//     leave room for two slots.  kRoundBytes stands for what a row costs however short its slices are.
+//     leave room for two slots.  kRoundBytes stands for what a row costs however short its slices are (12 KB against 8: policy
+//     loss of 301 x 32003 fp32 21.0 and 23.3 us, of 301 x 32003 bf16 14.6 and 17.9, of 150 x 64000 bf16 13.6 and 14.8).
 //   Policy loss of rows too wide for that: one slot; beyond it wide_kernel.
 // Two CTAs share an SM's 228 KB: 1 KB each is the system's, and pipe_kernel's own arrays may take 5 KB beside the slices.
-constexpr int64_t kSmallRow = 36 * 1024, kSliceLimit = 108 * 1024, kRoundBytes = 8 * 1024;
+constexpr int64_t kSmallRow = 36 * 1024, kSliceLimit = 108 * 1024, kRoundBytes = 12 * 1024;
 constexpr int64_t kStreamBytes = policy::kStages * policy::kChunk * 16;
 static_assert(kStreamBytes <= kSliceLimit, "two CTAs share an SM");
 
