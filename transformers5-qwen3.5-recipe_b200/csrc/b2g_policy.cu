@@ -149,6 +149,19 @@ __device__ __forceinline__ Vec<T> scaled_exp(const Vec<T>& x, F2 minus_m, F2 fac
   return r;
 }
 
+template <typename T>
+__device__ __forceinline__ Vec<T> scaled(const Vec<T>& e, F2 factor) {
+  Vec<T> r;
+#pragma unroll
+  for (int i = 0; i < Vec<T>::N / 2; ++i) {
+    float lo, hi;
+    split(e.pair(i) * factor, lo, hi);
+    r.w[2 * i] = __float_as_uint(lo);
+    r.w[2 * i + 1] = __float_as_uint(hi);
+  }
+  return r;
+}
+
 // A row as 16-byte vectors of the memory it lies in: vector v holds the columns [v * N - shift, (v + 1) * N - shift), so the
 // inner vectors are aligned whatever the row's own alignment is, and at most the first and the last one are partial.
 template <typename T>
@@ -565,6 +578,8 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const T* logits
 //   Bound: two exponentials per logit at 16 per cycle and SM (126 us of the 218), then HBM (155 us); the two overlap only between
 //   CTAs.  Replacing one exponential in four by a polynomial on the fp32 pipe was slower (231 us): the loops issue 12 instructions
 //   per logit, and the polynomial adds six to every one that it replaces.
+//   fp32 logits: an exponential has as many bits as its logit, takes its place in S, and G only scales it (2000 x 16000: 62 against
+//   68 us).  A bf16 logit's place is too small for it: a cotangent that is rounded twice is not what the type can hold.
 // Log-probabilities: nothing is wanted twice, so a slice passes through the slots in chunks of kTurns vectors a lane, which a warp
 // of its own copies, 52 KB at a time (a bulk copy costs some 40 ns beside its bytes: with 4 KB copies by every warp 105 us in
 // place of 97, 1024 x 248320 bf16 with a tenth of the rows left out).
@@ -644,9 +659,27 @@ struct Part {
 struct Info { float reference; int y; };
 
 constexpr double kFarAbove = 16384.0;      // 2^14
-// A lane's sum over its n vectors in shared memory, kStep bytes apart, and the warp's.
-template <typename T, int kStep>
+// A lane's sum over its n vectors in shared memory, kStep bytes apart, and the warp's.  kKeep: 32-bit exponentials take the places
+// of their logits.
+template <typename T, int kStep, bool kKeep = false>
 __device__ __forceinline__ double lane_sum_against(uint32_t place, int n, float ref, const Scale& c) {
+  if constexpr (kKeep) {
+    static_assert(sizeof(T) == 4, "an exponential needs as many bits as its logit has");
+    F2 sum = f2(0.f, 0.f);
+    float lo, hi;
+#pragma unroll 2
+    for (int i = 0; i < n; ++i) {
+      const Vec<T> x = from_shared<T>(place + i * kStep);
+      const F2 m = f2(-ref, -ref), e = exp_from<T, true>(x.pair(0), m, c), f = exp_from<T, true>(x.pair(1), m, c);
+      sum = sum + (e + f);
+      float w[4];
+      split(e, w[0], w[1]);
+      split(f, w[2], w[3]);
+      dev::sts128(place + i * kStep, __float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3]));
+    }
+    split(sum, lo, hi);
+    return (double)lo + (double)hi;
+  }
   const F2 minus_ref = f2(-ref, -ref);
   F2 d = f2(0.f, 0.f);
   int i = 0;
@@ -663,18 +696,27 @@ __device__ __forceinline__ double warp_total(double d) {
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   return d;
 }
-template <typename T, int kStep>
+template <typename T, int kStep, bool kKeep = false>
 __device__ __forceinline__ double warp_sum_against(uint32_t place, int n, float ref, const Scale& c) {
-  return warp_total(lane_sum_against<T, kStep>(place, n, ref, c));
+  return warp_total(lane_sum_against<T, kStep, kKeep>(place, n, ref, c));
 }
 // The same against its own maximum; out of line, it is rare.
-template <typename T, int kStep>
+template <typename T, int kStep, bool kKeep = false>
 __device__ __noinline__ Stat warp_sum_far(uint32_t place, int n, Scale c) {
   float m = kLowest;
   for (int i = 0; i < n; ++i) m = vec_max(from_shared<T>(place + i * kStep), m);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return Stat{m, warp_sum_against<T, kStep>(place, n, m, c)};
+  return Stat{m, warp_sum_against<T, kStep, kKeep>(place, n, m, c)};
+}
+// Logits that their exponentials have replaced, from memory once more: vectors v, v + 32, ... of a row.
+template <typename T, int kStep>
+__device__ __noinline__ void fetch_again(const T* x, int64_t V, int v, uint32_t place, int n) {
+  const Row<T> row(x, V);
+  for (int i = 0; i < n; ++i) {
+    const Vec<T> w = row.load(v + i * 32);
+    dev::sts128(place + i * kStep, w.w[0], w.w[1], w.w[2], w.w[3]);
+  }
 }
 
 __device__ __forceinline__ Stat join_two(Stat a, Stat b, double inv_tau) {
@@ -701,6 +743,7 @@ template <typename T, bool kPolicy>
 __global__ void __launch_bounds__(kPipeThreads<kPolicy>, 2) pipe_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out, int64_t rows,
                                                                 int cluster, int slots, int lead, int per, int per_warp) {
   constexpr int N = Vec<T>::N, kStep = 32 * 16;
+  constexpr bool kKeep = kPolicy && sizeof(T) == 4;      // G finds the exponentials of S in the logits' places
   extern __shared__ __align__(16) uint8_t space[];
   // policy loss: one per slot and warp, whose copies are its own; log-probabilities: one per slot, and every warp is done with it
   constexpr int kPlaces = kPolicy ? kMaxSlots : kStages, kOwners = kPolicy ? kWorkerWarps : 1;
@@ -890,6 +933,7 @@ __global__ void __launch_bounds__(kPipeThreads<kPolicy>, 2) pipe_kernel(const T*
     auto look_up = [&](int k) { return info[k % kInfo]; };
     auto wait_for = [&](int k) { return dev::mbar_wait(dev::smem_u32(&referred[k % kInfo]), (k / kInfo) & 1, &gave_up, a.status, 504); };
     uint32_t phase = 0u;            // bit i: parity of the next arrival in slot i
+    float against[kMaxSlots] = {0.f, 0.f};       // what this warp's exponentials in a slot were taken against
     // the first rows are fetched before anybody knows whether they take part: a call of few rows is all latency
     for (int k = 0; k < min(slots, count); ++k) {
       const T* const x = x0 + k * pitch;
@@ -914,10 +958,19 @@ __global__ void __launch_bounds__(kPipeThreads<kPolicy>, 2) pipe_kernel(const T*
           if (!steady) part = Part<T>(x0 + k * pitch, V, begin, limit, lane);
           const uint32_t place = base + s_slot * slot_bytes + lane * 16;
           const int mine = part.owns(row.y, begin, lane);
-          if (mine >= 0) hide<T>(place + mine * kStep, (row.y + part.shift) % N);      // the target's term is the scalar warp's
-          Stat mine_sum{row.reference, warp_sum_against<T, kStep>(place, part.n, row.reference, c)};
-          if (!(mine_sum.d < kFarAbove)) mine_sum = warp_sum_far<T, kStep>(place, part.n, c);
+          auto hide_mine = [&] { if (mine >= 0) hide<T>(place + mine * kStep, (row.y + part.shift) % N); };
+          hide_mine();                                  // the target's term is the scalar warp's
+          Stat mine_sum{row.reference, warp_sum_against<T, kStep, kKeep>(place, part.n, row.reference, c)};
+          if (!(mine_sum.d < kFarAbove)) {
+            if (kKeep) {
+              fetch_again<T, kStep>(x0 + k * pitch, a.V, begin + lane, place, part.n);
+              hide_mine();
+            }
+            mine_sum = warp_sum_far<T, kStep, kKeep>(place, part.n, c);
+          }
           if (lane == 0) sums[p][warp] = mine_sum;
+          if (s_slot == 0) against[0] = mine_sum.m;
+          else against[1] = mine_sum.m;
         }
         __syncwarp();
         if (lane == 0) dev::mbar_arrive(dev::smem_u32(&summed[p]));
@@ -948,9 +1001,16 @@ __global__ void __launch_bounds__(kPipeThreads<kPolicy>, 2) pipe_kernel(const T*
         if (b.x == 0.f) {                     // a clipped token, a row that takes no part: nothing of the logits is wanted
           for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, zeros<T>());
         } else {
-          const F2 factor = f2(b.y, b.y), minus_ref = f2(-b.z, -b.z);
+          if constexpr (kKeep) {
+            const float own = g_slot == 0 ? against[0] : against[1], f = own == b.z ? b.y : b.y * (float)exp(((double)own - (double)b.z) * a.inv_tau);
+            const F2 factor = f2(f, f);
 #pragma unroll 2
-          for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled_exp(from_shared<T>(place + i * kStep), minus_ref, factor, c));
+            for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled(from_shared<T>(place + i * kStep), factor));
+          } else {
+            const F2 factor = f2(b.y, b.y), minus_ref = f2(-b.z, -b.z);
+#pragma unroll 2
+            for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled_exp(from_shared<T>(place + i * kStep), minus_ref, factor, c));
+          }
           if (part.owns(y, begin, lane) >= 0) o[y] = from_float<T>(b.w);              // its writer puts the target's entry right
         }
         if (++g_slot == slots) g_slot = 0;
