@@ -600,3 +600,26 @@ def test_tokens_that_cannot_occur(cuda):
     grad = ops.preference_loss_bwd(torch.ones(2, device=cuda), coef, ends, 8)
     beta = float(torch.tensor(0.1))
     assert grad.tolist() == [0.0, 0.0, -beta, -beta, 0.0, 0.0, beta, beta]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(900, 700), (700, 9001), (450, 50001), (90, 260003), (3, 130003)])
+def test_rows_that_take_no_part_change_no_other(cuda, dtype, rows, vocab):
+    """Ignored rows before, behind, between and instead of all others: the rest is the same bit for bit, the ignored ones are 0."""
+    from b2g import ops
+
+    g = torch.Generator(device=cuda).manual_seed(vocab)
+    x = torch.randn(rows, vocab, device=cuda, generator=g).to(dtype)
+    target = torch.randint(0, vocab, (rows,), device=cuda, generator=g)
+    adv = torch.randn(rows, device=cuda, generator=g)
+    every = ops.token_logprobs(x, target, dtype=torch.float64)[0]
+    loss, logp, _, grad = ops.policy_loss(x, target, adv)
+    at = torch.arange(rows, device=cuda)
+    for dead in (at < rows // 2, at >= rows // 3, at % 3 != 1, at % 7 == 0, at >= 0):
+        t = torch.where(dead, -100, target)
+        got = ops.token_logprobs(x, t, dtype=torch.float64)[0]
+        assert torch.equal(got, torch.where(dead, 0.0, every))
+        l, lp, _, gr = ops.policy_loss(x, t, adv)
+        assert torch.equal(l, torch.where(dead, 0.0, loss)) and torch.equal(lp, torch.where(dead, 0.0, logp))
+        assert torch.equal(gr, torch.where(dead[:, None], torch.zeros((), dtype=dtype, device=cuda), grad))
+    ops.check_status()
