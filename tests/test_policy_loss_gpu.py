@@ -561,7 +561,8 @@ def test_many_rows_of_every_path_repeat_bit_for_bit(cuda):
         adv = torch.randn(rows, generator=g, device=cuda)
         want = ops.policy_loss(x, t, adv)
         logp = ops.token_logprobs(x, t)[0]
-        assert torch.equal(logp, want[1])
+        # wide rows have a kernel of their own for either: twice the error of a log-sum-exp, and half a step on both sides
+        assert bool(((logp - want[1]).abs().double() <= 2 * ref.lse_error(vocab) + 2.0 ** -23 * logp.abs().double()).all())
         for _ in range(3):
             got = ops.policy_loss(x, t, adv)
             assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(ops.token_logprobs(x, t)[0], logp)
