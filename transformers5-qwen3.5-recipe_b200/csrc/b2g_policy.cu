@@ -561,8 +561,8 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const T* logits
 
 // ---- rows in a pipeline ------------------------------------------------------------------------------
 // Clusters that stay and go from row to row, two CTAs on every SM (two whose phases differ keep memory and the special-function
-// unit busier than one of twice the size: 1024 x 248320 bf16 in 218 against 233 us).  13 warps work, two more do everything that
-// is latency.  For every row k:
+// unit busier than one of twice the size: 1024 x 248320 bf16 in 218 against 233 us).  12 warps work, three on each scheduler, two
+// more do everything that is latency (207 us; with 13 workers 211, with 8 209, with 16, at 56 registers a thread, 219).  For every row k:
 //   the first of them reads 128 samples and the target's logit, and publishes their maximum as the row's reference: a sum of
 //     exponentials needs no maximum, only a number near it, so the workers need no pass for one and their sums simply add up;
 //   S(k): the workers' sums of exp((z - reference)/tau) over everything but the target, one number per warp.  A warp whose sum
@@ -575,19 +575,19 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(const T* logits
 // by one lane: as 16-byte copies of every lane they took the load-store unit as long as the arithmetic), reads them in S and in G,
 // and fetches those of the row `slots` further on into the same place.  One copy per CTA and row, by a warp that waits until all
 // are done with the slot, 240 against 219 us; a slice that passes twice, the second time from L2, 233 us.
-//   Bound: two exponentials per logit at 16 per cycle and SM (126 us of the 218), then HBM (155 us); the two overlap only between
+//   Bound: two exponentials per logit at 16 per cycle and SM (126 us of the 207), then HBM (155 us); the two overlap only between
 //   CTAs.  Replacing one exponential in four by a polynomial on the fp32 pipe was slower (231 us): the loops issue 12 instructions
 //   per logit, and the polynomial adds six to every one that it replaces.
 //   fp32 logits: an exponential has as many bits as its logit, takes its place in S, and G only scales it (2000 x 16000: 62 against
 //   68 us).  A bf16 logit's place is too small for it: a cotangent that is rounded twice is not what the type can hold.
 // Log-probabilities: nothing is wanted twice, so a slice passes through the slots in chunks of kTurns vectors a lane, which a warp
-// of its own copies, 52 KB at a time (a bulk copy costs some 40 ns beside its bytes: with 4 KB copies by every warp 105 us in
-// place of 97, 1024 x 248320 bf16 with a tenth of the rows left out).
+// of its own copies, 54 KB at a time (a bulk copy costs some 40 ns beside its bytes: with 4 KB copies by every warp 105 us in
+// place of 89, 1024 x 248320 bf16 with a tenth of the rows left out).
 //   Bound: HBM (70 us; the same kernel without its arithmetic takes 6 us less).
 // All waits are bounded; a CTA whose wait ran out stops working, and all CTAs of a cluster leave together.
-constexpr int kWorkerWarps = 13, kWorkers = kWorkerWarps * 32, kRing = 8, kMaxCluster = 10, kMaxLead = 3, kAhead = 7, kInfo = 16, kSamples = 4;
+constexpr int kWorkerWarps = 12, kWorkers = kWorkerWarps * 32, kRing = 8, kMaxCluster = 10, kMaxLead = 3, kAhead = 7, kInfo = 16, kSamples = 4;
 constexpr int kMaxSlots = 2;                                             // policy loss
-constexpr int kStages = 2, kTurns = 8, kChunk = kWorkers * kTurns;       // log-probabilities
+constexpr int kStages = 2, kTurns = 9, kChunk = kWorkers * kTurns;       // log-probabilities
 
 struct Share { float m, unused; double d; };       // what a CTA sends: its sum and what it is against (16 bytes: one store)
 
@@ -683,7 +683,7 @@ __device__ __forceinline__ double lane_sum_against(uint32_t place, int n, float 
   const F2 minus_ref = f2(-ref, -ref);
   F2 d = f2(0.f, 0.f);
   int i = 0;
-#pragma unroll 2
+#pragma unroll 4
   for (; i + 1 < n; i += 2)
     d = d + (exp_sum(from_shared<T>(place + i * kStep), minus_ref, c) + exp_sum(from_shared<T>(place + (i + 1) * kStep), minus_ref, c));
   if (i < n) d = d + exp_sum(from_shared<T>(place + i * kStep), minus_ref, c);
@@ -737,11 +737,11 @@ __device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
 }
 
 template <bool kPolicy>
-constexpr int kPipeThreads = kWorkers + (kPolicy ? 64 : 96);      // two CTAs of either have the 64 registers a thread that an SM holds for them
+constexpr int kPipeThreads = kWorkers + (kPolicy ? 64 : 96);      // so that two CTAs of either have 64 registers a thread
 
 template <typename T, bool kPolicy>
 __global__ void __launch_bounds__(kPipeThreads<kPolicy>, 2) pipe_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out, int64_t rows,
-                                                                int cluster, int slots, int lead, int per, int per_warp) {
+                                                                int cluster, int slots, int lead, int per) {
   constexpr int N = Vec<T>::N, kStep = 32 * 16;
   constexpr bool kKeep = kPolicy && sizeof(T) == 4;      // G finds the exponentials of S in the logits' places
   extern __shared__ __align__(16) uint8_t space[];
@@ -923,8 +923,10 @@ __global__ void __launch_bounds__(kPipeThreads<kPolicy>, 2) pipe_kernel(const T*
       if (j >= 0) fine = dev::mbar_wait(dev::smem_u32(&ready[j % kRing]), (j / kRing) & 1, &gave_up, a.status, 503);
     }
   } else {
-    const int begin = rank * per + warp * per_warp, limit = min((rank + 1) * per, begin + per_warp), slot_bytes = per * 16;
-    const uint32_t base = dev::smem_u32(space) + warp * per_warp * 16, V = (uint32_t)a.V;
+    // whole turns of 32 vectors, dealt out as evenly as they can be
+    const int turns = (per + 31) / 32, from = warp * turns / kWorkerWarps * 32, to = (warp + 1) * turns / kWorkerWarps * 32;
+    const int begin = rank * per + from, limit = rank * per + min(per, to), slot_bytes = per * 16;
+    const uint32_t base = dev::smem_u32(space) + from * 16, V = (uint32_t)a.V;
     const Scale c = a.c;
     const bool steady = (ld * (int64_t)sizeof(T)) % 16 == 0;
     const T* const x0 = logits + first * ld;
@@ -1008,8 +1010,17 @@ __global__ void __launch_bounds__(kPipeThreads<kPolicy>, 2) pipe_kernel(const T*
             for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled(from_shared<T>(place + i * kStep), factor));
           } else {
             const F2 factor = f2(b.y, b.y), minus_ref = f2(-b.z, -b.z);
-#pragma unroll 2
-            for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled_exp(from_shared<T>(place + i * kStep), minus_ref, factor, c));
+            if (wide && part.full_begin == begin && part.full_end == part.end) {
+              uint4* const to16 = reinterpret_cast<uint4*>(to) + begin + lane;
+#pragma unroll 4
+              for (int i = 0; i < part.n; ++i) {
+                const Vec<T> w = scaled_exp(from_shared<T>(place + i * kStep), minus_ref, factor, c);
+                __stcs(to16 + i * 32, make_uint4(w.w[0], w.w[1], w.w[2], w.w[3]));
+              }
+            } else {
+#pragma unroll 1
+              for (int i = 0; i < part.n; ++i) put(begin + lane + i * 32, scaled_exp(from_shared<T>(place + i * kStep), minus_ref, factor, c));
+            }
           }
           if (part.owns(y, begin, lane) >= 0) o[y] = from_float<T>(b.w);              // its writer puts the target's entry right
         }
@@ -1357,13 +1368,11 @@ static int launch_pipe(const T* logits, int64_t ld, const policy::RowArgs& a, T*
   const int64_t slice = (need + best - 1) / best * 16;
   const int slots = !kPolicy || kSliceLimit / slice < policy::kMaxSlots ? 1 : policy::kMaxSlots;
   const int lead = slots - 1;      // G trails S by a row where there is a second slot to wait in
-  // whole turns of 32 vectors per warp; the last warps may have none
-  const int per_warp = (int)((slice / 16 + policy::kWorkers - 1) / policy::kWorkers) * 32;
   cudaLaunchAttribute at[1];
   cudaLaunchConfig_t cfg = pipe_config<T, kPolicy>(best, kPolicy ? slice * slots : kStreamBytes, at);
   cfg.gridDim = dim3((unsigned)((rows < best_resident ? rows : best_resident) * best));
   cfg.stream = s;
-  B2G_CUDA_OK(cudaLaunchKernelEx(&cfg, policy::pipe_kernel<T, kPolicy>, logits, ld, a, out, ld_out, rows, best, slots, lead, (int)(slice / 16), per_warp));
+  B2G_CUDA_OK(cudaLaunchKernelEx(&cfg, policy::pipe_kernel<T, kPolicy>, logits, ld, a, out, ld_out, rows, best, slots, lead, (int)(slice / 16)));
   return 0;
 }
 
