@@ -1156,6 +1156,9 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(const L* __restrict_
   __shared__ double2 part[kPairClusterMax][2];       // of the cluster's first CTA: every CTA's sum and count of either sequence
   const int rank = blockIdx.x % cluster, half = threadIdx.x / kHalf, thread = threadIdx.x % kHalf, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t p = blockIdx.x / cluster;
+  // Another CTA's shared memory may be written only once that CTA has started: all arrive here, and wait before they send.  A CTA
+  // with nothing to read comes to its store after two loads.
+  dev::cluster_arrive();
   int64_t begin, end;
   bounds(offsets, p + half * P, N, begin, end, status);
   double s = 0.0;                                    // differences and sums in 64 bits
@@ -1188,6 +1191,7 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(const L* __restrict_
   }
   if (lane == 0) { warp_sum[warp] = s; warp_count[warp] = n; }
   __syncthreads();
+  dev::cluster_wait();
   if (threadIdx.x < 2) {                             // thread h: sequence h
     double sum = 0.0, count = 0.0;
     for (int i = 0; i < kHalfWarps; ++i) { sum += warp_sum[threadIdx.x * kHalfWarps + i]; count += (double)warp_count[threadIdx.x * kHalfWarps + i]; }
