@@ -277,6 +277,7 @@ __global__ void __launch_bounds__(160) lora_down_tma_kernel(const __grid_constan
         mma_bf16(acc[0], a, b[0], b[1]);
         mma_bf16(acc[1], a, b[2], b[3]);
       }
+      dev::fence_proxy_async_smem();      // as in lora_wgrad_tma_kernel: the refill must not overtake the last fragments' reads
       __syncwarp();
       if (lane == 0) dev::mbar_arrive(empty(st));
       if (++st == kDtStages) { st = 0; ph ^= 1; }
@@ -482,6 +483,10 @@ __global__ void __launch_bounds__(160) lora_wgrad_tma_kernel(const __grid_consta
         mma_bf16(acc[np * 2 + 1], a, b[2], b[3]);
       }
     }
+    // The fragments were read through the generic proxy and the refill is a write of the async proxy, which an arrival alone does
+    // not put behind them: without the fence a few rows of the last fragment were now and then those of the step after (up to one
+    // call in six of [8192, 16]^T [8192, 4096]).
+    dev::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) dev::mbar_arrive(empty(st));
     if (++st == kWtStages) { st = 0; ph ^= 1; }
