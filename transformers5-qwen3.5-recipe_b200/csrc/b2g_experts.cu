@@ -5,9 +5,10 @@
 //
 // One warp per token; lane i holds experts [i * kPer, (i + 1) * kPer), so the lowest lane of a tie holds the lowest expert.
 // The order of c is its order in 64 bits (without a bias: the order of the logits), so the choice does not depend on how an
-// exponential is rounded.  The work is done in 32 bits; where two neighbours of the order lie closer than the 32-bit scores can
-// be wrong and are not equal by construction (same logit, same bias), the warp ranks its candidates, or its groups, once more in
-// 64 bits.  NaN among the logits send it over the whole token in 64 bits.
+// exponential is rounded.  The work is done in 32 bits; where a choice lies closer to its neighbour among the chosen, or the last
+// one to anything left out, than their 32-bit values can be wrong, and the two are not equal by construction (same logit, same
+// bias), the warp ranks its candidates, or its groups, once more in 64 bits.  NaN among the logits (with groups: among the choices)
+// send it over the whole token in 64 bits.
 #include "b2g_common.cuh"
 
 namespace b2g {
@@ -30,7 +31,7 @@ __device__ __forceinline__ double score_of(double x, int fn) {
   return sqrt(fmax(x, 0.0) + log1p(exp(-fabs(x))));
 }
 
-// Relative error 2^-21.5 at most: exponential and logarithm 2^-22, sum, quotient and root half a step each.
+// Relative error 2^-20.8 at most: exponential, fast quotient and logarithm 2^-22 each, sum and root half a step.
 __device__ __forceinline__ float score_of(float x, int fn) {
   const float n = expf(-fabsf(x));
   if (fn == kSigmoid) return __fdividef(x >= 0.f ? 1.f : n, 1.f + n);
@@ -252,9 +253,10 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
   const T* row = logits + t * ld;
   WarpSpace<kPer>& ws = space[warp];
   const bool wide = (reinterpret_cast<uintptr_t>(row) & 15) == 0, grouped = kScored && M < G, biased = kScored && bias;
-  // 32-bit scores are off by 2^-21.5 (softmax: 2^-18, the exponent being rounded at sizes up to 100); twice that for a difference
-  const float eps = fn == kSoftmax ? 7.62939453125e-6f : 9.5367431640625e-7f;
-  constexpr float kStep = 2.384185791015625e-7f;      // and 2^-22 of the sums
+  // 32-bit scores are off by 2^-20.8 (softmax: 2^-17.5, the exponent being rounded at sizes up to 100): eps / 2; sums by half a step of
+  // theirs, 2^-24, for which a quarter of kStep stands
+  const float eps = fn == kSoftmax ? 1.52587890625e-5f : 1.9073486328125e-6f;
+  constexpr float kStep = 2.384185791015625e-7f;
 
   // c[j]: what expert first + j is chosen by; NaN where there is none to choose
   float c[kPer], top = -INFINITY, denominator = 1.f, smax = 1.f;
@@ -295,6 +297,18 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
       for (int j = 0; j < kPer; ++j) s[j] = c[j] = s[j] + b[j];
     }
     if (grouped) {                                     // s: what the groups are compared by
+      // A group's two best may cancel, so what rounding has cost them goes by the largest choice and not by their sum.
+      float largest = smax;
+      if (biased) {
+        float all = 0.f;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          all += fabsf(s[j]);
+          largest = fmaxf(largest, fabsf(s[j]) < INFINITY ? fabsf(s[j]) : 0.f);
+        }
+        unsure = unsure || __any_sync(0xffffffffu, all != all);
+        largest = lanes_max(largest);
+      }
       Two two{-INFINITY, -INFINITY};
       int group = lane;
       if (lane_shift >= 0) {                           // its first lane speaks for a group
@@ -326,7 +340,8 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
           last = all;
           if (lane == src) worth = NAN;
         } else {
-          if (!(last - all > 2.f * eps * smax + kStep * fabsf(last)) && !unsure)
+          // two choices in either group, eps / 2 of a score and half a step of itself each, and half a step of their sum
+          if (!(last - all > 2.f * eps * smax + 2.f * kStep * largest) && !unsure)
             kept = groups_in_64_bits<T, kPer>(row, bias, fn, G, M, best, E, ws.value);
         }
       }
@@ -401,16 +416,26 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
     const bool out = lane < K;
     Pick p = out ? ws.sorted[lane] : Pick{0.f, 0};
     if (biased) {
-      bool close = false;
-      if (out && lane + 1 < min(n, ranks)) {
-        const Pick q = ws.sorted[lane + 1];            // a score is at most its choice less its bias, give or take a step
-        const float bp = bias[p.id], bq = bias[q.id];
-        close = !(p.c - q.c > eps * fmaxf(fabsf(p.c - bp), fabsf(q.c - bq)) + kStep * (fabsf(p.c) + fabsf(bp) + fabsf(bq))) &&
-                !(bp == bq && load_logit(row, p.id) == load_logit(row, q.id));
+      // What a 32-bit choice may be off by: a score is at most its choice less its bias, give or take a step.
+      auto slack = [&](float choice, float b) { return 0.5f * eps * fabsf(choice - b) + kStep * (fabsf(choice) + fabsf(b)); };
+      auto near = [&](const Pick& u, const Pick& v) {  // u.c >= v.c: is v before u in 64 bits, for all that is known?
+        const float bu = bias[u.id], bv = bias[v.id];
+        return !(u.c - v.c > slack(u.c, bu) + slack(v.c, bv)) && !(bu == bv && load_logit(row, u.id) == load_logit(row, v.id));
+      };
+      bool close = out && lane + 1 < K && near(p, ws.sorted[lane + 1]);
+      // The border: anything that was left out, not only the first of it.  One of a large score under a large negative bias may be
+      // off by more than the others, and one that equals the last choice by construction says nothing about those behind it.
+      const Pick last = ws.sorted[K - 1];
+      const float reach = eps * smax + 2.f * kStep * (smax + fabsf(last.c));
+      for (int h = lane; h < n; h += 32) {
+        const Pick o = ws.candidate[h];
+        const bool left_out = o.c < last.c || (o.c == last.c && o.id > last.id);
+        if (left_out && !(last.c - o.c > reach + 2.f * kStep * fabsf(o.c))) close = close || near(last, o);
       }
       if (__any_sync(0xffffffffu, close)) {            // the candidates once more, in 64 bits
         double all = 1.0;
-        if (fn == kSoftmax) {
+        const bool nothing = top == -INFINITY;         // every score is 0
+        if (fn == kSoftmax && !nothing) {
           float x[kPer];
           load_lane<T, kPer>(row, first, E, wide, -INFINITY, x);
           all = 0.0;
@@ -422,7 +447,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
         for (int h = lane; h < n; h += 32) {
           const int id = ws.candidate[h].id;
           const double x = load_logit(row, id);
-          ws.exact[h] = (fn == kSoftmax ? exp(x - (double)top) / all : score_of(x, fn)) + (double)bias[id];
+          ws.exact[h] = (fn != kSoftmax ? score_of(x, fn) : nothing ? 0.0 : exp(x - (double)top) / all) + (double)bias[id];
         }
         __syncwarp();
         for (int h = lane; h < n; h += 32) {
