@@ -489,34 +489,43 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const T* __restrict_
 // dl from dw.  With u_j = w_j / alpha and dot = sum_i g_i w_i:  renormalised ds_j s_j = u_j (alpha g_j - dot), else ds_j s_j = g_j w_j;
 // the slopes of the score functions relative to the score are 1 - sigmoid (sigmoid), sigmoid / (2 softplus) (sqrtsoftplus) and
 // 1 (softmax, whose common denominator cancels when renormalised and otherwise gives every expert - s_e * dot).
-// The choices' own terms are in 64 bits, and each product is rounded before the difference: alpha g_j - dot cancels where one
-// expert has nearly all the weight, and with a single choice it is 0 and has to come out as 0.
+// The choices' own terms are in 64 bits, from the logits and not from the weights that fp32 has rounded, and each product is rounded
+// before the difference: alpha g_j - dot cancels where one expert has nearly all the weight, and with a single choice it is 0 and
+// has to come out as 0.  Softmax that is not renormalised needs the sum over the row for that; its 32-bit exponentials are added in
+// 64 bits, so that the rest beside a dominant one keeps its digits.
 // A warp takes kTokens tokens at once, 32 / kTokens lanes on the choices of each, and then writes their rows one after the other:
 // with one token a warp spent most of its time waiting for three short loads (65536 x 256 bf16, top 8: 16 us, 13.5 us with four).
 template <typename T, int kPer, int kTokens>
 __global__ void __launch_bounds__(kWarps * 32) route_bwd_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ grad_w,
-                                                                const float* __restrict__ weights, const int64_t* __restrict__ indices, int fn,
-                                                                int renorm, float alpha, T* __restrict__ grad, int64_t tokens, int E, int K) {
-  constexpr int N = 16 / sizeof(T), kLanes = 32 / kTokens;
+                                                                const int64_t* __restrict__ indices, int fn, int renorm, float alpha,
+                                                                T* __restrict__ grad, int64_t tokens, int E, int K) {
+  constexpr int N = 16 / sizeof(T), kLanes = 32 / kTokens, kNotChosen = 0x7FC0DEAD;      // a NaN that no arithmetic gives
   __shared__ __align__(16) float value[kWarps][kTokens][32 * kPer];
-  __shared__ float dots[kWarps][kTokens];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = lane * kPer, mine = lane / kLanes, slot = lane % kLanes;
   const int64_t t0 = ((int64_t)blockIdx.x * kWarps + warp) * kTokens, t = t0 + mine;
   if (t0 >= tokens) return;
   const bool in = t < tokens && slot < K;
-  const float g = in ? grad_w[t * K + slot] : 0.f, w = in ? weights[t * K + slot] : 0.f;
+  const float g = in ? grad_w[t * K + slot] : 0.f;
   const int64_t e64 = in ? indices[t * K + slot] : -1;
   const bool ok = e64 >= 0 && e64 < E;
   const int e = ok ? (int)e64 : 0;
-  const float raw = ok && fn != kSoftmax ? load_logit(logits + t * ld, e) : 0.f;
+  const float raw = ok ? load_logit(logits + t * ld, e) : 0.f;
+  const bool whole_row = fn == kSoftmax && !renorm;
 #pragma unroll
   for (int u = 0; u < kTokens; ++u)
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) value[warp][u][first + j] = 0.f;
+    for (int j = 0; j < kPer; ++j) value[warp][u][first + j] = whole_row ? __int_as_float(kNotChosen) : 0.f;
   const double g64 = g, raw64 = raw;
-  double own = 0.0, part = w, total = 1.0;           // a score, its weight, and what it was divided by
-  if (fn != kSoftmax) {
-    own = ok ? score_of(raw64, fn) : 0.0;
+  double own = 0.0, part = 0.0, total = 1.0;         // a score, its weight, and what it was divided by
+  if (!whole_row) {
+    if (fn == kSoftmax) {                            // of the chosen logits
+      float m = ok ? raw : -INFINITY;
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      own = !ok || (m == -INFINITY && raw == raw) ? 0.0 : exp(raw64 - (double)m);
+    } else {
+      own = ok ? score_of(raw64, fn) : 0.0;
+    }
     if (renorm) {
       total = own;
 #pragma unroll
@@ -532,39 +541,51 @@ __global__ void __launch_bounds__(kWarps * 32) route_bwd_kernel(const T* __restr
   if (renorm) slope = __dadd_rn(slope, -dot) / total;
   double d;
   if (fn == kSoftmax) {
-    d = slope * (part / (double)alpha);              // not renormalised: alpha g s, and the row's share below
+    d = slope * own;                                 // the slope is divided by the sum of the choices
   } else {
     const double sig = 1.0 / (1.0 + exp(-raw64));
     if (fn == kSigmoid) d = slope * (sig * (1.0 / (1.0 + exp(raw64))));
     else d = raw64 < -600.0 ? slope * 0.5 * own : slope * (sig / (2.0 * own));      // far below 0 both are e^(x/2) / 2
   }
   __syncwarp();
-  if (ok) value[warp][mine][e] = (float)d;
-  if (slot == 0) dots[warp][mine] = (float)dot;
+  if (ok && !whole_row) value[warp][mine][e] = (float)d;
   __syncwarp();
 #pragma unroll
   for (int u = 0; u < kTokens; ++u) {
     if (t0 + u >= tokens) return;
     float v[kPer];
+    if (!whole_row) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = value[warp][u][first + j];
-    if (fn == kSoftmax && !renorm) {
+      for (int j = 0; j < kPer; ++j) v[j] = value[warp][u][first + j];
+    } else {                                         // every expert has its share; the choices' entries go through shared memory
       const T* row = logits + (t0 + u) * ld;
-      const float of_row = dots[warp][u];
-      float x[kPer], sum = 0.f;
+      float x[kPer];
       load_lane<T, kPer>(row, first, E, (reinterpret_cast<uintptr_t>(row) & 15) == 0, -INFINITY, x);
       float top = x[0];
 #pragma unroll
       for (int j = 1; j < kPer; ++j) top = fmaxf(top, x[j]);
       top = warp_maxf(top);
+      double sum = 0.0;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         x[j] = top == -INFINITY && x[j] == x[j] ? 0.f : expf(x[j] - top);
-        sum += x[j];
+        sum += (double)x[j];
       }
-      sum = warp_sum(sum);
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) v[j] -= x[j] == 0.f ? 0.f : x[j] / sum * of_row;
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const bool chosen = ok && mine == u;
+      const double s = !chosen || (top == -INFINITY && raw == raw) ? 0.0 : exp(raw64 - (double)top) / sum;
+      double of_row = chosen ? __dmul_rn(__dmul_rn((double)alpha, g64), s) : 0.0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) of_row += __shfl_xor_sync(0xffffffffu, of_row, o);
+      const float each = (float)(of_row / sum);
+      if (chosen) value[warp][u][e] = (float)(s * __dadd_rn(__dmul_rn((double)alpha, g64), -of_row));
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        v[j] = value[warp][u][first + j];
+        if (__float_as_int(v[j]) == kNotChosen) v[j] = x[j] == 0.f ? 0.f : -x[j] * each;
+      }
     }
     T* out = grad + (t0 + u) * (int64_t)E;
     bool written = false;
@@ -672,7 +693,7 @@ extern "C" int b2g_route_experts_bwd(const void* logits, int64_t ld, int logits_
   const int tokens = top_k <= 8 && T >= 8192 ? 4 : 1;
   const int blocks = (int)((T + experts::kWarps * tokens - 1) / (experts::kWarps * tokens));
 #define B2G_ROUTE_BWD_AS(TYPE, PER, TOKENS)                                                                                                \
-  experts::route_bwd_kernel<TYPE, PER, TOKENS><<<blocks, experts::kWarps * 32, 0, s>>>(static_cast<const TYPE*>(logits), ld, grad_weights, weights, \
+  experts::route_bwd_kernel<TYPE, PER, TOKENS><<<blocks, experts::kWarps * 32, 0, s>>>(static_cast<const TYPE*>(logits), ld, grad_weights, \
       indices, score_fn, renormalize, scaling, static_cast<TYPE*>(grad_logits), T, E, top_k)
 #define B2G_ROUTE_BWD(PER)                                              \
   do {                                                                  \
