@@ -257,17 +257,6 @@ __device__ __forceinline__ Given given(const RowArgs& a, int64_t row) {
   return Given{a.weight ? a.weight[row] : 1.f, a.advantage[row], a.old_logp ? a.old_logp[row] : 0.f, a.ref_logp ? a.ref_logp[row] : 0.f};
 }
 
-// 1 - p of the target, the entry of the cotangent that cancels when the target is nearly certain.  16-bit logits take the exact
-// value; fp32 logits take it from z/tau and lse rounded to 32 bits, as the elementary form of the gradient in that type does (off
-// by half a step of lse), unless lse is so large (a vocabulary masked throughout by the type's lowest value) that it holds no
-// log d any more.
-template <typename T>
-__device__ __forceinline__ float rest_of(double exact, float zy, double logp, float tau) {
-  if (sizeof(T) == 2) return (float)exact;
-  const float z = zy / tau, lse = (float)((double)z - logp);
-  return fabsf(lse) < 16384.f ? 1.f - expf(z - lse) : (float)exact;
-}
-
 __device__ __forceinline__ void put_logp(const RowArgs& a, int64_t row, double logp, float4 stats) {
   if (a.logp64) static_cast<double*>(a.logp)[row] = logp;
   else static_cast<float*>(a.logp)[row] = (float)logp;
@@ -318,7 +307,7 @@ template <typename T, bool kPolicy>
 __device__ __forceinline__ float4 conclude(const RowArgs& a, const Stat& t, float zy, const Given& in, int64_t r, bool write) {
   const double d = whole_sum<T>(t.d), above = ((double)zy - (double)t.m) * a.inv_tau, own = exp(above), all = own + d;
   const double logp = own > d ? -log1p(d / own) : above - log(all);
-  const float per_sum = 1.f / (float)all, rest = rest_of<T>((double)((float)d * per_sum), zy, logp, a.tau);
+  const float per_sum = 1.f / (float)all, rest = (float)d * per_sum;
   if (!kPolicy) {
     if (write) put_logp(a, r, logp, make_float4(t.m, per_sum, rest, (float)((double)zy * a.inv_tau - logp)));
     return make_float4(0.f, 0.f, 0.f, 0.f);
