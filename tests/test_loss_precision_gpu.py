@@ -65,3 +65,42 @@ def test_a_shift_of_all_logits_changes_no_gradient(cuda):
             got = ops.policy_loss((logits + shift).to(cuda), target.to(cuda), adv)[3]
             assert torch.equal((logits + shift) - shift, logits)
             torch.testing.assert_close(got, want, rtol=2.0 ** -20, atol=0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(256, 3001), (128, 9001), (96, 32003), (64, 129280)])
+@pytest.mark.parametrize("tau", [1.0, 0.973, 0.899])
+def test_log_probabilities_of_flat_rows(cuda, dtype, rows, vocab, tau):
+    """fp64 log-probabilities of rows without a standing-out token, root mean square over the rows.
+
+    A term is off by up to 2^-22 (exponential), 3 * 2^-24 (tree) and 2 * 2^-24 of its exponent, 16 at most for the terms that count;
+    uniformly distributed that is 1 / sqrt(3) of it, and the terms' errors are independent: with n = (sum p)^2 / sum p^2 of them
+    the sum's is 1 / sqrt(n) of one.  ex2.approx is short by 3.7e-8 ... 5.9e-8 according to the fraction, 4.9e-8 of which is
+    put back: 1.2e-8 may be left."""
+    from b2g import ops
+
+    g = torch.Generator().manual_seed(vocab + rows)
+    logits = (torch.randn(rows, vocab, generator=g) * 1.5).to(dtype)
+    target = torch.randint(0, vocab, (rows,), generator=g)
+    t32 = float(torch.tensor(tau, dtype=torch.float32))
+    want = ref.logprobs(logits.double(), target, t32)
+    got = ops.token_logprobs(logits.to(cuda), target.to(cuda), tau, dtype=torch.float64)[0].cpu()
+    p = torch.softmax(logits.double() / t32, 1)
+    n = 1.0 / (p * p).sum(1)
+    one = (2.0 ** -22 + 2.0 ** -24 * (3 + 2 * 16)) / math.sqrt(3.0)
+    bound = float((one * one / n).mean().sqrt()) + 1.2e-8
+    rms = float((got - want).pow(2).mean().sqrt())
+    bias = float((got - want).mean())
+    assert rms <= bound, (rms, bias, bound)
+
+
+def test_equal_logits_show_the_whole_correction(cuda):
+    """exp2(0) is exact, and so is what a row of equal logits sums: there the average that is put back for ex2.approx is an error,
+    4.9e-8 in every log-probability of bf16 rows.  fp32 rows use no such correction: a double's steps, and 2^-24 of the sum's."""
+    from b2g import ops
+
+    for vocab in (1000, 9001, 129280):
+        t = torch.tensor([5], device=cuda)
+        for dtype, bound in ((torch.bfloat16, 5e-8), (torch.float32, 2.0 ** -30)):
+            got = float(ops.token_logprobs(torch.full((1, vocab), 2.5, dtype=dtype, device=cuda), t, dtype=torch.float64)[0])
+            assert abs(got + math.log(vocab)) <= bound + 1e-14 * math.log(vocab), (vocab, dtype)

@@ -14,7 +14,8 @@ namespace policy {
 
 constexpr float kLowest = -3.402823466e38f;
 // ex2.approx falls short by 4.9e-8 of its value on average (measured over 4 Mi arguments in [-20, 0], 3.7e-8 to 5.9e-8 in
-// the eight octiles of the fraction); a sum of many of them is that much too small.
+// the eight octiles of the fraction); a sum of many of them is that much too small.  The average is right for sums of many terms:
+// a rest of one or two terms keeps up to 1.2e-8 of it, and terms that ex2 gives exactly (equal logits: 2^0) are 4.9e-8 too large.
 constexpr double kEx2Shortfall = 4.9e-8;
 
 template <typename T>
@@ -35,8 +36,9 @@ __device__ __forceinline__ float ex2(float x) {
 
 // exp((z - m) / tau).  16-bit logits: one ex2, its factor log2(e)/tau in two parts (a single fp32 factor is off by 1.3e-8,
 // which times the spread of the logits would reach every log-probability with the same sign).  fp32 logits, whose gradient
-// keeps 24 bits, take the full exponential; they move twice the bytes per value, so it is as well hidden.
-struct Scale { float hi, lo, inv; };
+// keeps 24 bits, take the full exponential, its factor 1/tau in two parts for the same reason (off by up to 6e-8, and the same
+// in the sum and in the gradient, whose entries cancel over a row); they move twice the bytes per value, so it is as well hidden.
+struct Scale { float hi, lo, inv, inv_lo; };
 // Two floats in one 64-bit register pair: one instruction of the two-wide fp32 pipe each.
 struct F2 { uint64_t v; };
 __device__ __forceinline__ F2 f2(float lo, float hi) {
@@ -71,7 +73,7 @@ __device__ __forceinline__ F2 exp_from(F2 z, F2 minus_m, const Scale& c) {
     split(kSum ? fma2(x, h, x * f2(c.lo, c.lo)) : x * h, lo, hi);
     return f2(ex2(lo), ex2(hi));
   } else {
-    split(x * f2(c.inv, c.inv), lo, hi);
+    split(fma2(x, f2(c.inv, c.inv), x * f2(c.inv_lo, c.inv_lo)), lo, hi);
     return f2(expf(lo), expf(hi));
   }
 }
@@ -1277,11 +1279,14 @@ static policy::RowArgs row_args(const int64_t* target, int64_t V, int64_t ignore
   policy::RowArgs a = {};
   a.target = target; a.V = V; a.ignore_index = ignore_index; a.tau = tau; a.status = status;
   a.inv_tau = 1.0 / tau;
-  const double c = 1.4426950408889634 / tau;    // log2(e) / tau
-  a.c.hi = (float)c;
-  if ((double)a.c.hi >= c) a.c.hi = nextafterf(a.c.hi, 0.f);   // the low part is positive: -inf logits times both parts stay -inf
-  a.c.lo = (float)(c - (double)a.c.hi);
-  a.c.inv = 1.f / tau;
+  // the low parts are positive: -inf logits times both parts stay -inf
+  auto in_two = [](double c, float& hi, float& lo) {
+    hi = (float)c;
+    if ((double)hi >= c) hi = nextafterf(hi, 0.f);
+    lo = (float)(c - (double)hi);
+  };
+  in_two(1.4426950408889634 / tau, a.c.hi, a.c.lo);    // log2(e) / tau
+  in_two(1.0 / tau, a.c.inv, a.c.inv_lo);
   return a;
 }
 
