@@ -1,4 +1,5 @@
-"""GPU: digits of the row losses where something cancels: 1 - p of a nearly certain target, temperatures, sums of many terms."""
+"""GPU: digits of the row losses where something cancels: 1 - p of a nearly certain target, temperatures, sums of many terms; NaN that
+must not get lost."""
 import math
 
 import pytest
@@ -104,3 +105,18 @@ def test_equal_logits_show_the_whole_correction(cuda):
         for dtype, bound in ((torch.bfloat16, 5e-8), (torch.float32, 2.0 ** -30)):
             got = float(ops.token_logprobs(torch.full((1, vocab), 2.5, dtype=dtype, device=cuda), t, dtype=torch.float64)[0])
             assert abs(got + math.log(vocab)) <= bound + 1e-14 * math.log(vocab), (vocab, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [200, 9001, 40003, 1_000_003])
+def test_an_undefined_advantage_reaches_the_gradient(cuda, dtype, vocab):
+    from b2g import ops
+
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randn(3, vocab, generator=g).to(dtype).to(cuda)
+    target = torch.tensor([1, 2, 3], device=cuda)
+    adv = torch.tensor([1.0, float("nan"), -1.0], device=cuda)
+    for old in (None, torch.zeros(3, device=cuda)):
+        loss, _, _, grad = ops.policy_loss(logits, target, adv, old_logp=old)
+        assert bool(torch.isnan(loss[1])) and bool(torch.isnan(grad[1]).all())
+        assert bool(torch.isfinite(grad[[0, 2]]).all()) and bool(torch.isfinite(loss[[0, 2]]).all())

@@ -269,7 +269,7 @@ __device__ __forceinline__ void put_logp(const RowArgs& a, int64_t row, double l
 __device__ __forceinline__ float policy_scalars(const RowArgs& a, const Given& in, double logp, int64_t row, bool write) {
   const double adv = in.advantage, ratio = a.old_logp ? exp(logp - (double)in.old_logp) : (logp != logp ? logp : 1.0);
   const double clipped = fmin(fmax(ratio, 1.0 - (double)a.clip_low), 1.0 + (double)a.clip_high);
-  const bool inside = ratio * adv <= clipped * adv || ratio != ratio;
+  const bool inside = ratio * adv <= clipped * adv || ratio != ratio || adv != adv;      // NaN goes on to the gradient
   double loss = inside ? -ratio * adv : -clipped * adv, slope = inside ? -ratio * adv : 0.0, kl = 0.0;
   if (a.ref_logp) {
     const double d = (double)in.ref_logp - logp, em = expm1(d);
