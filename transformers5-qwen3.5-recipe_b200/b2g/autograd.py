@@ -22,6 +22,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 
@@ -393,6 +394,11 @@ def grouped_lora_experts(sel, gate_payload, up_payload, down_payload, quant_gate
 
 
 # ---- routing and post-training losses -----------------------------------------------------------
+def _carries_derivative(t: torch.Tensor) -> bool:
+    """Whether a call on ``t`` has to be an autograd node.  A forward-mode tangent is one that has no rule here: the node refuses it."""
+    return (t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None
+
+
 def _first_order_only(what: str) -> None:
     if torch.is_grad_enabled():
         raise RuntimeError(f"{what} does not support higher-order gradients")
@@ -420,7 +426,7 @@ class _RouteExperts(torch.autograd.Function):
 def route_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor] = None, score_function: str = "softmax", groups: int = 1,
                   top_groups: int = 1, group_experts: int = 1, renormalize: bool = True, scaling_factor: float = 1.0):
     """``ops.route_experts`` whose weights carry the gradient to the logits (the bias enters the choice only and gets none)."""
-    if not (logits.requires_grad and torch.is_grad_enabled()):
+    if not _carries_derivative(logits):
         return ops.route_experts(logits, top_k, bias, score_function, groups, top_groups, group_experts, renormalize, scaling_factor)
     return _RouteExperts.apply(logits, bias, (top_k, groups, top_groups, group_experts), (score_function, renormalize, scaling_factor))
 
@@ -445,7 +451,7 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, temperature: floa
     """Log-probabilities ``[rows]`` (fp32 or fp64) of the targets under ``softmax(logits / temperature)``, 0 where the target is
     ``ignore_index``; the logits stay as they are and get their gradient in their own type.  Take fp64 where the values are
     summed over a sequence, as ``preference_loss`` does."""
-    if not (logits.requires_grad and torch.is_grad_enabled()):
+    if not _carries_derivative(logits):
         return ops.token_logprobs(logits, target, temperature, ignore_index, dtype)[0]
     return _TokenLogprobs.apply(logits, target, temperature, ignore_index, dtype)
 
