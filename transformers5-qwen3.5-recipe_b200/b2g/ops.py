@@ -459,7 +459,8 @@ def preference_loss(logp: torch.Tensor, offsets: torch.Tensor, ref_logp: Optiona
 
     ``logp`` and ``ref_logp`` are fp32 or fp64 (sums are in fp64).  Sequence ``s`` is the tokens ``offsets[s]:offsets[s + 1]``; the
     chosen sequences come first, the rejected ones follow in the same order.  ``L_s`` is the sum (``average``: the mean) of ``logp - ref_logp`` over the tokens whose
-    ``target`` is not ``ignore_index`` (all of them without ``target``), 0 for a sequence without tokens.  ``"sigmoid"``:
+    ``target`` is not ``ignore_index`` (all of them without ``target``; it is asked for nothing else, so a target that
+    ``token_logprobs`` has reported as outside the vocabulary still counts), 0 for a sequence without tokens.  ``"sigmoid"``:
     ``-(1 - label_smoothing) log sigmoid(beta gap) - label_smoothing log sigmoid(-beta gap)``, ``gap = L_chosen - L_rejected``;
     ``"squared"``: ``(gap - 1 / (2 beta))^2``.  ``chosen`` and ``rejected`` are the rewards ``beta L_s``; ``coef`` is the gradient
     of a counted token.  Offsets that decrease or leave the tokens are clamped and reported through the status word (905)."""

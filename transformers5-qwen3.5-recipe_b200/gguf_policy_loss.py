@@ -153,8 +153,11 @@ def packed_preference_loss(hidden_states: torch.Tensor, lm_head, target: torch.T
                            chunk_size: int = _PACKED_LM_HEAD_CHUNK_SIZE) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(loss [pairs], chosen rewards, rejected rewards)`` of ``ops.preference_loss`` on the packed head.  The tokens of all
     sequences lie one behind the other (``hidden_states [tokens, hidden]``), the chosen sequences first; ``offsets`` has
-    ``2 * pairs + 1`` entries."""
+    ``2 * pairs + 1`` entries.  A target outside the vocabulary is reported through the status word (902) and takes no part, in the
+    sums and in the mean's count alike."""
     if target.dim() != 1:
         raise ValueError(f"packed_preference_loss takes the sequences one behind the other, got targets {tuple(target.shape)}")
     logp = packed_token_logprobs(hidden_states, lm_head, target, ignore_index=ignore_index, dtype=torch.float64, chunk_size=chunk_size)
+    # the pairs' kernel knows no vocabulary: it is told which tokens the log-probabilities have left out
+    target = target.masked_fill((target < 0) | (target >= int(lm_head.out_features)), ignore_index)
     return _ag.preference_loss(logp, offsets, ref_logp, beta, label_smoothing, loss_type, average, target, ignore_index)
