@@ -367,6 +367,12 @@ def _cotangent_out(logits: torch.Tensor, out: Optional[torch.Tensor], what: str)
     return out
 
 
+def _wrote_into(out: Optional[torch.Tensor]) -> None:
+    """Autograd learns of a buffer of the caller's that a kernel has overwritten: a graph that has saved it must not use it."""
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+
+
 _LOGP_DTYPES = (torch.float32, torch.float64)
 
 
@@ -404,9 +410,10 @@ def token_logprobs_bwd(grad_logp: torch.Tensor, logits: torch.Tensor, target: to
     if tuple(stats.shape) != (rows, 4) or stats.device != logits.device:
         raise ValueError(f"stats must be the [{rows}, 4] tensor of token_logprobs on the logits' device")
     temperature = _temperature(temperature)
-    out = _cotangent_out(logits, out, "token_logprobs_bwd")
+    given, out = out, _cotangent_out(logits, out, "token_logprobs_bwd")
     _launch("b2g_token_logprobs_bwd", logits, _a(logits), ld, int(logits.dtype == torch.float32), _a(target), _a(stats), _a(grad_logp),
             int(grad_logp.dtype == torch.float64), _a(out), out.stride(0) if rows > 1 else v, rows, v, temperature, int(ignore_index))
+    _wrote_into(given)
     return out
 
 
@@ -433,11 +440,12 @@ def policy_loss(logits: torch.Tensor, target: torch.Tensor, advantage: torch.Ten
         raise ValueError(f"kl_coef must be finite and not negative, got {kl_coef}")
     if kl_coef != 0.0 and ref_logp is None:
         raise ValueError("policy_loss: a KL term needs ref_logp")
-    out = _cotangent_out(logits, out, "policy_loss")
+    given, out = out, _cotangent_out(logits, out, "policy_loss")
     loss, logp, kl = (torch.empty(rows, dtype=torch.float32, device=logits.device) for _ in range(3))
     _launch("b2g_policy_loss", logits, _a(logits), ld, int(logits.dtype == torch.float32), _a(target), _a(advantage), _a(old_logp), _a(ref_logp),
             _a(weight), float(clip_low), float(clip_high), float(kl_coef), temperature, _a(loss), _a(logp), _a(kl), _a(out),
             out.stride(0) if rows > 1 else v, rows, v, int(ignore_index), _a(status_word(logits.device)))
+    _wrote_into(given)
     return loss, logp, kl, out
 
 
