@@ -362,7 +362,10 @@ def _cotangent_out(logits: torch.Tensor, out: Optional[torch.Tensor], what: str)
         def span(t):
             return t.storage_offset(), t.storage_offset() + (t.shape[0] - 1) * t.stride(0) + t.shape[1]
         (a0, a1), (b0, b1) = span(out), span(logits)
-        if a0 < b1 and b0 < a1:
+        pitch, columns = logits.stride(0), out.shape[1]
+        # rows of one pitch lie side by side where their columns do
+        beside = out.shape[0] > 1 and out.stride(0) == pitch and columns <= (a0 - b0) % pitch <= pitch - columns
+        if a0 < b1 and b0 < a1 and not beside:
             raise ValueError(f"{what}: out overlaps the logits without being the logits")
     return out
 
