@@ -18,6 +18,7 @@
 #include <cstring>
 
 #include "../../include/b2g.h"
+#include "b2g_once.h"
 
 // ---------------------------------------------------------------------------------------------
 // Host-side error plumbing: every extern "C" entry returns 0 or a negative B2G_E_* code and
@@ -49,7 +50,7 @@ inline int fail(int code, const char* fmt, ...) {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Per-kernel function attributes, set once per kernel and device instead of before every launch.
+// Per-kernel function attributes, set once per kernel and device instead of before every launch, and before any other thread's.
 //   B2G_KERNEL_SMEM(kernel, bytes): opt in to `bytes` of dynamic shared memory.
 //   B2G_KERNEL_MAX_SHARED(kernel) : ask for the largest shared-memory partition of the SM.  The split between L1 and shared
 //     memory is an SM-wide setting that cannot change while any CTA is resident; the kernels that run between or beside the
@@ -57,26 +58,23 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 //     (largest) partition as the GEMM, so that the GEMM, which needs nearly all of it, can start on an SM where one of them is
 //     still resident.  They stream and do not miss the L1.  The token permute kernels keep the default: they re-read rows
 //     through the L1 (a token's row is gathered once per route) and measured 10-25 % slower with the small L1.
-inline bool first_use_on_device(std::atomic<uint64_t>& seen) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return true;
-  const uint64_t bit = 1ull << dev;
-  return (seen.fetch_or(bit, std::memory_order_acq_rel) & bit) == 0;
+inline int current_device() {
+  int dev = -1;
+  return cudaGetDevice(&dev) == cudaSuccess ? dev : -1;
 }
+#define B2G_ONCE_PER_DEVICE(...)                                                                                    \
+  do {                                                                                                              \
+    static ::b2g::OncePerDevice once_;                                                                              \
+    const int once_rc_ = ::b2g::once_on(once_, ::b2g::current_device(), [&]() -> int { __VA_ARGS__; return 0; });     \
+    if (once_rc_) return once_rc_;                                                                                  \
+  } while (0)
 #define B2G_KERNEL_SMEM(kernel, bytes)                                                                              \
-  do {                                                                                                              \
-    static std::atomic<uint64_t> seen_{0};                                                                          \
-    if (::b2g::first_use_on_device(seen_)) {                                                                        \
+  B2G_ONCE_PER_DEVICE(                                                                                              \
       B2G_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes)));         \
-      B2G_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)); \
-    }                                                                                                               \
-  } while (0)
+      B2G_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)))
 #define B2G_KERNEL_MAX_SHARED(kernel)                                                                               \
-  do {                                                                                                              \
-    static std::atomic<uint64_t> seen_{0};                                                                          \
-    if (::b2g::first_use_on_device(seen_))                                                                          \
-      B2G_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)); \
-  } while (0)
+  B2G_ONCE_PER_DEVICE(                                                                                              \
+      B2G_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)))
 
 // Number of SMs of the current device (cached per device id).
 int sm_count();

@@ -1342,11 +1342,9 @@ static int resident_clusters(int cluster, int* out) {
 template <typename T, bool kPolicy>
 static int launch_pipe(const T* logits, int64_t ld, const policy::RowArgs& a, T* out, int64_t ld_out, int64_t rows, cudaStream_t s, bool* taken) {
   constexpr int N = 16 / sizeof(T);
-  static std::atomic<uint64_t> seen{0};
-  if (first_use_on_device(seen)) {
-    B2G_CUDA_OK(cudaFuncSetAttribute(policy::pipe_kernel<T, kPolicy>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSliceLimit));
-    B2G_CUDA_OK(cudaFuncSetAttribute(policy::pipe_kernel<T, kPolicy>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  }
+  B2G_ONCE_PER_DEVICE(
+      B2G_CUDA_OK(cudaFuncSetAttribute(policy::pipe_kernel<T, kPolicy>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSliceLimit));
+      B2G_CUDA_OK(cudaFuncSetAttribute(policy::pipe_kernel<T, kPolicy>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)));
   const int64_t need = (a.V + 2 * (N - 1)) / N;      // vectors of a row at its worst alignment
   int best = 0, best_resident = 0;
   for (int slots = policy::kMaxSlots; slots >= 1 && best == 0; --slots) {
