@@ -56,6 +56,11 @@ extern "C" {
 B2G_API const char* b2g_last_error(void);
 B2G_API int b2g_abi_version(void);
 
+/* *word = the address of the current device's own status word (int32, 0 until a kernel reports), for use as `status` in any
+ * entry.  It belongs to the library and lives as long; asking for it allocates nothing and is allowed while a stream is being captured.
+ * This entry has no counterpart in the reference. */
+B2G_API int b2g_status_word(void** word);
+
 /* Upload the IQ2_XXS magnitude table (256 rows x 8 bytes, HOST pointer) to the current device.
  * The table is third-party data owned by the gguf package; the caller reads it from there
  * (gguf.quants.IQ2_XXS.grid) and hands it in once per device before any IQ2_XXS call. */

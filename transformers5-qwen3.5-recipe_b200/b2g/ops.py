@@ -81,11 +81,24 @@ _status: dict[int, torch.Tensor] = {}
 _grid_done: set[int] = set()
 
 
+class _LibraryWord:
+    """The library's status word of the current device as torch takes foreign memory."""
+
+    def __init__(self) -> None:
+        address = C.c_void_p()
+        _lib.call("b2g_status_word", C.byref(address))
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address.value, False), "strides": None, "version": 2}
+
+
 def status_word(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    if idx not in _status:
-        _status[idx] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-    return _status[idx]
+    word = _status.get(idx)
+    if word is None:
+        # the library's memory and not a new tensor: in a first call that a graph captures that would be the graph's, whose replays
+        # would clear it; and one word for all, whoever comes first
+        with torch.cuda.device(idx):
+            word = _status.setdefault(idx, torch.as_tensor(_LibraryWord(), device=torch.device("cuda", idx)))
+    return word
 
 
 def check_status(device: Optional[torch.device] = None) -> None:
