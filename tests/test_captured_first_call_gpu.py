@@ -1,4 +1,5 @@
-"""GPU: an operator's first call in a process is one that a CUDA graph captures.  In a process of its own, which has called nothing before."""
+"""GPU: an operator's first call in a process is made in an unusual place: while a CUDA graph captures, or in inference mode.  In a
+process of its own, which has called nothing before."""
 import subprocess
 import sys
 
@@ -60,4 +61,35 @@ print("fine")
 
 def test_first_call_in_a_capture(cuda):
     r = subprocess.run([sys.executable, "-c", PROGRAM, str(PKG)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+INFERENCE = r"""
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from b2g import _lib, ops
+
+dev = torch.device("cuda", 0)
+target = torch.tensor([1, 50, 3], device=dev)
+with torch.inference_mode():
+    logp, _ = ops.token_logprobs(torch.zeros(3, 40, device=dev), target)
+for _ in range(2):
+    try:
+        ops.check_status()
+    except _lib.B2GError as e:
+        assert "902" in str(e)
+        ops.token_logprobs(torch.zeros(3, 40, device=dev), target)
+    else:
+        raise AssertionError("nothing was reported")
+try:
+    ops.check_status()
+except _lib.B2GError:
+    ops.check_status()
+print("fine")
+"""
+
+
+def test_first_call_in_inference_mode(cuda):
+    r = subprocess.run([sys.executable, "-c", INFERENCE, str(PKG)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]

@@ -96,7 +96,7 @@ def status_word(device: torch.device) -> torch.Tensor:
     if word is None:
         # the library's memory and not a new tensor: in a first call that a graph captures that would be the graph's, whose replays
         # would clear it; and one word for all, whoever comes first
-        with torch.cuda.device(idx):
+        with torch.inference_mode(False), torch.cuda.device(idx):
             word = _status.setdefault(idx, torch.as_tensor(_LibraryWord(), device=torch.device("cuda", idx)))
     return word
 
