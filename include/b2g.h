@@ -11,7 +11,7 @@
  *     ([rows, K / block * block_bytes]); quant types use the GGML ids (8 = Q8_0, 10 = Q2_K,
  *     11 = Q3_K, 12 = Q4_K, 13 = Q5_K, 14 = Q6_K, 16 = IQ2_XXS, 22 = IQ2_S).
  *   - `status` (nullable) is a device int32 the kernels write a non-zero code into when a bounded
- *     device-side wait runs out (1xx-5xx) or an input is out of range (901 receive buffer too small, 902 label
+ *     device-side wait runs out (1xx-6xx; the rank-side products, whose entries take no status, use b2g_status_word's) or an input is out of range (901 receive buffer too small, 902 label
  *     outside the vocabulary, 903 expert id outside [0, E), 904 expert offsets beyond the row count, 905 sequence offsets
  *     that decrease or leave the tokens); it is never written on a healthy run and only the first code is kept.
  *
@@ -185,6 +185,13 @@ B2G_API int b2g_lora_down(const void* x, const void* w, int w_is_cr, float scale
 B2G_API int64_t b2g_lora_wgrad_workspace_bytes(int64_t M, int64_t C);
 B2G_API int b2g_lora_wgrad(const void* s, const void* t, float scale, void* out, int transpose_out, void* workspace,
                    int64_t workspace_bytes, int64_t M, int64_t C, int r, void* stream);
+
+/* TEST HOOKS (no counterpart in the reference): b2g_lora_down of [r, C] weights (C a multiple of 64) and b2g_lora_wgrad whose loads
+ * are held back and whose bounded waits give up after 64 polls.  The wait for the first tile runs out, the kernel returns and
+ * b2g_status_word's word holds 602 or 612; the outputs are unspecified. */
+B2G_API int b2g_debug_stalled_lora_down(const void* x, const void* w, void* out_plain, int64_t M, int64_t C, int r, void* stream);
+B2G_API int b2g_debug_stalled_lora_wgrad(const void* s, const void* t, void* out, void* workspace, int64_t workspace_bytes, int64_t M,
+                                 int64_t C, int r, void* stream);
 
 /* The same factor gradient for callers that cannot allocate device memory (a plug-in inside another
  * framework's memory plan, a host that was handed only input and output buffers, a process whose pool is

@@ -33,6 +33,8 @@ SIGNATURES = {
     "b2g_lora_down": (_i32, [_vp, _vp, _i32, _f32, _vp, _vp, _i64, _i64, _i32, _vp]),
     "b2g_lora_wgrad_workspace_bytes": (_i64, [_i64, _i64]),
     "b2g_lora_wgrad": (_i32, [_vp, _vp, _f32, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "b2g_debug_stalled_lora_down": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "b2g_debug_stalled_lora_wgrad": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
     "b2g_lora_wgrad_static_max_bytes": (_i64, []),
     "b2g_lora_wgrad_static": (_i32, [_vp, _vp, _f32, _vp, _i32, _i64, _i64, _i32, _vp]),
     "b2g_router_topk": (_i32, [_vp, _i32, _vp, _i32, _vp, _i64, _i32, _i32, _vp]),

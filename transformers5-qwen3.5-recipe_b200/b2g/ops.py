@@ -103,7 +103,7 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 def check_status(device: Optional[torch.device] = None) -> None:
     """Synchronise and raise if any kernel on the device reported a problem through the status word: a bounded wait that
-    ran out (sites 1xx-5xx), a receive buffer too small for an expert-parallel exchange (901), a label outside the
+    ran out (sites 1xx-6xx), a receive buffer too small for an expert-parallel exchange (901), a label outside the
     vocabulary in a loss kernel (902), an expert id outside the expert count in the routing plan (903), expert
     offsets beyond the rows of a grouped product (904), sequence offsets that decrease or leave the tokens (905)."""
     devs = [device.index if device is not None and device.index is not None else torch.cuda.current_device()] \

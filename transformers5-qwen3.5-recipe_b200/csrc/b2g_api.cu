@@ -104,9 +104,6 @@ static int encode_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataTyp
   return 0;
 }
 
-// A status word per device for callers that have no memory of their own at hand, or none that outlives the call.
-__device__ int g_status_word = 0;
-
 // IQ2_XXS magnitude table, one copy per device that uploaded it.
 __device__ uint2 g_iq2xxs_grid[256];
 static bool g_grid_ready[64] = {false};
@@ -146,8 +143,7 @@ int b2g_abi_version(void) { return 1; }
 
 int b2g_status_word(void** word) {
   B2G_REQUIRE(word != nullptr, "status word: null pointer");
-  B2G_CUDA_OK(cudaGetSymbolAddress(word, b2g::g_status_word));
-  return 0;
+  return b2g::library_status(reinterpret_cast<int**>(word));
 }
 
 int b2g_set_iq2xxs_grid(const uint8_t* host_grid_256x8) {

@@ -78,6 +78,8 @@ inline int current_device() {
 
 // Number of SMs of the current device (cached per device id).
 int sm_count();
+// The current device's status word that belongs to the library (b2g_status_word).
+int library_status(int** out);
 
 // Driver entry point for tensor-map encoding, fetched through the runtime so that the
 // library has no link-time dependency on libcuda.
