@@ -234,8 +234,8 @@ B2G_API int b2g_route_experts(const void* logits, int64_t ld, int logits_dtype, 
                       int top_k, void* stream);
 
 /* Gradient of the weights with respect to the logits: grad_logits [T, E] contiguous, in the logits' type, from grad_weights and
- * the indices [T, top_k] of b2g_route_experts.  Every entry is written; ids outside [0, E) are skipped.  weights [T, top_k] must be
- * given and is not read: the gradient makes its own from the logits in 64 bits.
+ * the indices [T, top_k] of b2g_route_experts.  Every entry is written; ids outside [0, E) are skipped.  weights is not read and may be
+ * null: the gradient makes its own from the logits in 64 bits.
  * Covers the autograd of the gather / softmax / normalisation of fast_moe_ranking.py:273-316. */
 B2G_API int b2g_route_experts_bwd(const void* logits, int64_t ld, int logits_dtype, const float* grad_weights, const float* weights,
                           const int64_t* indices, int score_fn, int renormalize, float scaling, void* grad_logits, int64_t T, int E,

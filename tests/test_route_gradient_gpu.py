@@ -59,3 +59,27 @@ def test_rows_of_few_and_of_no_experts(cuda):
         (want,) = torch.autograd.grad(ref.weights(x64, idx.cpu()[:4], "softmax", renorm, 1.0), x64, cot.double()[:4])
         torch.testing.assert_close(grad.cpu().double()[:4], want, rtol=2.0 ** -21, atol=1e-14)
         assert bool((grad[4:] == 0).all())
+
+
+def test_weights_are_changed_in_place_like_any_tensor(cuda):
+    """Masking or scaling them in place changes nothing that the gradient needs."""
+    from b2g import ops
+    from fast_moe_ranking import route_experts
+
+    g = torch.Generator(device=cuda).manual_seed(5)
+    logits = torch.randn(300, 64, generator=g, device=cuda)
+    keep = (torch.rand(300, 6, generator=g, device=cuda) < 0.7).float()
+    cot = torch.randn(300, 6, generator=g, device=cuda)
+    for fn in ("softmax", "sigmoid", "sqrtsoftplus"):
+        for renorm in (True, False):
+            x = logits.clone().requires_grad_(True)
+            w, idx = route_experts(x, 6, score_function=fn, renormalize=renorm)
+            (want,) = torch.autograd.grad(w * keep, x, cot)
+            w, _ = route_experts(x, 6, score_function=fn, renormalize=renorm)
+            w.mul_(keep)
+            (got,) = torch.autograd.grad(w, x, cot)
+            assert torch.equal(got, want)
+            assert torch.equal(ops.route_experts_bwd(cot * keep, logits, None, idx, fn, renorm), want)
+            assert torch.equal(ops.route_experts_bwd(cot * keep, logits, w.detach(), idx, fn, renorm), want)
+    with pytest.raises(TypeError, match="grad_weights"):
+        ops.route_experts_bwd(None, logits, None, idx)

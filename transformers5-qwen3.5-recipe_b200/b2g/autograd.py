@@ -409,7 +409,7 @@ class _RouteExperts(torch.autograd.Function):
     def forward(ctx, logits, bias, choice, weighting):
         weights, indices = ops.route_experts(logits, choice[0], bias, weighting[0], *choice[1:], *weighting[1:])
         ctx.set_materialize_grads(False)         # no zeros for the ids' gradient, which does not exist
-        ctx.save_for_backward(logits, weights, indices)
+        ctx.save_for_backward(logits, indices)   # not the weights, which are the caller's to change
         ctx.weighting = weighting
         ctx.mark_non_differentiable(indices)
         return weights, indices
@@ -419,8 +419,8 @@ class _RouteExperts(torch.autograd.Function):
         _first_order_only("route_experts")
         if grad_weights is None:
             return None, None, None, None
-        logits, weights, indices = ctx.saved_tensors
-        return ops.route_experts_bwd(grad_weights.contiguous(), logits, weights, indices, *ctx.weighting), None, None, None
+        logits, indices = ctx.saved_tensors
+        return ops.route_experts_bwd(grad_weights.contiguous(), logits, None, indices, *ctx.weighting), None, None, None
 
 
 def route_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor] = None, score_function: str = "softmax", groups: int = 1,

@@ -652,18 +652,25 @@ def route_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor]
     return weights, indices
 
 
-def route_experts_bwd(grad_weights: torch.Tensor, logits: torch.Tensor, weights: torch.Tensor, indices: torch.Tensor,
+def route_experts_bwd(grad_weights: torch.Tensor, logits: torch.Tensor, weights: Optional[torch.Tensor], indices: torch.Tensor,
                       score_function: str = "softmax", renormalize: bool = True, scaling_factor: float = 1.0) -> torch.Tensor:
-    """Gradient ``[T, E]`` of the logits, in their type, from that of the weights; ``weights`` and ``indices`` are ``route_experts``' own."""
+    """Gradient ``[T, E]`` of the logits, in their type, from that of the weights; ``indices`` are ``route_experts``' own.  ``weights``
+    may be ``None``: the gradient makes its own from the logits in 64 bits."""
     t, e, ld, fn = _route_settings(logits, score_function, scaling_factor)
     _need(indices, torch.int64, "indices")
     if indices.dim() != 2 or indices.shape[0] != t:
         raise ValueError(f"indices must be [{t}, top_k], got {tuple(indices.shape)}")
+    if grad_weights is None:
+        raise TypeError("route_experts_bwd needs grad_weights")
     for name, x in (("weights", weights), ("grad_weights", grad_weights)):
+        if x is None:
+            continue
         _need(x, torch.float32, name)
         if x.shape != indices.shape:
             raise ValueError(f"{name} must be {tuple(indices.shape)}, got {tuple(x.shape)}")
-    if not logits.device == indices.device == weights.device == grad_weights.device:
+        if x.device != logits.device:
+            raise RuntimeError("route_experts_bwd: all tensors must be on the logits' device")
+    if logits.device != indices.device:
         raise RuntimeError("route_experts_bwd: all tensors must be on the logits' device")
     grad = torch.empty(t, e, dtype=logits.dtype, device=logits.device)
     _launch("b2g_route_experts_bwd", logits, _a(logits), ld, int(logits.dtype == torch.float32), _a(grad_weights), _a(weights), _a(indices), fn,

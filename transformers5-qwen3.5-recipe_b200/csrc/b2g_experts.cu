@@ -687,7 +687,7 @@ extern "C" int b2g_route_experts_bwd(const void* logits, int64_t ld, int logits_
                                      int top_k, void* stream) {
   if (int rc = check_route("route_experts_bwd", logits, ld, logits_dtype, score_fn, scaling, T, E, top_k)) return rc;
   if (T == 0) return 0;
-  B2G_REQUIRE(grad_weights && weights && indices && grad_logits, "route_experts_bwd: null pointer");
+  B2G_REQUIRE(grad_weights && indices && grad_logits, "route_experts_bwd: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // four tokens a warp where their choices fit its lanes and there are tokens for all SMs
   const int tokens = top_k <= 8 && T >= 8192 ? 4 : 1;
