@@ -126,7 +126,8 @@ B2G_API int b2g_cross_entropy_inplace(void* logits, int64_t ld, const int64_t* t
 /* Log-probabilities of the target tokens of rows of logits [rows, V] (row pitch ld elements; logits_dtype 0 = bf16, 1 = fp32):
  *   logp[row] = z[target] / temperature - log sum_i exp(z[i] / temperature)
  * in fp32 or fp64 (logp_dtype 0 | 1: sums over long sequences keep their digits in fp64).  stats[row] (4 floats, 16-byte
- * aligned) = {max z, 1 / sum_i exp((z[i] - max z) / temperature), 1 - p of the target, log-sum-exp} is what the gradient reads.  A row whose target is
+ * aligned) = {m, 1 / sum_i exp((z[i] - m) / temperature), 1 - p of the target, log-sum-exp}: a reference m near the row's maximum (wide
+ * rows: the largest of a sample, or of a part of the row) and the next two are what the gradient reads; the last is for the caller.  A row whose target is
  * ignore_index gets logp 0 whatever its logits are; a target outside [0, V) is reported (status 902) and treated the
  * same way.  -inf logits have probability zero; a live row that holds NaN or +inf, or nothing but -inf, gives NaN.
  * This entry has no counterpart in the reference (its losses are supervised only). */

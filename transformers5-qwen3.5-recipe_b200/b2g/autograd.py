@@ -425,7 +425,8 @@ class _RouteExperts(torch.autograd.Function):
 
 def route_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor] = None, score_function: str = "softmax", groups: int = 1,
                   top_groups: int = 1, group_experts: int = 1, renormalize: bool = True, scaling_factor: float = 1.0):
-    """``ops.route_experts`` whose weights carry the gradient to the logits (the bias enters the choice only and gets none)."""
+    """``ops.route_experts`` whose weights carry the gradient to the logits (the bias enters the choice only and gets none).  Groups are
+    compared by their best choice unless ``group_experts`` says 2, which is the default of ``fast_moe_ranking.route_experts``."""
     if not _carries_derivative(logits):
         return ops.route_experts(logits, top_k, bias, score_function, groups, top_groups, group_experts, renormalize, scaling_factor)
     return _RouteExperts.apply(logits, bias, (top_k, groups, top_groups, group_experts), (score_function, renormalize, scaling_factor))

@@ -396,8 +396,9 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, temperature: floa
                    dtype: torch.dtype = torch.float32):
     """``(logp [rows], stats [rows, 4])`` of bf16 or fp32 ``logits [rows, V]``: ``logp = z_y / temperature - log sum exp(z / temperature)``
     in fp32 or fp64 (a sum of many log-probabilities or of their differences keeps its digits in fp64), 0 where ``target`` is
-    ``ignore_index``.  ``stats`` (row maximum, reciprocal sum of exponentials, 1 - p of the target, log-sum-exp) is what
-    ``token_logprobs_bwd`` reads.  A target outside the vocabulary is reported through the status word (902) and ignored."""
+    ``ignore_index``.  ``stats`` is what ``token_logprobs_bwd`` reads: a reference ``m`` near the row's maximum (wide
+    rows: the largest of a sample, or of a part of the row), ``1 / sum exp((z - m) / temperature)``, 1 - p of the target; and the log-sum-exp, for the
+    caller.  A target outside the vocabulary is reported through the status word (902) and ignored."""
     rows, v, ld = _logit_rows(logits, "logits")
     if target is None:
         raise TypeError("token_logprobs needs targets")
@@ -641,8 +642,8 @@ def route_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor]
     """``(weights [T, top_k] fp32, indices [T, top_k] int64)`` of bf16 or fp32 ``logits [T, E]``, best expert first.
 
     Scores ``s`` (softmax, sigmoid or sqrt-softplus), choices ``c = s + bias`` compared in 64 bits (ties: the lower id), of the
-    ``groups`` equal groups only the ``top_groups`` with the largest sum of their ``group_experts`` best choices, weights from
-    the unbiased scores, optionally renormalised, times ``scaling_factor``."""
+    ``groups`` equal groups only the ``top_groups`` with the largest sum of their ``group_experts`` best choices (1 unless given, where
+    ``fast_moe_ranking.route_experts`` takes 2), weights from the unbiased scores, optionally renormalised, times ``scaling_factor``."""
     t, e, ld, fn = _route_settings(logits, score_function, scaling_factor)
     _row_vector(bias, logits, e, torch.float32, "bias")
     weights = torch.empty(t, int(top_k), dtype=torch.float32, device=logits.device)

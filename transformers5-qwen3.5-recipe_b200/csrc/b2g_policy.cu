@@ -14,8 +14,11 @@ namespace policy {
 
 constexpr float kLowest = -3.402823466e38f;
 // ex2.approx falls short by 4.9e-8 of its value on average (measured over 4 Mi arguments in [-20, 0], 3.7e-8 to 5.9e-8 in
-// the eight octiles of the fraction); a sum of many of them is that much too small.  The average is right for sums of many terms:
-// a rest of one or two terms keeps up to 1.2e-8 of it, and terms that ex2 gives exactly (equal logits: 2^0) are 4.9e-8 too large.
+// the eight octiles of the fraction); a sum of many of them is that much too small.  That is an average of what lies well below the
+// reference: by bins of the argument it is 5.0e-8 to 5.2e-8 from -32 to -2, 4.2e-8 to 5.4e-8 from -2 to -0.5, 1e-8 to 2e-8 from -0.5
+// to 0, and above 0 ex2 is 3.4e-8 too LARGE.  So it overdoes rows that are carried by terms at or above the reference: 2.5e-8 in
+// wide rows of normal logits of spread 2 (5e-8 at temperature 0.7), whose reference is the largest of a sample, and 4.9e-8 where
+// all logits are equal.  Rows with a dominant token, whose terms lie below, are off by 5e-9.
 constexpr double kEx2Shortfall = 4.9e-8;
 
 template <typename T>
@@ -239,7 +242,7 @@ struct RowArgs {
   // log-probabilities
   void* logp;          // fp32, or fp64 when logp64
   int logp64;
-  float4* stats;       // what the backward pass of the log-probabilities reads: m, 1/sum of exp((z - m)/tau), 1 - p of the target, lse
+  float4* stats;       // what the backward pass of the log-probabilities reads: m, 1/sum of exp((z - m)/tau), 1 - p of the target; and lse for the caller
   // policy loss
   const float *advantage, *old_logp, *ref_logp, *weight;
   float clip_low, clip_high, kl_coef;
@@ -728,7 +731,7 @@ __device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
 }
 
 template <bool kPolicy>
-constexpr int kPipeThreads = kWorkers + (kPolicy ? 64 : 96);      // so that two CTAs of either have 64 registers a thread
+constexpr int kPipeThreads = kWorkers + (kPolicy ? 64 : 96);      // two CTAs of either fit an SM's registers: 72 and 64 a thread
 
 template <typename T, bool kPolicy>
 __global__ void __launch_bounds__(kPipeThreads<kPolicy>, 2) pipe_kernel(const T* logits, int64_t ld, RowArgs a, T* out, int64_t ld_out, int64_t rows,
@@ -1300,7 +1303,8 @@ static policy::RowArgs row_args(const int64_t* target, int64_t V, int64_t ignore
 //     rounds * (slice + kRoundBytes),  rounds = rows / clusters that the device holds at once (of 296 places 8-CTA clusters fill
 //     264, 9-CTA clusters 270, 5-CTA clusters 280: the GPCs have 16 to 20 SMs), for the policy loss among those whose slices
 //     leave room for two slots.  kRoundBytes stands for what a row costs however short its slices are (12 KB against 8: policy
-//     loss of 301 x 32003 fp32 21.0 and 23.3 us, of 301 x 32003 bf16 14.6 and 17.9, of 150 x 64000 bf16 13.6 and 14.8).
+//     loss without temperature, old or reference log-probabilities of 301 x 32003 fp32 21.0 and 23.3 us, of 301 x 32003 bf16 14.6 and
+//     17.9, of 150 x 64000 bf16 13.6 and 14.8).
 //   Policy loss of rows too wide for that: one slot; beyond it wide_kernel.
 // Two CTAs share an SM's 228 KB: 1 KB each is the system's, and pipe_kernel's own arrays may take 5 KB beside the slices.
 constexpr int64_t kSmallRow = 36 * 1024, kSliceLimit = 108 * 1024, kRoundBytes = 12 * 1024;
